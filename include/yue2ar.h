@@ -256,6 +256,87 @@ int yar_sample_device_noalloc(yar_model *model, const uint16_t *logits, int64_t 
                               const int32_t *history, int n_history, int step, int phase,
                               uint64_t seed, int32_t *token, float *scores, void *stream);
 
+/* ---- Operators on a paged key/value cache in the caller's device memory -----------------
+ * No counterpart in the reference (its cache is one contiguous array per layer,
+ * native/src/ar.cpp:98-132). They compute what a session's own paths compute on its pool,
+ * for callers that hold a cache of the same layout themselves. Every pointer inside them is
+ * device memory of ONE device (any, whichever is current), except the page lists of
+ * yar_kv_copy_pages. A call checks its arguments (YAR_INVALID_INPUT), enqueues on `stream`
+ * (a cudaStream_t; NULL = default stream) and returns: it allocates nothing, waits for
+ * nothing and may be captured into a graph (make the first call on a device outside of a
+ * capture). There is no working memory beyond the arguments, so calls may overlap as far as
+ * their outputs are different memory. The calling thread's current device is unchanged.
+ * What only the device sees (a page index or a length out of range) reads nothing outside
+ * the pool: the positions concerned count as not visible, and a bit is added to *error
+ * (an int32 that the caller zeroes and reads; NULL = not reported). */
+enum {
+  YAR_KV_BAD_PAGE = 1,    /* a page index outside the pool among the positions a query sees */
+  YAR_KV_BAD_LENGTH = 2,  /* a length (count) beyond pages_per_row pages: cut to that */
+  YAR_KV_BAD_OFFSETS = 4, /* query offsets that decrease or pass n_queries: that row is skipped */
+  YAR_KV_EXPIRED = 64     /* a wait inside a kernel ran out: the outputs are not valid */
+};
+
+/* [layers][pages][2 (k, v)][kv_heads][page_tokens][head_dim] BF16 (a session's layout),
+ * 16-byte aligned. page_tokens: a power of two in [16, 4096]; head_dim: 64 or 128. Keys are
+ * cached as they enter the products (normalized and rotated). */
+typedef struct yar_kv_pool {
+  void *data;
+  int32_t layers, pages, kv_heads, page_tokens, head_dim;
+} yar_kv_pool;
+
+/* Row r's positions [i * page_tokens, (i + 1) * page_tokens) lie in page
+ * page_table[r * table_stride + i], i < pages_per_row; lengths[r] positions are cached
+ * (0 or less: none). Entries behind the length, and entries of pages that a window hides,
+ * are not read (freed pages may stand there as -1). Rows may share pages. */
+typedef struct yar_kv_rows {
+  const int32_t *page_table;
+  int64_t table_stride;
+  const int32_t *lengths;
+  int32_t rows, pages_per_row;
+} yar_kv_rows;
+
+/* Attention of one new token per row over its cached positions: for row r and each head,
+ * out = softmax(scale * q . k_j) v_j over the visible j. The query is the row's last cached
+ * position; j < lengths[r] is visible when window is 0, or j < sinks, or
+ * j >= lengths[r] - window (the last `window` positions, itself included, and the first
+ * `sinks`). A row that sees nothing gets zeros. q and out: BF16 [rows][heads][head_dim],
+ * row strides in elements (multiples of 8), not overlapping; heads: a multiple of kv_heads,
+ * at most 16 for each. FP32 scores, statistics and sums; one rounding of the result.
+ * max_length (0: the table's end): a bound of the lengths; it only chooses into how many
+ * parts a row's positions are split, longer rows stay right. */
+int yar_kv_attn_decode(const yar_kv_pool *pool, int layer, const yar_kv_rows *rows, const void *q, int64_t q_stride,
+                       int heads, void *out, int64_t out_stride, int window, int sinks, double scale, int max_length,
+                       int32_t *error, void *stream);
+
+/* The same for prompts: row r's queries are q[offsets[r]] .. q[offsets[r + 1] - 1] (int32
+ * [rows + 1], ascending, at most n_queries), the last n of its lengths[r] cached positions
+ * (their keys and values are in the cache already); the query at position p sees j <= p when
+ * window is 0, or j < sinks, or j > p - window. A query before position 0 (more queries than
+ * lengths[r]) sees nothing and gets zeros. q and out: [n_queries][heads][head_dim]; out rows
+ * in front of offsets[0] or behind offsets[rows] are left as they were. */
+int yar_kv_attn_prefill(const yar_kv_pool *pool, int layer, const yar_kv_rows *rows, const int32_t *offsets,
+                        int64_t n_queries, const void *q, int64_t q_stride, int heads, void *out, int64_t out_stride,
+                        int window, int sinks, double scale, int32_t *error, void *stream);
+
+/* Copy page src_pages[i] of `src` to page dst_pages[i] of `dst`, i < n, in every layer: the
+ * first tokens[i] positions of K and V (tokens NULL: the whole page). The pools are one, or
+ * two that differ in their number of pages at most. The lists are HOST arrays, read before
+ * the call returns. A page may be the source of many copies (a fork); a destination that is
+ * listed twice, or is a source in the same pool, is refused. */
+int yar_kv_copy_pages(const yar_kv_pool *src, const yar_kv_pool *dst, const int32_t *src_pages,
+                      const int32_t *dst_pages, const int32_t *tokens, int n, void *stream);
+
+/* Move the used pages to the front of the pool. Used are the U pages that stand among the
+ * first counts[r] entries of a row of the table (-1 is no page; pages may be shared). The
+ * k-th used page with index >= U moves to the k-th unused page with index < U, both in
+ * ascending order; the pages behind U keep their bytes. new_table (the same table, or
+ * another that does not overlap it) gets every entry renamed; entries behind counts[r] are
+ * copied. remap[pages]: each used page's new index, -1 for the others. used[1]: U. work: int32
+ * [1 + 2 * pages], scratch. At most 2**20 pages. */
+int yar_kv_compact(const yar_kv_pool *pool, const int32_t *page_table, int64_t table_stride, int rows,
+                   int pages_per_row, const int32_t *counts, int32_t *new_table, int64_t new_stride, int32_t *remap,
+                   int32_t *used, int32_t *work, int32_t *error, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

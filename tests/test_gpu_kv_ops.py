@@ -1,0 +1,464 @@
+"""The paged-cache operators against a plain implementation in 64 bits.
+
+Attention tolerance, per output value. Let A = sum_j p_j |v_j| (p: the exact weights) and
+S = max_j scale sum_d |q_d k_jd|.
+* products of BF16 values are exact in FP32; a sum of D of them in FP32, in any order, and its
+  scaling are off by at most (D + 2) 2^-24 S, and forming the exponent by 4 x 2^-24 S more, so
+  each weight by a factor within exp(+-2 (D + 6) 2^-24 S); the weights' sum too (doubled);
+* the exponential itself, and the sums over the keys in FP32 (partial sums of positive terms,
+  rescaled per block): 2^-18 covers 2^-22 per exponential and 64 rounded blocks;
+* the weights enter the second product as BF16 (off by 2^-8 each at most) in the prompt form,
+  as two BF16 parts (2^-16) in the single-token form;
+* the result is rounded to BF16 once: 2^-8 of it.
+"""
+import math
+
+import numpy as np
+import pytest
+
+from tests.conftest import load_package
+
+pytestmark = pytest.mark.gpu
+
+P_ROUND = {"decode": 2.0 ** -16, "prefill": 2.0 ** -8}
+
+
+@pytest.fixture(scope="module")
+def yar():
+    return load_package()
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch
+    return torch
+
+
+def visible(length, pos, window, sinks):
+    """Positions that a query at `pos` sees of `length` cached ones, by the definition."""
+    j = np.arange(max(0, min(length, pos + 1)))
+    return j[(j < sinks) | (j > pos - window)] if window else j
+
+
+class Cache:
+    """A pool of random values in shuffled pages: every value that no query may see (other
+    layers, unlisted pages, slots behind a row's length) is NaN or infinite."""
+
+    def __init__(self, torch, lens, kv=2, dim=64, page=16, seed=0, spread=1.0, window=0, sinks=0, first_pos=None):
+        rng = np.random.default_rng(seed)
+        self.lens, self.kv, self.dim, self.page = lens, kv, dim, page
+        per = max(1, max((x + page - 1) // page for x in lens))
+        pages = per * len(lens) + 3
+        data = np.full((2, pages, 2, kv, page, dim), np.nan, np.float32)
+        data[0] = np.inf
+        perm = rng.permutation(pages)
+        table = np.full((len(lens), per), -1, np.int64)
+        self.k, self.v = [], []
+        used = 0
+        for r, n in enumerate(lens):
+            k = rng.standard_normal((kv, max(n, 0), dim)).astype(np.float32) * spread
+            v = rng.standard_normal((kv, max(n, 0), dim)).astype(np.float32)
+            k, v = (torch.from_numpy(x).bfloat16().float().numpy() for x in (k, v))
+            self.k.append(k.astype(np.float64)), self.v.append(v.astype(np.float64))
+            first = n - 1 if first_pos is None else first_pos[r]
+            hidden = max(0, first - window + 1) if window else 0  # positions before this one: only sinks are seen
+            for i in range((n + page - 1) // page):
+                a, b = i * page, min(n, (i + 1) * page)
+                if a >= sinks and b <= hidden:
+                    continue  # a freed page: -1 in the table
+                table[r, i] = perm[used]
+                used += 1
+                data[1, table[r, i], 0, :, :b - a] = k[:, a:b]
+                data[1, table[r, i], 1, :, :b - a] = v[:, a:b]
+        self.pool = torch.from_numpy(data).bfloat16().cuda()
+        self.table = torch.from_numpy(table.astype(np.int32)).cuda()
+        self.lengths = torch.tensor(lens, dtype=torch.int32, device="cuda")
+
+    def attend(self, q, row, pos, scale, window, sinks, round_p):
+        """(result, tolerance) [heads][dim] of one query in 64 bits."""
+        heads = q.shape[0]
+        group = heads // self.kv
+        j = visible(self.lens[row], pos, window, sinks)
+        out, tol = np.zeros(q.shape), np.zeros(q.shape)
+        if j.size == 0:
+            return out, tol
+        for h in range(heads):
+            k, v = self.k[row][h // group][j], self.v[row][h // group][j]
+            s = scale * (k @ q[h])
+            big = (scale * (np.abs(k) @ np.abs(q[h]))).max()
+            p = np.exp(s - s.max())
+            p /= p.sum()
+            out[h] = p @ v
+            a = p @ np.abs(v)
+            off = math.expm1(4 * (self.dim + 6) * 2.0 ** -24 * big) + 2.0 ** -18 + round_p
+            tol[h] = off * a * (1 + 2.0 ** -8) + 2.0 ** -8 * np.abs(out[h]) + 1e-30
+        return out, tol
+
+
+def check(torch, got, want, tol):
+    got = got.double().cpu().numpy()
+    assert np.isfinite(got).all()
+    bad = np.abs(got - want) > tol
+    assert not bad.any(), (int(bad.sum()), float((np.abs(got - want) / tol).max()))
+
+
+def queries(torch, n, heads, dim, seed, spread=1.0):
+    rng = np.random.default_rng(seed + 1000)
+    q = torch.from_numpy((rng.standard_normal((n, heads, dim)) * spread).astype(np.float32)).bfloat16()
+    return q.cuda(), q.double().numpy()
+
+
+DECODE = [
+    # lens, kv, group, dim, page, window, sinks
+    ([1], 2, 2, 64, 16, 0, 0), ([1, 2, 0, 5], 8, 2, 128, 256, 0, 0), ([15, 16, 17], 1, 1, 64, 16, 0, 0),
+    ([63, 64, 65, 127, 128, 129], 2, 2, 128, 64, 0, 0), ([255, 256, 257], 8, 2, 128, 256, 0, 0),
+    ([1000, 0, 33, 777], 2, 7, 64, 32, 0, 0), ([513], 8, 2, 128, 256, 0, 0), ([3000], 1, 16, 128, 128, 0, 0),
+    ([4100, 1], 4, 3, 128, 16, 0, 0), ([700, 20, 64, 1], 2, 8, 64, 16, 1, 0), ([700, 20, 64, 1], 2, 4, 64, 16, 17, 3),
+    ([900, 300, 0, 301, 299], 2, 2, 128, 256, 300, 4), ([2000, 1999], 1, 9, 128, 32, 100, 70),
+    ([500], 2, 2, 64, 16, 64, 0), ([600, 601], 2, 2, 128, 4096, 37, 600), ([90] * 40, 2, 1, 64, 64, 50, 1),
+    ([9001], 2, 2, 128, 256, 2048, 4),
+]
+
+
+@pytest.mark.parametrize("lens,kv,group,dim,page,window,sinks", DECODE)
+def test_decode_matches_the_definition(yar, torch, lens, kv, group, dim, page, window, sinks):
+    c = Cache(torch, lens, kv, dim, page, seed=len(lens) + lens[0], window=window, sinks=sinks)
+    q, q64 = queries(torch, len(lens), kv * group, dim, lens[0])
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    got = yar.kv_attn_decode(c.pool, 1, c.table, c.lengths, q, window=window, sinks=sinks, error=err)
+    pairs = [c.attend(q64[r], r, n - 1, dim ** -0.5, window, sinks, P_ROUND["decode"]) for r, n in enumerate(lens)]
+    check(torch, got, np.stack([p[0] for p in pairs]), np.stack([p[1] for p in pairs]))
+    assert err.item() == 0
+    # A bound of the lengths changes the split, not the result beyond rounding.
+    hint = yar.kv_attn_decode(c.pool, 1, c.table, c.lengths, q, window=window, sinks=sinks, max_length=max(1, max(lens)))
+    check(torch, hint, np.stack([p[0] for p in pairs]), np.stack([p[1] for p in pairs]))
+    hint = yar.kv_attn_decode(c.pool, 1, c.table, c.lengths, q, window=window, sinks=sinks, max_length=1)
+    check(torch, hint, np.stack([p[0] for p in pairs]), np.stack([p[1] for p in pairs]))
+
+
+PREFILL = [
+    # queries per row, cached before them, kv, group, dim, page, window, sinks
+    ([1], [0], 2, 2, 64, 16, 0, 0), ([77], [0], 2, 2, 64, 16, 0, 0), ([5, 0, 130], [0, 9, 3], 1, 1, 128, 256, 0, 0),
+    ([127, 128, 129], [1, 0, 500], 2, 2, 128, 64, 0, 0), ([300], [700], 8, 2, 128, 256, 0, 0),
+    ([64, 1, 200], [0, 1000, 63], 2, 3, 64, 32, 0, 0), ([260], [0], 1, 8, 128, 16, 0, 0),
+    ([200, 40], [0, 400], 2, 2, 128, 256, 1, 0), ([200, 40], [0, 400], 2, 2, 64, 16, 17, 3),
+    ([600], [0], 2, 2, 128, 256, 128, 4), ([150, 257], [900, 1], 2, 1, 128, 32, 100, 70),
+    ([333], [1111], 1, 4, 64, 128, 200, 130), ([500], [0], 2, 7, 64, 64, 300, 0), ([520], [2000], 2, 2, 128, 256, 512, 4),
+]
+
+
+@pytest.mark.parametrize("ns,before,kv,group,dim,page,window,sinks", PREFILL)
+def test_prefill_matches_the_definition(yar, torch, ns, before, kv, group, dim, page, window, sinks):
+    lens = [n + b for n, b in zip(ns, before)]
+    c = Cache(torch, lens, kv, dim, page, seed=lens[0], window=window, sinks=sinks, first_pos=before)
+    offs = np.concatenate([[0], np.cumsum(ns)])
+    q, q64 = queries(torch, int(offs[-1]), kv * group, dim, lens[0])
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    got = yar.kv_attn_prefill(c.pool, 1, c.table, c.lengths, torch.tensor(offs, dtype=torch.int32, device="cuda"), q,
+                              window=window, sinks=sinks, error=err)
+    want, tol = np.zeros(q64.shape), np.zeros(q64.shape)
+    for r, (n, b) in enumerate(zip(ns, before)):
+        for i in range(n):
+            t = offs[r] + i
+            want[t], tol[t] = c.attend(q64[t], r, b + i, dim ** -0.5, window, sinks, P_ROUND["prefill"])
+    check(torch, got, want, tol)
+    assert err.item() == 0
+
+
+def test_large_scores_and_a_given_scale(yar, torch):
+    """Scores far from zero (a running maximum that moves, weights that vanish)."""
+    for dim, spread, scale in ((128, 6.0, None), (64, 3.0, 0.7)):
+        lens = [300, 41]
+        c = Cache(torch, lens, 2, dim, 16, seed=3, spread=spread)
+        q, q64 = queries(torch, 2, 4, dim, 5, spread)
+        s = dim ** -0.5 if scale is None else scale
+        got = yar.kv_attn_decode(c.pool, 1, c.table, c.lengths, q, scale=scale)
+        pairs = [c.attend(q64[r], r, n - 1, s, 0, 0, P_ROUND["decode"]) for r, n in enumerate(lens)]
+        check(torch, got, np.stack([p[0] for p in pairs]), np.stack([p[1] for p in pairs]))
+        q, q64 = queries(torch, 60, 4, dim, 6, spread)
+        got = yar.kv_attn_prefill(c.pool, 1, c.table, c.lengths, torch.tensor([0, 40, 60], dtype=torch.int32).cuda(), q,
+                                  scale=scale)
+        pairs = [c.attend(q64[t], 0 if t < 40 else 1, 260 + t if t < 40 else 21 + t - 40, s, 0, 0, P_ROUND["prefill"])
+                 for t in range(60)]
+        check(torch, got, np.stack([p[0] for p in pairs]), np.stack([p[1] for p in pairs]))
+
+
+def test_strided_tensors_and_rows_behind_the_last(yar, torch):
+    c = Cache(torch, [40, 90], 2, 64, 16, seed=8)
+    wide = torch.randn(6, 9, 64, device="cuda").bfloat16()
+    q = wide[:, 2:6]  # row stride 9 x 64
+    out_wide = torch.full((6, 6, 64), 7.0, device="cuda", dtype=torch.bfloat16)
+    table = torch.full((2, 11), 1 << 30, dtype=torch.int32, device="cuda")
+    table[:, :c.table.shape[1]] = c.table
+    tab = table[:, :c.table.shape[1]]
+    dense = yar.kv_attn_decode(c.pool, 1, c.table, c.lengths, q[:2].contiguous())
+    yar.kv_attn_decode(c.pool, 1, tab, c.lengths, q[:2], out=out_wide[:2, 1:5])
+    assert torch.equal(out_wide[:2, 1:5], dense)
+    assert (out_wide[2:] == 7).all() and (out_wide[:, 0] == 7).all() and (out_wide[:, 5] == 7).all()
+    # Queries 1..4 belong to the two rows; 0 and 5 to none: left as they were.
+    offs = torch.tensor([1, 3, 5], dtype=torch.int32, device="cuda")
+    dense = yar.kv_attn_prefill(c.pool, 1, c.table, c.lengths, torch.tensor([0, 2, 4], dtype=torch.int32).cuda(),
+                                q[1:5].contiguous())
+    out_wide.fill_(7.0)
+    yar.kv_attn_prefill(c.pool, 1, tab, c.lengths, offs, q, out=out_wide[:, 1:5])
+    assert torch.equal(out_wide[1:5, 1:5], dense)
+    assert (out_wide[0] == 7).all() and (out_wide[5] == 7).all()
+    assert (out_wide[:, 0] == 7).all() and (out_wide[:, 5] == 7).all()
+
+
+def test_queries_before_the_first_position_see_nothing(yar, torch):
+    c = Cache(torch, [3, 0], 2, 64, 16, seed=4)
+    q, q64 = queries(torch, 9, 4, 64, 2)
+    got = yar.kv_attn_prefill(c.pool, 1, c.table, c.lengths, torch.tensor([0, 5, 9], dtype=torch.int32).cuda(), q)
+    assert (got[:2] == 0).all() and (got[5:] == 0).all()
+    for i in range(2, 5):
+        want, tol = c.attend(q64[i], 0, i - 2, 0.125, 0, 0, P_ROUND["prefill"])
+        check(torch, got[i], want, tol)
+
+
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 256)])
+def test_bad_pages_lengths_and_offsets_are_reported_and_not_followed(yar, torch, dim, page):
+    n = 3 * page
+    c = Cache(torch, [n, n], 2, dim, page, seed=11)
+    q, q64 = queries(torch, 2, 4, dim, 9)
+    good = yar.kv_attn_decode(c.pool, 1, c.table, c.lengths, q)
+    for bad in (-1, -5, c.pool.shape[1], 2 ** 31 - 1):
+        table = c.table.clone()
+        table[0, 1] = bad
+        err = torch.zeros(1, dtype=torch.int32, device="cuda")
+        got = yar.kv_attn_decode(c.pool, 1, table, c.lengths, q, error=err)
+        assert err.item() == 1 and torch.equal(got[1], good[1])
+        # The bad page's positions count as not visible.
+        k, v = c.k[0], c.v[0]
+        c.k[0], c.v[0] = (np.concatenate([x[:, :page], x[:, 2 * page:]], axis=1) for x in (k, v))
+        c.lens[0] = 2 * page
+        want, tol = c.attend(q64[0], 0, 2 * page - 1, dim ** -0.5, 0, 0, P_ROUND["decode"])
+        _, tol_pre = c.attend(q64[0], 0, 2 * page - 1, dim ** -0.5, 0, 0, P_ROUND["prefill"])
+        c.k[0], c.v[0], c.lens[0] = k, v, n
+        check(torch, got[0], want, tol)
+        err.zero_()
+        offs = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+        pre = yar.kv_attn_prefill(c.pool, 1, table, c.lengths, offs, q, error=err)
+        assert err.item() == 1
+        check(torch, pre[0], want, tol_pre)
+    # A length beyond the table is cut to the table's positions.
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    long = torch.tensor([n + 1, 2 ** 31 - 1], dtype=torch.int32, device="cuda")
+    assert torch.equal(yar.kv_attn_decode(c.pool, 1, c.table, long, q, error=err), good)
+    assert err.item() == 2
+    err.zero_()
+    pre = yar.kv_attn_prefill(c.pool, 1, c.table, c.lengths, torch.tensor([0, 1, 2], dtype=torch.int32).cuda(), q)
+    assert torch.equal(yar.kv_attn_prefill(c.pool, 1, c.table, long, torch.tensor([0, 1, 2], dtype=torch.int32).cuda(),
+                                           q, error=err), pre)
+    assert err.item() == 2
+    # Negative lengths: nothing cached.
+    neg = torch.tensor([-3, -2 ** 31], dtype=torch.int32, device="cuda")
+    assert (yar.kv_attn_decode(c.pool, 1, c.table, neg, q) == 0).all()
+    # Offsets that decrease or pass the queries: those rows are skipped.
+    for offs, kept in (([0, 1, 3], [0]), ([1, 0, 2], []), ([-1, 1, 2], [1])):
+        err.zero_()
+        out = torch.full_like(q, 7.0)
+        yar.kv_attn_prefill(c.pool, 1, c.table, c.lengths, torch.tensor(offs, dtype=torch.int32).cuda(), q, out=out,
+                            error=err)
+        assert err.item() == 4, offs
+        if kept:
+            for t in range(2):
+                assert torch.equal(out[t], pre[t] if t in kept else torch.full_like(out[t], 7.0)), (offs, t)
+
+
+def test_layers_and_shared_pages(yar, torch):
+    """Rows with the same table give the same bits, on either layer."""
+    c = Cache(torch, [200], 2, 128, 64, seed=5)
+    pool = c.pool.clone()
+    pool[0] = pool[1]
+    q, _ = queries(torch, 1, 4, 128, 1)
+    table, lens = c.table.expand(3, -1).contiguous(), c.lengths.expand(3).contiguous()
+    got = yar.kv_attn_decode(pool, 0, table, lens, q.expand(3, -1, -1).contiguous())
+    one = yar.kv_attn_decode(pool, 1, c.table, c.lengths, q, max_length=0)
+    for r in range(3):
+        assert torch.equal(got[r], got[0])
+    assert (got[0].float() - one[0].float()).abs().max() <= 2.0 ** -7 * one.float().abs().max()
+
+
+def test_captured_calls_on_another_stream_replay(yar, torch):
+    """Both forms, copies and compaction captured into one graph on a side stream; replayed on
+    new inputs in the same buffers, two graphs interleaved."""
+    c = Cache(torch, [150, 60], 2, 64, 16, seed=12)
+    spare = torch.cat([c.pool, torch.zeros_like(c.pool)], dim=1).contiguous()
+    q, _ = queries(torch, 2, 4, 64, 3)
+    offs = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+    n = c.pool.shape[1]
+    src = [int(p) for p in c.table[0].tolist() if p >= 0][:2]
+    yar.kv_attn_decode(spare, 1, c.table, c.lengths, q)  # first calls outside of the capture
+    yar.kv_attn_prefill(spare, 1, c.table, c.lengths, offs, q)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for window in (0, 20):
+        side = torch.cuda.Stream()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            a = yar.kv_attn_decode(spare, 1, c.table, c.lengths, q, window=window, sinks=2)
+            b = yar.kv_attn_prefill(spare, 1, c.table, c.lengths, offs, q, window=window, sinks=2)
+            yar.kv_copy_pages(spare, src, [n, n + 1])
+        graphs.append(g), outs.append((a, b))
+    for seed in (1, 2):
+        q.copy_(queries(torch, 2, 4, 64, 40 + seed)[0])
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for (a, b), window in zip(outs, (0, 20)):
+            assert torch.equal(a, yar.kv_attn_decode(spare, 1, c.table, c.lengths, q, window=window, sinks=2))
+            assert torch.equal(b, yar.kv_attn_prefill(spare, 1, c.table, c.lengths, offs, q, window=window, sinks=2))
+        assert torch.equal(spare[:, n:n + 2].view(torch.int16), spare[:, src].view(torch.int16))
+
+
+def test_calls_on_two_streams_at_once(yar, torch):
+    c = Cache(torch, [1500, 700, 900], 2, 128, 64, seed=13)
+    q, _ = queries(torch, 3, 4, 128, 4)
+    want = yar.kv_attn_decode(c.pool, 1, c.table, c.lengths, q)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = [[], []]
+    for _ in range(20):
+        for s, o in zip(streams, outs):
+            with torch.cuda.stream(s):
+                o.append(yar.kv_attn_decode(c.pool, 1, c.table, c.lengths, q))
+    torch.cuda.synchronize()
+    for o in outs[0] + outs[1]:
+        assert torch.equal(o, want)
+
+
+def test_host_memory_is_refused(yar, torch):
+    c = Cache(torch, [20], 2, 64, 16, seed=1)
+    q, _ = queries(torch, 1, 4, 64, 1)
+    with pytest.raises(ValueError):
+        yar.kv_attn_decode(c.pool, 1, c.table, c.lengths, q.cpu())
+    host = torch.zeros(1, 4, 64, dtype=torch.bfloat16)
+    st = yar.lib.yar_kv_attn_decode(yar._kv_pool(c.pool), 1, yar._kv_rows(c.table, c.lengths), host.data_ptr(), 256, 4,
+                                    q.data_ptr(), 256, 0, 0, 0.125, 0, None, None)
+    assert st == yar.INVALID_INPUT and b"device memory" in yar.lib.yar_last_error()
+
+
+@pytest.mark.parametrize("layers,kv,dim,page,pairs", [(1, 1, 64, 16, 1), (3, 2, 128, 64, 5), (2, 8, 128, 256, 3),
+                                                       (2, 1, 64, 16, 300)])
+def test_copy_pages(yar, torch, layers, kv, dim, page, pairs):
+    g = torch.Generator().manual_seed(pairs)
+    pages = 2 * pairs + 3
+    pool = torch.randint(-32768, 32767, (layers, pages, 2, kv, page, dim), generator=g, dtype=torch.int32)
+    pool = pool.to(torch.int16).cuda().view(torch.bfloat16)  # any bits, NaN patterns among them
+    perm = torch.randperm(pages, generator=g).tolist()
+    dst = perm[:pairs]
+    src = [perm[pairs + i // 2] for i in range(pairs)]  # a page may be copied to several places
+    tokens = [(i * 7) % (page + 1) for i in range(pairs)]
+    for tok in (None, tokens):
+        want = pool.view(torch.int16).clone()
+        for i, (a, b) in enumerate(zip(src, dst)):
+            t = page if tok is None else tok[i]
+            want[:, b, :, :, :t] = want[:, a, :, :, :t]
+        got = pool.clone()
+        yar.kv_copy_pages(got, src, dst, tokens=tok)
+        assert torch.equal(got.view(torch.int16), want)
+    # Into a pool with another number of pages.
+    other = torch.zeros((layers, pairs + 1, 2, kv, page, dim), dtype=torch.bfloat16, device="cuda")
+    yar.kv_copy_pages(pool, src, list(range(pairs, 0, -1)), dst_pool=other)
+    for i, a in enumerate(src):
+        assert torch.equal(other[:, pairs - i].view(torch.int16), pool[:, a].view(torch.int16))
+    assert (other[:, 0] == 0).all()
+
+
+def plan(pages, table, counts):
+    """The renamed table, remap, used count and moves by the definition."""
+    used = sorted({int(p) for row, n in zip(table, counts) for p in row[:max(0, n)] if 0 <= p < pages})
+    u = len(used)
+    holes = [p for p in range(u) if p not in set(used)]
+    moves = dict(zip([p for p in used if p >= u], holes))
+    remap = np.full(pages, -1, np.int32)
+    for p in used:
+        remap[p] = moves.get(p, p)
+    new = table.copy()
+    for r, n in enumerate(counts):
+        for i in range(max(0, min(n, table.shape[1]))):
+            if 0 <= table[r, i] < pages:
+                new[r, i] = remap[table[r, i]]
+    return new, remap, u, moves
+
+
+@pytest.mark.parametrize("pages,rows,per_row,kv,dim,page", [(5, 1, 3, 1, 64, 16), (64, 4, 9, 2, 64, 16),
+                                                              (33, 5, 7, 8, 128, 64), (2500, 40, 30, 1, 64, 16),
+                                                              (70000, 3, 50, 1, 64, 16), (40, 0, 1, 2, 64, 16)])
+def test_compaction(yar, torch, pages, rows, per_row, kv, dim, page):
+    rng = np.random.default_rng(pages)
+    layers = 2 if pages < 10000 else 1
+    pool = torch.randint(-32768, 32767, (layers, pages, 2, kv, page, dim), dtype=torch.int32, device="cuda")
+    pool = pool.to(torch.int16).view(torch.bfloat16)
+    table = rng.choice(pages, size=(rows, per_row), replace=rows * per_row > pages).astype(np.int32)
+    table[rng.random(table.shape) < 0.2] = -1  # freed pages
+    if rows > 1:
+        table[1, :2] = table[0, :2]  # shared pages
+    counts = rng.integers(0, per_row + 1, rows).astype(np.int32)
+    new, remap, u, moves = plan(pages, table, counts)
+    d = lambda x: torch.from_numpy(x).cuda()  # noqa: E731
+    for in_place in (False, True):
+        got, t, err = pool.clone(), d(table), torch.zeros(1, dtype=torch.int32, device="cuda")
+        out, rm, used = yar.kv_compact(got, t, d(counts), out=t if in_place else None, error=err)
+        assert err.item() == 0 and used.item() == u
+        np.testing.assert_array_equal(rm.cpu().numpy(), remap)
+        np.testing.assert_array_equal(out.cpu().numpy(), new)
+        want = pool.view(torch.int16).clone()
+        for a, b in moves.items():
+            want[:, b] = want[:, a]
+        assert torch.equal(got.view(torch.int16), want)
+        if not in_place:
+            assert torch.equal(t, d(table))
+
+
+def test_compaction_reports_bad_entries_and_leaves_them(yar, torch):
+    pool = torch.zeros((1, 8, 2, 1, 16, 64), dtype=torch.bfloat16, device="cuda")
+    table = torch.tensor([[7, 8, -2, 2], [6, 2 ** 31 - 1, -1, 9]], dtype=torch.int32, device="cuda")
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out, remap, used = yar.kv_compact(pool, table, torch.tensor([4, 1], dtype=torch.int32, device="cuda"), error=err)
+    assert err.item() == 1 and used.item() == 3
+    assert out.tolist() == [[1, 8, -2, 2], [0, 2 ** 31 - 1, -1, 9]]
+    assert remap.tolist() == [-1, -1, 2, -1, -1, -1, 0, 1]
+    err.zero_()
+    out, _, used = yar.kv_compact(pool, table, torch.tensor([-1, 99], dtype=torch.int32, device="cuda"), error=err)
+    assert err.item() == 3 and used.item() == 1 and out.tolist()[0] == table.tolist()[0]
+
+
+def test_forked_rows_attend_alike_and_survive_compaction(yar, torch):
+    """A run as a server makes it: a prompt's row forked (full pages shared, the last page
+    copied), one fork's window moved on (pages freed), the pool compacted: every attention
+    over the renamed table gives the bits from before."""
+    c = Cache(torch, [100], 2, 128, 16, seed=21)
+    per = c.table.shape[1] + 2
+    free = [p for p in range(c.pool.shape[1]) if p not in c.table[0].tolist()]
+    pool = torch.cat([c.pool, torch.zeros_like(c.pool)], dim=1).contiguous()
+    free += list(range(c.pool.shape[1], pool.shape[1]))
+    first = c.table[0].tolist()
+    table = torch.full((2, per), -1, dtype=torch.int32)
+    table[0, :len(first)] = torch.tensor(first)
+    table[1, :len(first)] = torch.tensor(first)
+    fresh = free[-1]
+    yar.kv_copy_pages(pool, [first[6]], [fresh], tokens=[4])  # 100 = 6 x 16 + 4
+    table[1, 6] = fresh
+    table = table.cuda()
+    lens = torch.tensor([100, 100], dtype=torch.int32, device="cuda")
+    q, _ = queries(torch, 1, 4, 128, 1)
+    q = q.expand(2, -1, -1).contiguous()
+    both = yar.kv_attn_decode(pool, 1, table, lens, q)
+    assert torch.equal(both[0], both[1])
+    seen = yar.kv_attn_decode(pool, 1, table, lens, q, window=30, sinks=3)
+    offs = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+    pre = yar.kv_attn_prefill(pool, 1, table, lens, offs, q, window=30, sinks=3)
+    # Row 0 ends; row 1 frees what its window hides (positions 3..69: pages 1..3).
+    table[0] = -1
+    table[1, 1:4] = -1
+    counts = torch.tensor([0, 7], dtype=torch.int32, device="cuda")
+    new, remap, used = yar.kv_compact(pool, table, counts)
+    assert used.item() == 4 and sorted(p for p in new[1].tolist() if p >= 0) == [0, 1, 2, 3]
+    small = pool[:, :4].contiguous()
+    lens = torch.tensor([0, 100], dtype=torch.int32, device="cuda")
+    again = yar.kv_attn_decode(small, 1, new, lens, q, window=30, sinks=3)
+    assert torch.equal(again[1], seen[1]) and (again[0] == 0).all()
+    offs = torch.tensor([0, 0, 1], dtype=torch.int32, device="cuda")
+    assert torch.equal(yar.kv_attn_prefill(small, 1, new, lens, offs, q[:1].contiguous(), window=30, sinks=3)[0], pre[1])

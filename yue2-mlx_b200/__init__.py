@@ -52,6 +52,16 @@ class _Sampling(ctypes.Structure):
                 ("min_tokens", ctypes.c_int32), ("max_tokens", ctypes.c_int32)]
 
 
+class _KvPool(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("layers", ctypes.c_int32), ("pages", ctypes.c_int32),
+                ("kv_heads", ctypes.c_int32), ("page_tokens", ctypes.c_int32), ("head_dim", ctypes.c_int32)]
+
+
+class _KvRows(ctypes.Structure):
+    _fields_ = [("page_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("lengths", ctypes.c_void_p),
+                ("rows", ctypes.c_int32), ("pages_per_row", ctypes.c_int32)]
+
+
 CANCEL_FN = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p)
 TOKEN_FN = ctypes.CFUNCTYPE(None, ctypes.c_void_p, ctypes.c_int, ctypes.c_int32)
 
@@ -101,6 +111,12 @@ def _load_library(path: str = LIB_PATH) -> ctypes.CDLL:
                                 ctypes.POINTER(ctypes.c_float)]),
         "yar_sample_device_noalloc": (I, [P, P, ctypes.c_int64, I, I, D, ctypes.POINTER(_Sampling), i32p, I, I, I,
                                           U64, P, P, P]),
+        "yar_kv_attn_decode": (I, [ctypes.POINTER(_KvPool), I, ctypes.POINTER(_KvRows), P, ctypes.c_int64, I, P,
+                                   ctypes.c_int64, I, I, D, I, P, P]),
+        "yar_kv_attn_prefill": (I, [ctypes.POINTER(_KvPool), I, ctypes.POINTER(_KvRows), P, ctypes.c_int64, P,
+                                    ctypes.c_int64, I, P, ctypes.c_int64, I, I, D, P, P]),
+        "yar_kv_copy_pages": (I, [ctypes.POINTER(_KvPool), ctypes.POINTER(_KvPool), i32p, i32p, i32p, I, P]),
+        "yar_kv_compact": (I, [ctypes.POINTER(_KvPool), P, ctypes.c_int64, I, I, P, P, ctypes.c_int64, P, P, P, P, P]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -430,6 +446,125 @@ def generate_tokens(model: ARModel, prefix, sampling: Sampling, seed: int, phase
     finally:
         if own:
             s.close()
+
+
+# ---- Operators on a paged key/value cache in the caller's device tensors ----------------
+# Thin wrappers of the yar_kv_* entry points (include/yue2ar.h has their contracts) for CUDA
+# tensors of a library with torch's tensor interface; torch itself is not imported here.
+
+def _kv_tensor(t, name: str, dtype: str, ndim: int):
+    if str(t.dtype) != "torch." + dtype or t.dim() != ndim:
+        raise ValueError(f"{name} must be a {ndim}-D {dtype} tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be on a CUDA device")
+
+
+def _kv_int32(t, name: str, least: int) -> int:
+    _kv_tensor(t, name, "int32", 1)
+    if t.shape[0] < least or not t.is_contiguous():
+        raise ValueError(f"{name} must hold at least {least} contiguous values")
+    return t.data_ptr()
+
+
+def _kv_pool(pool) -> _KvPool:
+    _kv_tensor(pool, "pool", "bfloat16", 6)
+    layers, pages, two, kv_heads, page_tokens, head_dim = pool.shape
+    if two != 2 or not pool.is_contiguous():
+        raise ValueError("pool must be contiguous [layers][pages][2][kv_heads][page_tokens][head_dim]")
+    return _KvPool(pool.data_ptr(), layers, pages, kv_heads, page_tokens, head_dim)
+
+
+def _kv_rows(table, lengths) -> _KvRows:
+    _kv_tensor(table, "page_table", "int32", 2)
+    rows, per_row = table.shape
+    if per_row > 1 and table.stride(1) != 1:
+        raise ValueError("page_table's entries of a row must be contiguous")
+    return _KvRows(table.data_ptr(), table.stride(0) if rows > 1 else per_row,
+                   _kv_int32(lengths, "lengths", rows), rows, per_row)
+
+
+def _kv_heads(t, name: str, dim: int) -> int:
+    """The row stride of a [rows][heads][dim] BF16 tensor whose rows are contiguous."""
+    _kv_tensor(t, name, "bfloat16", 3)
+    if t.shape[2] != dim or t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != dim):
+        raise ValueError(f"{name} must be [rows][heads][{dim}] with contiguous rows")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * dim
+
+
+def _kv_stream(t, stream):
+    if stream is not None:
+        return stream
+    import sys
+    return sys.modules["torch"].cuda.current_stream(t.device).cuda_stream
+
+
+def _kv_error(error):
+    return None if error is None else _kv_int32(error, "error", 1)
+
+
+def kv_attn_decode(pool, layer: int, page_table, lengths, q, out=None, window: int = 0, sinks: int = 0, scale=None,
+                   max_length: int = 0, error=None, stream=None):
+    """Attention of one token per row over its paged cache (yar_kv_attn_decode): q and the
+    result [rows][heads][dim] BF16, page_table [rows][pages_per_row] and lengths [rows] int32.
+    ``window``/``sinks``: only the last ``window`` positions and the first ``sinks`` are visible
+    (0: all). ``scale`` defaults to dim ** -0.5, ``stream`` to torch's current one."""
+    c_pool, rows = _kv_pool(pool), _kv_rows(page_table, lengths)
+    out = q.new_empty(q.shape) if out is None else out
+    dim = c_pool.head_dim
+    if q.shape[0] != rows.rows or out.shape != q.shape:
+        raise ValueError("q and out need one row for each row of page_table")
+    qs, os_ = _kv_heads(q, "q", dim), _kv_heads(out, "out", dim)
+    _check(lib.yar_kv_attn_decode(c_pool, layer, rows, q.data_ptr(), qs, q.shape[1], out.data_ptr(), os_, window,
+                                  sinks, dim ** -0.5 if scale is None else scale, max_length, _kv_error(error),
+                                  _kv_stream(q, stream)))
+    return out
+
+
+def kv_attn_prefill(pool, layer: int, page_table, lengths, offsets, q, out=None, window: int = 0, sinks: int = 0,
+                    scale=None, error=None, stream=None):
+    """Causal attention of each row's queries q[offsets[r]:offsets[r + 1]] (the last of its
+    lengths[r] cached positions) over its paged cache (yar_kv_attn_prefill); the other
+    arguments as ``kv_attn_decode``'s. A result allocated here is undefined outside the rows'
+    queries."""
+    c_pool, rows = _kv_pool(pool), _kv_rows(page_table, lengths)
+    out = q.new_empty(q.shape) if out is None else out
+    dim = c_pool.head_dim
+    if out.shape != q.shape:
+        raise ValueError("out must have q's shape")
+    qs, os_ = _kv_heads(q, "q", dim), _kv_heads(out, "out", dim)
+    _check(lib.yar_kv_attn_prefill(c_pool, layer, rows, _kv_int32(offsets, "offsets", rows.rows + 1), q.shape[0],
+                                   q.data_ptr(), qs, q.shape[1], out.data_ptr(), os_, window, sinks,
+                                   dim ** -0.5 if scale is None else scale, _kv_error(error), _kv_stream(q, stream)))
+    return out
+
+
+def kv_copy_pages(pool, src, dst, tokens=None, dst_pool=None, stream=None):
+    """Copy pages src[i] of ``pool`` to dst[i] of ``dst_pool`` (default: the same pool), the first
+    tokens[i] positions (default: all) of every layer (yar_kv_copy_pages; host lists)."""
+    a, b = _i32(src), _i32(dst)
+    t = None if tokens is None else _i32(tokens)
+    if a.ndim != 1 or a.shape != b.shape or (t is not None and t.shape != a.shape):
+        raise ValueError("src, dst and tokens must be lists of one length")
+    _check(lib.yar_kv_copy_pages(_kv_pool(pool), _kv_pool(pool if dst_pool is None else dst_pool),
+                                 _ptr(a, ctypes.c_int32), _ptr(b, ctypes.c_int32),
+                                 None if t is None else _ptr(t, ctypes.c_int32), a.size, _kv_stream(pool, stream)))
+
+
+def kv_compact(pool, page_table, counts, out=None, error=None, stream=None):
+    """Move the used pages to the front of the pool (yar_kv_compact). Returns (the renamed
+    table, remap [pages]: each page's new index or -1, used [1]); ``out`` may be ``page_table``."""
+    c_pool, rows = _kv_pool(pool), _kv_rows(page_table, counts)
+    out = page_table.new_empty(page_table.shape) if out is None else out
+    if out.shape != page_table.shape:
+        raise ValueError("out must have page_table's shape")
+    new = _kv_rows(out, counts)
+    remap = page_table.new_empty((c_pool.pages,))
+    used = page_table.new_empty((1,))
+    work = page_table.new_empty((1 + 2 * c_pool.pages,))
+    _check(lib.yar_kv_compact(c_pool, rows.page_table, rows.table_stride, rows.rows, rows.pages_per_row, rows.lengths,
+                              new.page_table, new.table_stride, remap.data_ptr(), used.data_ptr(), work.data_ptr(),
+                              _kv_error(error), _kv_stream(pool, stream)))
+    return out, remap, used
 
 
 def header_functions(header: str | None = None) -> list[str]:

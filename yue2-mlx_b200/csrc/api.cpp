@@ -35,6 +35,17 @@ void sample_device_noalloc(Model &m, const uint16_t *logits, long long row_strid
                            double cfg_scale, const ::yar_sampling &smp, const int32_t *history, int n_history,
                            int step, int phase, uint64_t seed, int32_t *token, float *scores,
                            cudaStream_t st);
+void kv_attn_decode(const ::yar_kv_pool *pool, int layer, const ::yar_kv_rows *rows, const void *q, int64_t q_stride,
+                    int heads, void *out, int64_t out_stride, int window, int sinks, double scale, int max_length,
+                    int32_t *error, cudaStream_t st);
+void kv_attn_prefill(const ::yar_kv_pool *pool, int layer, const ::yar_kv_rows *rows, const int32_t *offsets,
+                     int64_t n_queries, const void *q, int64_t q_stride, int heads, void *out, int64_t out_stride,
+                     int window, int sinks, double scale, int32_t *error, cudaStream_t st);
+void kv_copy_pages(const ::yar_kv_pool *from, const ::yar_kv_pool *to, const int32_t *src, const int32_t *dst,
+                   const int32_t *tokens, int n, cudaStream_t st);
+void kv_compact(const ::yar_kv_pool *pool, const int32_t *table, int64_t table_stride, int rows, int pages_per_row,
+                const int32_t *counts, int32_t *new_table, int64_t new_stride, int32_t *remap, int32_t *used,
+                int32_t *work, int32_t *error, cudaStream_t st);
 }  // namespace yar
 
 struct yar_model {
@@ -430,6 +441,40 @@ int yar_sample_device_noalloc(yar_model *model, const uint16_t *logits, int64_t 
     need(n_history == 0 || history, "history pointer missing");
     yar::sample_device_noalloc(*model->m, logits, row_stride, rows, n, cfg_scale, *sampling, history, n_history,
                                step, phase, seed, token, scores, static_cast<cudaStream_t>(stream));
+  });
+}
+
+int yar_kv_attn_decode(const yar_kv_pool *pool, int layer, const yar_kv_rows *rows, const void *q, int64_t q_stride,
+                       int heads, void *out, int64_t out_stride, int window, int sinks, double scale, int max_length,
+                       int32_t *error, void *stream) {
+  return guarded([&] {
+    yar::kv_attn_decode(pool, layer, rows, q, q_stride, heads, out, out_stride, window, sinks, scale, max_length,
+                        error, static_cast<cudaStream_t>(stream));
+  });
+}
+
+int yar_kv_attn_prefill(const yar_kv_pool *pool, int layer, const yar_kv_rows *rows, const int32_t *offsets,
+                        int64_t n_queries, const void *q, int64_t q_stride, int heads, void *out, int64_t out_stride,
+                        int window, int sinks, double scale, int32_t *error, void *stream) {
+  return guarded([&] {
+    yar::kv_attn_prefill(pool, layer, rows, offsets, n_queries, q, q_stride, heads, out, out_stride, window, sinks,
+                         scale, error, static_cast<cudaStream_t>(stream));
+  });
+}
+
+int yar_kv_copy_pages(const yar_kv_pool *src, const yar_kv_pool *dst, const int32_t *src_pages,
+                      const int32_t *dst_pages, const int32_t *tokens, int n, void *stream) {
+  return guarded([&] {
+    yar::kv_copy_pages(src, dst, src_pages, dst_pages, tokens, n, static_cast<cudaStream_t>(stream));
+  });
+}
+
+int yar_kv_compact(const yar_kv_pool *pool, const int32_t *page_table, int64_t table_stride, int rows,
+                   int pages_per_row, const int32_t *counts, int32_t *new_table, int64_t new_stride, int32_t *remap,
+                   int32_t *used, int32_t *work, int32_t *error, void *stream) {
+  return guarded([&] {
+    yar::kv_compact(pool, page_table, table_stride, rows, pages_per_row, counts, new_table, new_stride, remap, used,
+                    work, error, static_cast<cudaStream_t>(stream));
   });
 }
 
