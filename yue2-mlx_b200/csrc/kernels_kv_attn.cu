@@ -1,5 +1,7 @@
 // kernels_kv_attn.cu — attention over a paged cache: softmax(scale q K^T) V of the visible
 // positions, zeros for a query that sees nothing.
+#include <algorithm>
+
 #include "common.cuh"
 #include "kv_ops.h"
 
@@ -87,10 +89,370 @@ void simple(const KvAttnParams &p, int head_dim, cudaStream_t st) {
 }
 }  // namespace
 
+// ---------------------------------------------------------------------------------------
+// Single tokens: q [rows][heads][D], one query per row and head.
+//
+// A query row of a KV head's group reads each cached K and V value once for the whole
+// group, so the kernel is bound by HBM: 2 x 2 x D bytes per position and KV head. The work
+// of one (row, kv head) is split over a thread-block cluster of C blocks (C a power of two
+// up to 16: one row of eight heads then still fills 128 SMs), the parts joined through
+// distributed shared memory: no partials in global memory, no counters, nothing to clear
+// between calls.
+//
+// Each of a block's four warps takes 16 positions at a time (a slice) through its own ring
+// of cp.async copies (16 bytes a lane, any page size; rows that are not visible or whose
+// page is bad arrive as zeros), so no barrier separates the warps until their states are
+// joined. Per slice, on mma.m16n8k16 (BF16 in, FP32 out), with the group's queries as the
+// eight columns (two column tiles for groups of more than eight):
+//   S [16 keys x 8] = K q^T, D / 16 products;
+//   m = max(m, S), P = 2^(S scale log2(e) - m), l += P in FP32;
+//   O^T [D x 8] += V^T P, with P as two BF16 parts (P keeps 16 bits, so the result's error
+//   is its own rounding): P's fragment is transposed in registers (movmatrix).
+// The tensor work per slice is 8 KB of shared memory read once: about a third of the time in
+// which HBM delivers the slice's 8 KB to an SM.
+namespace {
+constexpr int kDecWarps = 4, kDecThreads = 32 * kDecWarps, kDecSlice = 16;
+constexpr int kDecMaxCluster = 16;
+
+template <int D>
+struct DecCfg {
+  static constexpr int kStage = 2 * kDecSlice * D * 2;           // bytes of one slice: K, then V
+  static constexpr int kStages = D == 128 ? 3 : 6;               // ring depth of a warp
+  static constexpr int kRing = kDecWarps * kStages * kStage;     // 96 KB: two blocks per SM
+};
+
+__device__ __forceinline__ uint32_t kv_smem(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+// 16 bytes to shared memory; `ok` false: zeros, nothing read.
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a));
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a));
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t a) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+  return r;
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// 2^x by the PTX approximate base-2 exponential (relative error below 2^-22; 2^-inf = 0).
+__device__ __forceinline__ float kv_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+// This block's shared memory address `a` as seen in block `rank` of the cluster.
+__device__ __forceinline__ float ld_cluster(uint32_t a, uint32_t rank) {
+  uint32_t r;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(r) : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory");
+}
+
+// Grid (C, kv_heads, rows), clusters of C blocks along x. NT: column tiles (groups of up to
+// 8 NT heads).
+template <int D, int NT>
+__global__ void __launch_bounds__(kDecThreads, 2) k_kv_attn_decode(const __grid_constant__ KvAttnParams p) {
+  using Cfg = DecCfg<D>;
+  constexpr int KS = D / 16, CPR = D / 8, Q = 8 * NT;  // mma steps, 16-byte chunks of a row, columns
+  extern __shared__ __align__(128) unsigned char ring[];
+  // After the loop the ring's space holds the warps' outputs, [warp][Q][D] FP32.
+  static_assert(kDecWarps * Q * D * 4 <= Cfg::kRing, "the warps' outputs fit the ring");
+  __shared__ float wml[kDecWarps][Q][2];  // a warp's (m, l)
+  __shared__ float part_ml[Q][2];         // the block's
+  __shared__ float part_o[Q * D];         // the block's output, scaled to its m
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int C = gridDim.x, rank = blockIdx.x, kvh = blockIdx.y, row = blockIdx.z, G = p.heads / p.kv_heads;
+
+  const int P = 1 << p.page_shift, cap = p.pages_per_row << p.page_shift;
+  int len = p.lengths[row];
+  if (len > cap) {
+    if (rank == 0 && kvh == 0 && tid == 0 && p.error) atomicOr(p.error, kKvBadLength);
+    len = cap;
+  }
+  // The visible positions in order: [0, sinks), then [lo, len).
+  const int lo = p.window ? max(0, len - p.window) : 0, sinks = p.window ? min(p.sinks, lo) : 0;
+  const int seen = len > 0 ? sinks + len - lo : 0;
+  // Slices of this block: a contiguous share; warp w takes every fourth.
+  const int slices = (seen + kDecSlice - 1) / kDecSlice, per = (slices + C - 1) / C;
+  const int s0 = min(slices, rank * per), s1 = min(slices, s0 + per);
+  const int n = max(0, (s1 - s0 - warp + kDecWarps - 1) / kDecWarps);  // this warp's slices
+
+  const int *tab = p.table + size_t(row) * p.table_stride;
+  // Lane l (and l + 16) looks after key l & 15 of a slice: its page (-1: none).
+  auto page_of = [&](int i) {
+    const int v = (s0 + warp + i * kDecWarps) * kDecSlice + (lane & 15);
+    if (i >= n || v >= seen) return -1;
+    const int j = v < sinks ? v : lo + v - sinks;
+    const int page = tab[j >> p.page_shift];
+    if (page >= 0 && page < p.pages) return page;
+    if (p.error) atomicOr(p.error, kKvBadPage);
+    return -1;
+  };
+  const uint32_t my_ring = kv_smem(ring) + warp * Cfg::kStages * Cfg::kStage;
+  constexpr int RPI = 32 / CPR;  // rows that one warp-wide copy covers
+  const int cr = lane / CPR, cc = lane % CPR;
+  const char *head_base = reinterpret_cast<const char *>(p.kv) + size_t(kvh) * P * D * 2 + cc * 16;
+  const size_t v_off = p.page_elems;  // bytes from a K row to its V row: page_elems / 2 values
+  // Copy slice i into ring stage i % kStages; `page` as page_of(i) gave it.
+  auto issue = [&](int i, int page) {
+    if (i < n) {
+      const uint32_t st = my_ring + (i % Cfg::kStages) * Cfg::kStage;
+      const int v0 = (s0 + warp + i * kDecWarps) * kDecSlice;
+#pragma unroll
+      for (int r0 = 0; r0 < kDecSlice; r0 += RPI) {
+        const int r = r0 + cr, pg = __shfl_sync(0xFFFFFFFFu, page, r), v = v0 + r;
+        const int j = v < sinks ? v : lo + v - sinks;
+        const bool ok = pg >= 0;
+        const char *src = head_base + (ok ? size_t(pg) * p.page_elems * 2 + size_t(j & (P - 1)) * (D * 2) : 0);
+        const uint32_t dst = st + r * (D * 2) + ((cc ^ (r & 7)) << 4);
+        cp16(dst, src, ok);
+        cp16(dst + kDecSlice * D * 2, src + v_off, ok);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  // The ring's pages are looked up one slice before their copies are issued.
+  int pages[Cfg::kStages];
+#pragma unroll
+  for (int i = 0; i < Cfg::kStages - 1; ++i) pages[i] = page_of(i);
+  int next_page = page_of(Cfg::kStages - 1);
+  uint32_t valid[Cfg::kStages];  // per stage: bit k = key k of the slice is visible
+#pragma unroll
+  for (int i = 0; i < Cfg::kStages - 1; ++i) {
+    issue(i, pages[i]);
+    valid[i] = __ballot_sync(0xFFFFFFFFu, pages[i] >= 0) & 0xFFFFu;
+  }
+
+  // The group's queries as B fragments: column lane / 4, dims 2 (lane % 4) and + 8 of each 16.
+  uint32_t bq[NT][KS][2];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int h = 8 * t + (lane >> 2);
+    const bf16 *qr = p.q + size_t(row) * p.q_stride + size_t(kvh * G + min(h, G - 1)) * D + 2 * (lane & 3);
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      bq[t][k][0] = h < G ? *reinterpret_cast<const uint32_t *>(qr + 16 * k) : 0u;
+      bq[t][k][1] = h < G ? *reinterpret_cast<const uint32_t *>(qr + 16 * k + 8) : 0u;
+    }
+  }
+  const float sl2 = p.scale * 1.4426950408889634f;
+  float m[NT][2], l[NT][2], o[NT][KS][4];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    m[t][0] = m[t][1] = -INFINITY;
+    l[t][0] = l[t][1] = 0.f;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) o[t][k][0] = o[t][k][1] = o[t][k][2] = o[t][k][3] = 0.f;
+  }
+  const int kr = lane & 15, kc = lane >> 4;                               // K: row, chunk of the pair
+  const int vr = (lane & 7) + ((lane >> 4) << 3), vc = (lane >> 3) & 1;   // V, transposed
+
+  for (int i = 0; i < n; ++i) {
+    // Refill the stage that slice i - 1 left; look up the pages of the one after.
+    issue(i + Cfg::kStages - 1, next_page);
+    const uint32_t ahead = __ballot_sync(0xFFFFFFFFu, next_page >= 0) & 0xFFFFu;
+    next_page = page_of(i + Cfg::kStages);
+    asm volatile("cp.async.wait_group %0;" ::"n"(Cfg::kStages - 1) : "memory");
+    __syncwarp();
+    const uint32_t st = my_ring + (i % Cfg::kStages) * Cfg::kStage;
+    const uint32_t ok = valid[0];
+#pragma unroll
+    for (int k = 0; k + 2 < Cfg::kStages; ++k) valid[k] = valid[k + 1];
+    valid[Cfg::kStages - 2] = ahead;
+
+    float s[NT][4];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      uint32_t a[4];
+      ldsm4(a, st + kr * (D * 2) + (((2 * k + kc) ^ (kr & 7)) << 4));
+#pragma unroll
+      for (int t = 0; t < NT; ++t) mma16816(s[t], a, bq[t][k][0], bq[t][k][1]);
+    }
+    const bool in0 = (ok >> (lane >> 2)) & 1u, in1 = (ok >> ((lane >> 2) + 8)) & 1u;
+    uint32_t ph[NT][2], pl[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      if (ok != 0xFFFFu) {
+        s[t][0] = in0 ? s[t][0] : -INFINITY, s[t][1] = in0 ? s[t][1] : -INFINITY;
+        s[t][2] = in1 ? s[t][2] : -INFINITY, s[t][3] = in1 ? s[t][3] : -INFINITY;
+      }
+      float mn[2] = {fmaxf(s[t][0], s[t][2]) * sl2, fmaxf(s[t][1], s[t][3]) * sl2};
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) {
+        mn[0] = fmaxf(mn[0], __shfl_xor_sync(0xFFFFFFFFu, mn[0], x));
+        mn[1] = fmaxf(mn[1], __shfl_xor_sync(0xFFFFFFFFu, mn[1], x));
+      }
+      mn[0] = fmaxf(mn[0], m[t][0]), mn[1] = fmaxf(mn[1], m[t][1]);
+      if (__any_sync(0xFFFFFFFFu, mn[0] > m[t][0] || mn[1] > m[t][1])) {
+        // 0 when m was -inf, and 1 while it still is (no position seen).
+        const float a0 = mn[0] == m[t][0] ? 1.f : kv_ex2(m[t][0] - mn[0]);
+        const float a1 = mn[1] == m[t][1] ? 1.f : kv_ex2(m[t][1] - mn[1]);
+        l[t][0] *= a0, l[t][1] *= a1;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) o[t][k][0] *= a0, o[t][k][1] *= a1, o[t][k][2] *= a0, o[t][k][3] *= a1;
+        m[t][0] = mn[0], m[t][1] = mn[1];
+      }
+      const float n0 = m[t][0] == -INFINITY ? 0.f : -m[t][0], n1 = m[t][1] == -INFINITY ? 0.f : -m[t][1];
+      const float e0 = kv_ex2(fmaf(s[t][0], sl2, n0)), e1 = kv_ex2(fmaf(s[t][1], sl2, n1));
+      const float e2 = kv_ex2(fmaf(s[t][2], sl2, n0)), e3 = kv_ex2(fmaf(s[t][3], sl2, n1));
+      l[t][0] += e0 + e2, l[t][1] += e1 + e3;
+      const uint32_t h0 = pack2(e0, e1), h1 = pack2(e2, e3);
+      ph[t][0] = transpose8(h0), ph[t][1] = transpose8(h1);
+      pl[t][0] = transpose8(pack2(e0 - bf_lo(h0), e1 - bf_hi(h0)));
+      pl[t][1] = transpose8(pack2(e2 - bf_lo(h1), e3 - bf_hi(h1)));
+    }
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      uint32_t a[4];
+      ldsm4t(a, st + kDecSlice * D * 2 + vr * (D * 2) + (((2 * k + vc) ^ (vr & 7)) << 4));
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        mma16816(o[t][k], a, ph[t][0], ph[t][1]);
+        mma16816(o[t][k], a, pl[t][0], pl[t][1]);
+      }
+    }
+    __syncwarp();
+  }
+
+  // Join the warps, then the cluster's blocks: each state weighted by 2^(m - M).
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();  // every warp is done with its ring
+  float *wo = reinterpret_cast<float *>(ring);
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      float v = l[t][c];
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, x);
+      const int col = 8 * t + 2 * (lane & 3) + c;
+      if (lane < 4) wml[warp][col][0] = m[t][c], wml[warp][col][1] = v;
+      if (col < G) {
+        float *dst = wo + (warp * Q + col) * D + (lane >> 2);
+#pragma unroll
+        for (int k = 0; k < KS; ++k) dst[16 * k] = o[t][k][c], dst[16 * k + 8] = o[t][k][c + 2];
+      }
+    }
+  }
+  __syncthreads();
+  bf16 *out = p.out + size_t(row) * p.out_stride + size_t(kvh) * G * D;
+  for (int e = tid; e < G * D; e += kDecThreads) {
+    const int h = e / D;
+    float M = -INFINITY, L = 0.f, O = 0.f;
+#pragma unroll
+    for (int w = 0; w < kDecWarps; ++w) M = fmaxf(M, wml[w][h][0]);
+#pragma unroll
+    for (int w = 0; w < kDecWarps; ++w) {
+      if (wml[w][h][1] == 0.f) continue;  // saw nothing (a sum that is NaN goes on)
+      const float a = wml[w][h][0] == M ? 1.f : kv_ex2(wml[w][h][0] - M);
+      L += a * wml[w][h][1];
+      O += a * wo[(w * Q + h) * D + e % D];
+    }
+    if (C == 1) {
+      out[e] = f2bf(L == 0.f ? 0.f : O / L);
+    } else {
+      part_o[e] = O;
+      if (e % D == 0) part_ml[h][0] = M, part_ml[h][1] = L;
+    }
+  }
+  if (C == 1) return;
+  cluster_sync();
+  const uint32_t ml = kv_smem(part_ml), po = kv_smem(part_o);
+  for (int e = rank * kDecThreads + tid; e < G * D; e += C * kDecThreads) {
+    const int h = e / D;
+    // Every load is issued before any is used: one round trip.
+    float mv[kDecMaxCluster], lv[kDecMaxCluster], ov[kDecMaxCluster], M = -INFINITY, L = 0.f, O = 0.f;
+#pragma unroll
+    for (int c = 0; c < kDecMaxCluster; ++c) {
+      mv[c] = -INFINITY, lv[c] = ov[c] = 0.f;
+      if (c < C) {
+        mv[c] = ld_cluster(ml + h * 8, c);
+        lv[c] = ld_cluster(ml + h * 8 + 4, c);
+        ov[c] = ld_cluster(po + e * 4, c);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < kDecMaxCluster; ++c) M = fmaxf(M, mv[c]);
+#pragma unroll
+    for (int c = 0; c < kDecMaxCluster; ++c) {
+      if (lv[c] == 0.f) continue;
+      const float a = mv[c] == M ? 1.f : kv_ex2(mv[c] - M);
+      L += a * lv[c];
+      O += a * ov[c];
+    }
+    out[e] = f2bf(L == 0.f ? 0.f : O / L);
+  }
+  cluster_sync();  // no block leaves while another reads its part
+}
+
+template <int D, int NT>
+void decode_launch(const KvAttnParams &p, int cluster, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(cluster, p.kv_heads, p.rows);
+  cfg.blockDim = dim3(kDecThreads);
+  cfg.dynamicSmemBytes = DecCfg<D>::kRing;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  YAR_CUDA(cudaLaunchKernelEx(&cfg, k_kv_attn_decode<D, NT>, p));
+}
+
+template <int D, int NT>
+void decode_configure() {
+  YAR_CUDA(cudaFuncSetAttribute(k_kv_attn_decode<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, DecCfg<D>::kRing));
+  YAR_CUDA(cudaFuncSetAttribute(k_kv_attn_decode<D, NT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+}
+}  // namespace
+
 void launch_kv_attn_decode(const KvAttnParams &p, int head_dim, cudaStream_t st) {
-  KvAttnParams d = p;
-  d.n_queries = p.rows;
-  simple(d, head_dim, st);
+  // Blocks per (row, kv head): as many as one wave holds (two blocks per SM), but no block
+  // with fewer than two passes of its four warps (128 positions).
+  const long long cap = (long long)p.pages_per_row << p.page_shift;
+  long long most = p.max_length > 0 ? std::min<long long>(p.max_length, cap) : cap;
+  if (p.window) most = std::min<long long>(most, (long long)p.window + p.sinks);
+  const long long units = (long long)p.rows * p.kv_heads;
+  int cluster = 1;
+  while (cluster < kDecMaxCluster && units * cluster * 2 <= 2 * 148 && most > cluster * 128) cluster *= 2;
+  const int group = p.heads / p.kv_heads;
+  if (head_dim == 128)
+    group <= 8 ? decode_launch<128, 1>(p, cluster, st) : decode_launch<128, 2>(p, cluster, st);
+  else
+    group <= 8 ? decode_launch<64, 1>(p, cluster, st) : decode_launch<64, 2>(p, cluster, st);
+}
+
+void configure_kv_attn_kernels() {
+  decode_configure<128, 1>();
+  decode_configure<128, 2>();
+  decode_configure<64, 1>();
+  decode_configure<64, 2>();
 }
 
 void launch_kv_attn_prefill(const KvPool &pool, int layer, const KvAttnParams &p, cudaStream_t st) {

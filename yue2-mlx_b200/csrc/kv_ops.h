@@ -53,6 +53,7 @@ void launch_kv_copy_pages(const KvPool &from, const KvPool &to, const int32_t *s
 void launch_kv_compact(const KvPool &pool, const int *table, long long table_stride, int rows, int pages_per_row,
                        const int *counts, int *new_table, long long new_stride, int *remap, int *used, int *work,
                        int *error, cudaStream_t st);
+void configure_kv_attn_kernels();
 void configure_kv_kernels();
 
 }  // namespace yar
