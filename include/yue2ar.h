@@ -265,7 +265,7 @@ int yar_sample_device_noalloc(yar_model *model, const uint16_t *logits, int64_t 
  * (a cudaStream_t; NULL = default stream) and returns: it allocates nothing, waits for
  * nothing and may be captured into a graph (make the first call on a device outside of a
  * capture). There is no working memory beyond the arguments, so calls may overlap as far as
- * their outputs are different memory. The calling thread's current device is unchanged.
+ * their outputs (and workspaces) are different memory. The calling thread's current device is unchanged.
  * What only the device sees (a page index or a length out of range) reads nothing outside
  * the pool: the positions concerned count as not visible, and a bit is added to *error
  * (an int32 that the caller zeroes and reads; NULL = not reported). */
@@ -303,10 +303,15 @@ typedef struct yar_kv_rows {
  * row strides in elements (multiples of 8), not overlapping; heads: a multiple of kv_heads,
  * at most 16 for each. FP32 scores, statistics and sums; one rounding of the result.
  * max_length (0: the table's end): a bound of the lengths; it only chooses into how many
- * parts a row's positions are split, longer rows stay right. */
+ * parts a row's positions are split, longer rows stay right. workspace (device memory, any
+ * contents; NULL and 0: none) lets a few long rows be split over the whole GPU; with fewer
+ * bytes than yar_kv_attn_decode_workspace says it is not used. Calls that may overlap (other
+ * streams, graphs replayed at the same time) need a workspace each. */
 int yar_kv_attn_decode(const yar_kv_pool *pool, int layer, const yar_kv_rows *rows, const void *q, int64_t q_stride,
                        int heads, void *out, int64_t out_stride, int window, int sinks, double scale, int max_length,
-                       int32_t *error, void *stream);
+                       void *workspace, int64_t workspace_bytes, int32_t *error, void *stream);
+/* The bytes of workspace that yar_kv_attn_decode can use for these heads. */
+int yar_kv_attn_decode_workspace(int heads, int kv_heads, int head_dim, int64_t *bytes);
 
 /* The same for prompts: row r's queries are q[offsets[r]] .. q[offsets[r + 1] - 1] (int32
  * [rows + 1], ascending, at most n_queries), the last n of its lengths[r] cached positions

@@ -136,6 +136,27 @@ def test_decode_matches_the_definition(yar, torch, lens, kv, group, dim, page, w
     check(torch, hint, np.stack([p[0] for p in pairs]), np.stack([p[1] for p in pairs]))
 
 
+@pytest.mark.parametrize("lens,kv,group,dim,page,window,sinks", [
+    ([24000], 2, 2, 128, 256, 0, 0), ([6000, 1, 0, 12001], 1, 16, 128, 16, 0, 0), ([9000], 2, 3, 64, 64, 5000, 100)])
+def test_long_rows_split_into_parts(yar, torch, lens, kv, group, dim, page, window, sinks):
+    """With a workspace (rows split over the whole GPU, joined by a second kernel), with one
+    that is too small, and without (a cluster)."""
+    c = Cache(torch, lens, kv, dim, page, seed=3, window=window, sinks=sinks)
+    q, q64 = queries(torch, len(lens), kv * group, dim, 4)
+    pairs = [c.attend(q64[r], r, n - 1, dim ** -0.5, window, sinks, P_ROUND["decode"]) for r, n in enumerate(lens)]
+    want, tol = np.stack([p[0] for p in pairs]), np.stack([p[1] for p in pairs])
+    size = yar.kv_attn_decode_workspace(kv * group, kv, dim)
+    dirty = torch.full((size,), 255, dtype=torch.uint8, device="cuda")
+    guard = torch.full((size + 64,), 255, dtype=torch.uint8, device="cuda")
+    for ws in (None, dirty, guard[:size], dirty[:size - 4]):
+        got = yar.kv_attn_decode(c.pool, 1, c.table, c.lengths, q, window=window, sinks=sinks, workspace=ws)
+        check(torch, got, want, tol)
+    assert (guard[size:] == 255).all()
+    got = yar.kv_attn_decode(c.pool, 1, c.table, c.lengths, q, window=window, sinks=sinks,
+                             stream=torch.cuda.current_stream().cuda_stream)
+    check(torch, got, want, tol)
+
+
 PREFILL = [
     # queries per row, cached before them, kv, group, dim, page, window, sinks
     ([1], [0], 2, 2, 64, 16, 0, 0), ([77], [0], 2, 2, 64, 16, 0, 0), ([5, 0, 130], [0, 9, 3], 1, 1, 128, 256, 0, 0),
@@ -335,7 +356,7 @@ def test_host_memory_is_refused(yar, torch):
         yar.kv_attn_decode(c.pool, 1, c.table, c.lengths, q.cpu())
     host = torch.zeros(1, 4, 64, dtype=torch.bfloat16)
     st = yar.lib.yar_kv_attn_decode(yar._kv_pool(c.pool), 1, yar._kv_rows(c.table, c.lengths), host.data_ptr(), 256, 4,
-                                    q.data_ptr(), 256, 0, 0, 0.125, 0, None, None)
+                                    q.data_ptr(), 256, 0, 0, 0.125, 0, None, 0, None, None)
     assert st == yar.INVALID_INPUT and b"device memory" in yar.lib.yar_last_error()
 
 

@@ -55,9 +55,9 @@ ROWS = [
 
 
 def decode(yar, p=None, r=None, layer=0, q=PTR, q_stride=256, heads=4, out=PTR, out_stride=256, window=0, sinks=0,
-           scale=0.125, max_length=0, error=None):
+           scale=0.125, max_length=0, workspace=None, workspace_bytes=0, error=None):
     return yar.lib.yar_kv_attn_decode(p or pool(yar), layer, r or rows(yar), q, q_stride, heads, out, out_stride,
-                                      window, sinks, scale, max_length, error, None)
+                                      window, sinks, scale, max_length, workspace, workspace_bytes, error, None)
 
 
 def prefill(yar, p=None, r=None, layer=0, offsets=PTR, n=5, q=PTR, q_stride=256, heads=4, out=PTR, out_stride=256,
@@ -79,12 +79,15 @@ def test_attention_refuses_bad_arguments(yar, call):
 
 def test_decode_and_prefill_own_arguments(yar):
     refused(yar, decode(yar, max_length=-1), "max_length")
+    refused(yar, decode(yar, workspace=PTR + 2, workspace_bytes=64), "workspace")
+    refused(yar, decode(yar, workspace=None, workspace_bytes=64), "workspace")
+    refused(yar, decode(yar, workspace=PTR, workspace_bytes=-1), "workspace")
     refused(yar, prefill(yar, n=-1), "n_queries")
     refused(yar, prefill(yar, n=1 << 31), "n_queries")
     refused(yar, prefill(yar, offsets=None), "offsets")
     assert prefill(yar, n=0, q=None, out=None, offsets=None) == yar.OK
-    refused(yar, yar.lib.yar_kv_attn_decode(None, 0, rows(yar), PTR, 256, 4, PTR, 256, 0, 0, .1, 0, None, None), "pool")
-    refused(yar, yar.lib.yar_kv_attn_decode(pool(yar), 0, None, PTR, 256, 4, PTR, 256, 0, 0, .1, 0, None, None), "rows")
+    refused(yar, yar.lib.yar_kv_attn_decode(None, 0, rows(yar), PTR, 256, 4, PTR, 256, 0, 0, .1, 0, None, 0, None, None), "pool")
+    refused(yar, yar.lib.yar_kv_attn_decode(pool(yar), 0, None, PTR, 256, 4, PTR, 256, 0, 0, .1, 0, None, 0, None, None), "rows")
 
 
 def copy(yar, src, dst, tokens=None, a=None, b=None):

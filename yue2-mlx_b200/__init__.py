@@ -20,6 +20,7 @@ from __future__ import annotations
 import ctypes
 import json
 import os
+import sys
 from dataclasses import dataclass
 
 import numpy as np
@@ -112,7 +113,8 @@ def _load_library(path: str = LIB_PATH) -> ctypes.CDLL:
         "yar_sample_device_noalloc": (I, [P, P, ctypes.c_int64, I, I, D, ctypes.POINTER(_Sampling), i32p, I, I, I,
                                           U64, P, P, P]),
         "yar_kv_attn_decode": (I, [ctypes.POINTER(_KvPool), I, ctypes.POINTER(_KvRows), P, ctypes.c_int64, I, P,
-                                   ctypes.c_int64, I, I, D, I, P, P]),
+                                   ctypes.c_int64, I, I, D, I, P, ctypes.c_int64, P, P]),
+        "yar_kv_attn_decode_workspace": (I, [I, I, I, ctypes.POINTER(ctypes.c_int64)]),
         "yar_kv_attn_prefill": (I, [ctypes.POINTER(_KvPool), I, ctypes.POINTER(_KvRows), P, ctypes.c_int64, P,
                                     ctypes.c_int64, I, P, ctypes.c_int64, I, I, D, P, P]),
         "yar_kv_copy_pages": (I, [ctypes.POINTER(_KvPool), ctypes.POINTER(_KvPool), i32p, i32p, i32p, I, P]),
@@ -452,8 +454,14 @@ def generate_tokens(model: ARModel, prefix, sampling: Sampling, seed: int, phase
 # Thin wrappers of the yar_kv_* entry points (include/yue2ar.h has their contracts) for CUDA
 # tensors of a library with torch's tensor interface; torch itself is not imported here.
 
+_kv_dtypes: dict = {}  # dtype object -> its name
+
+
 def _kv_tensor(t, name: str, dtype: str, ndim: int):
-    if str(t.dtype) != "torch." + dtype or t.dim() != ndim:
+    have = _kv_dtypes.get(t.dtype)
+    if have is None:
+        have = _kv_dtypes[t.dtype] = str(t.dtype)[len("torch."):]
+    if have != dtype or t.dim() != ndim:
         raise ValueError(f"{name} must be a {ndim}-D {dtype} tensor")
     if not t.is_cuda:
         raise ValueError(f"{name} must be on a CUDA device")
@@ -494,29 +502,41 @@ def _kv_heads(t, name: str, dim: int) -> int:
 def _kv_stream(t, stream):
     if stream is not None:
         return stream
-    import sys
-    return sys.modules["torch"].cuda.current_stream(t.device).cuda_stream
+    return sys.modules["torch"]._C._cuda_getCurrentRawStream(t.get_device())
 
 
 def _kv_error(error):
     return None if error is None else _kv_int32(error, "error", 1)
 
 
+def kv_attn_decode_workspace(heads: int, kv_heads: int, head_dim: int) -> int:
+    """Bytes of workspace that ``kv_attn_decode`` can use (yar_kv_attn_decode_workspace)."""
+    n = ctypes.c_int64()
+    _check(lib.yar_kv_attn_decode_workspace(heads, kv_heads, head_dim, ctypes.byref(n)))
+    return n.value
+
+
 def kv_attn_decode(pool, layer: int, page_table, lengths, q, out=None, window: int = 0, sinks: int = 0, scale=None,
-                   max_length: int = 0, error=None, stream=None):
+                   max_length: int = 0, workspace=None, error=None, stream=None):
     """Attention of one token per row over its paged cache (yar_kv_attn_decode): q and the
     result [rows][heads][dim] BF16, page_table [rows][pages_per_row] and lengths [rows] int32.
     ``window``/``sinks``: only the last ``window`` positions and the first ``sinks`` are visible
-    (0: all). ``scale`` defaults to dim ** -0.5, ``stream`` to torch's current one."""
+    (0: all). ``scale`` defaults to dim ** -0.5, ``stream`` to torch's current one, ``workspace``
+    (any tensor of ``kv_attn_decode_workspace`` bytes) to fresh memory where rows are long."""
     c_pool, rows = _kv_pool(pool), _kv_rows(page_table, lengths)
     out = q.new_empty(q.shape) if out is None else out
     dim = c_pool.head_dim
     if q.shape[0] != rows.rows or out.shape != q.shape:
         raise ValueError("q and out need one row for each row of page_table")
     qs, os_ = _kv_heads(q, "q", dim), _kv_heads(out, "out", dim)
-    _check(lib.yar_kv_attn_decode(c_pool, layer, rows, q.data_ptr(), qs, q.shape[1], out.data_ptr(), os_, window,
-                                  sinks, dim ** -0.5 if scale is None else scale, max_length, _kv_error(error),
-                                  _kv_stream(q, stream)))
+    heads = q.shape[1]
+    if workspace is None and stream is None and (max_length or rows.pages_per_row * c_pool.page_tokens) > 4096 and \
+            not 0 < window < 4096 and rows.rows * c_pool.kv_heads <= 74:
+        workspace = q.new_empty((kv_attn_decode_workspace(heads, c_pool.kv_heads, dim) // 2,))
+    w, wb = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
+    _check(lib.yar_kv_attn_decode(c_pool, layer, rows, q.data_ptr(), qs, heads, out.data_ptr(), os_, window,
+                                  sinks, dim ** -0.5 if scale is None else scale, max_length, w, wb,
+                                  _kv_error(error), _kv_stream(q, stream)))
     return out
 
 

@@ -37,7 +37,8 @@ void sample_device_noalloc(Model &m, const uint16_t *logits, long long row_strid
                            cudaStream_t st);
 void kv_attn_decode(const ::yar_kv_pool *pool, int layer, const ::yar_kv_rows *rows, const void *q, int64_t q_stride,
                     int heads, void *out, int64_t out_stride, int window, int sinks, double scale, int max_length,
-                    int32_t *error, cudaStream_t st);
+                    void *workspace, int64_t workspace_bytes, int32_t *error, cudaStream_t st);
+size_t kv_attn_decode_workspace(int heads, int kv_heads, int head_dim);
 void kv_attn_prefill(const ::yar_kv_pool *pool, int layer, const ::yar_kv_rows *rows, const int32_t *offsets,
                      int64_t n_queries, const void *q, int64_t q_stride, int heads, void *out, int64_t out_stride,
                      int window, int sinks, double scale, int32_t *error, cudaStream_t st);
@@ -446,10 +447,19 @@ int yar_sample_device_noalloc(yar_model *model, const uint16_t *logits, int64_t 
 
 int yar_kv_attn_decode(const yar_kv_pool *pool, int layer, const yar_kv_rows *rows, const void *q, int64_t q_stride,
                        int heads, void *out, int64_t out_stride, int window, int sinks, double scale, int max_length,
-                       int32_t *error, void *stream) {
+                       void *workspace, int64_t workspace_bytes, int32_t *error, void *stream) {
   return guarded([&] {
     yar::kv_attn_decode(pool, layer, rows, q, q_stride, heads, out, out_stride, window, sinks, scale, max_length,
-                        error, static_cast<cudaStream_t>(stream));
+                        workspace, workspace_bytes, error, static_cast<cudaStream_t>(stream));
+  });
+}
+
+int yar_kv_attn_decode_workspace(int heads, int kv_heads, int head_dim, int64_t *bytes) {
+  return guarded([&] {
+    need(bytes && kv_heads >= 1 && heads >= 1 && heads % kv_heads == 0 && heads / kv_heads <= 16 &&
+             (head_dim == 64 || head_dim == 128),
+         "heads must be a multiple of kv_heads, at most 16 for each, and head_dim 64 or 128");
+    *bytes = int64_t(yar::kv_attn_decode_workspace(heads, kv_heads, head_dim));
   });
 }
 

@@ -99,7 +99,7 @@ void simple(const KvAttnParams &p, int head_dim, cudaStream_t st) {
 // distributed shared memory: no partials in global memory, no counters, nothing to clear
 // between calls.
 //
-// Each of a block's four warps takes 16 positions at a time (a slice) through its own ring
+// Each of a block's warps takes 16 positions at a time (a slice) through its own ring
 // of cp.async copies (16 bytes a lane, any page size; rows that are not visible or whose
 // page is bad arrive as zeros), so no barrier separates the warps until their states are
 // joined. Per slice, on mma.m16n8k16 (BF16 in, FP32 out), with the group's queries as the
@@ -111,14 +111,15 @@ void simple(const KvAttnParams &p, int head_dim, cudaStream_t st) {
 // The tensor work per slice is 8 KB of shared memory read once: about a third of the time in
 // which HBM delivers the slice's 8 KB to an SM.
 namespace {
-constexpr int kDecWarps = 4, kDecThreads = 32 * kDecWarps, kDecSlice = 16;
-constexpr int kDecMaxCluster = 16;
+constexpr int kDecSlice = 16, kDecMaxCluster = 16;
 
-template <int D>
+// W warps of a block: 8, one block per SM (192 KB of rings), or 4, two blocks per SM.
+template <int D, int W>
 struct DecCfg {
-  static constexpr int kStage = 2 * kDecSlice * D * 2;           // bytes of one slice: K, then V
-  static constexpr int kStages = D == 128 ? 3 : 6;               // ring depth of a warp
-  static constexpr int kRing = kDecWarps * kStages * kStage;     // 96 KB: two blocks per SM
+  static constexpr int kThreads = 32 * W;
+  static constexpr int kStage = 2 * kDecSlice * D * 2;  // bytes of one slice: K, then V
+  static constexpr int kStages = D == 128 ? 3 : 6;      // ring depth of a warp
+  static constexpr int kRing = W * kStages * kStage;
 };
 
 __device__ __forceinline__ uint32_t kv_smem(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -172,18 +173,19 @@ __device__ __forceinline__ void cluster_sync() {
 
 // Grid (C, kv_heads, rows), clusters of C blocks along x. NT: column tiles (groups of up to
 // 8 NT heads).
-template <int D, int NT>
-__global__ void __launch_bounds__(kDecThreads, 2) k_kv_attn_decode(const __grid_constant__ KvAttnParams p) {
-  using Cfg = DecCfg<D>;
+template <int D, int NT, int W>
+__global__ void __launch_bounds__(32 * W, 8 / W) k_kv_attn_decode(const __grid_constant__ KvAttnParams p) {
+  using Cfg = DecCfg<D, W>;
   constexpr int KS = D / 16, CPR = D / 8, Q = 8 * NT;  // mma steps, 16-byte chunks of a row, columns
   extern __shared__ __align__(128) unsigned char ring[];
   // After the loop the ring's space holds the warps' outputs, [warp][Q][D] FP32.
-  static_assert(kDecWarps * Q * D * 4 <= Cfg::kRing, "the warps' outputs fit the ring");
-  __shared__ float wml[kDecWarps][Q][2];  // a warp's (m, l)
+  static_assert(W * Q * D * 4 <= Cfg::kRing, "the warps' outputs fit the ring");
+  __shared__ float wml[W][Q][2];  // a warp's (m, l)
   __shared__ float part_ml[Q][2];         // the block's
   __shared__ float part_o[Q * D];         // the block's output, scaled to its m
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int C = gridDim.x, rank = blockIdx.x, kvh = blockIdx.y, row = blockIdx.z, G = p.heads / p.kv_heads;
+  if (p.partials) pdl_launch_dependents();  // the join kernel may get ready; it waits for this grid's end
 
   const int P = 1 << p.page_shift, cap = p.pages_per_row << p.page_shift;
   int len = p.lengths[row];
@@ -194,32 +196,33 @@ __global__ void __launch_bounds__(kDecThreads, 2) k_kv_attn_decode(const __grid_
   // The visible positions in order: [0, sinks), then [lo, len).
   const int lo = p.window ? max(0, len - p.window) : 0, sinks = p.window ? min(p.sinks, lo) : 0;
   const int seen = len > 0 ? sinks + len - lo : 0;
-  // Slices of this block: a contiguous share; warp w takes every fourth.
+  // Slices of this block: a contiguous share; warp w takes every W-th.
   const int slices = (seen + kDecSlice - 1) / kDecSlice, per = (slices + C - 1) / C;
   const int s0 = min(slices, rank * per), s1 = min(slices, s0 + per);
-  const int n = max(0, (s1 - s0 - warp + kDecWarps - 1) / kDecWarps);  // this warp's slices
+  const int n = max(0, (s1 - s0 - warp + W - 1) / W);  // this warp's slices
 
   const int *tab = p.table + size_t(row) * p.table_stride;
-  // Lane l (and l + 16) looks after key l & 15 of a slice: its page (-1: none).
-  auto page_of = [&](int i) {
-    const int v = (s0 + warp + i * kDecWarps) * kDecSlice + (lane & 15);
+  // Lane l (and l + 16) looks after key l & 15 of a slice: its page-table entry (-1: no key),
+  // loaded two slices before the copies that need it.
+  auto entry_of = [&](int i) {
+    const int v = (s0 + warp + i * W) * kDecSlice + (lane & 15);
     if (i >= n || v >= seen) return -1;
-    const int j = v < sinks ? v : lo + v - sinks;
-    const int page = tab[j >> p.page_shift];
-    if (page >= 0 && page < p.pages) return page;
-    if (p.error) atomicOr(p.error, kKvBadPage);
-    return -1;
+    const int e = tab[(v < sinks ? v : lo + v - sinks) >> p.page_shift];
+    return e < 0 || e >= p.pages ? -2 : e;
   };
+  bool bad = false;  // an entry outside the pool (reported at the end)
   const uint32_t my_ring = kv_smem(ring) + warp * Cfg::kStages * Cfg::kStage;
   constexpr int RPI = 32 / CPR;  // rows that one warp-wide copy covers
   const int cr = lane / CPR, cc = lane % CPR;
   const char *head_base = reinterpret_cast<const char *>(p.kv) + size_t(kvh) * P * D * 2 + cc * 16;
   const size_t v_off = p.page_elems;  // bytes from a K row to its V row: page_elems / 2 values
-  // Copy slice i into ring stage i % kStages; `page` as page_of(i) gave it.
-  auto issue = [&](int i, int page) {
+  // Copy slice i into ring stage i % kStages; `page` as entry_of(i) gave it. Returns the keys
+  // that are there, a bit each.
+  auto issue = [&](int i, int page) -> uint32_t {
+    bad |= page == -2;
     if (i < n) {
       const uint32_t st = my_ring + (i % Cfg::kStages) * Cfg::kStage;
-      const int v0 = (s0 + warp + i * kDecWarps) * kDecSlice;
+      const int v0 = (s0 + warp + i * W) * kDecSlice;
 #pragma unroll
       for (int r0 = 0; r0 < kDecSlice; r0 += RPI) {
         const int r = r0 + cr, pg = __shfl_sync(0xFFFFFFFFu, page, r), v = v0 + r;
@@ -232,18 +235,16 @@ __global__ void __launch_bounds__(kDecThreads, 2) k_kv_attn_decode(const __grid_
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
+    return __ballot_sync(0xFFFFFFFFu, page >= 0) & 0xFFFFu;
   };
-  // The ring's pages are looked up one slice before their copies are issued.
-  int pages[Cfg::kStages];
+  constexpr int S = Cfg::kStages;
+  int pages[S + 1];
 #pragma unroll
-  for (int i = 0; i < Cfg::kStages - 1; ++i) pages[i] = page_of(i);
-  int next_page = page_of(Cfg::kStages - 1);
-  uint32_t valid[Cfg::kStages];  // per stage: bit k = key k of the slice is visible
+  for (int i = 0; i < S + 1; ++i) pages[i] = entry_of(i);
+  int page_a = pages[S - 1], page_b = pages[S];
+  uint32_t valid[S - 1];  // the keys of the slices in flight
 #pragma unroll
-  for (int i = 0; i < Cfg::kStages - 1; ++i) {
-    issue(i, pages[i]);
-    valid[i] = __ballot_sync(0xFFFFFFFFu, pages[i] >= 0) & 0xFFFFu;
-  }
+  for (int i = 0; i < S - 1; ++i) valid[i] = issue(i, pages[i]);
 
   // The group's queries as B fragments: column lane / 4, dims 2 (lane % 4) and + 8 of each 16.
   uint32_t bq[NT][KS][2];
@@ -270,17 +271,16 @@ __global__ void __launch_bounds__(kDecThreads, 2) k_kv_attn_decode(const __grid_
   const int vr = (lane & 7) + ((lane >> 4) << 3), vc = (lane >> 3) & 1;   // V, transposed
 
   for (int i = 0; i < n; ++i) {
-    // Refill the stage that slice i - 1 left; look up the pages of the one after.
-    issue(i + Cfg::kStages - 1, next_page);
-    const uint32_t ahead = __ballot_sync(0xFFFFFFFFu, next_page >= 0) & 0xFFFFu;
-    next_page = page_of(i + Cfg::kStages);
-    asm volatile("cp.async.wait_group %0;" ::"n"(Cfg::kStages - 1) : "memory");
+    // Refill the stage that slice i - 1 left.
+    const uint32_t ahead = issue(i + S - 1, page_a);
+    page_a = page_b;
+    page_b = entry_of(i + S + 1);
+    asm volatile("cp.async.wait_group %0;" ::"n"(S - 1) : "memory");
     __syncwarp();
-    const uint32_t st = my_ring + (i % Cfg::kStages) * Cfg::kStage;
-    const uint32_t ok = valid[0];
+    const uint32_t st = my_ring + (i % S) * Cfg::kStage, ok = valid[0];
 #pragma unroll
-    for (int k = 0; k + 2 < Cfg::kStages; ++k) valid[k] = valid[k + 1];
-    valid[Cfg::kStages - 2] = ahead;
+    for (int k = 0; k + 2 < S; ++k) valid[k] = valid[k + 1];
+    valid[S - 2] = ahead;
 
     float s[NT][4];
 #pragma unroll
@@ -338,6 +338,7 @@ __global__ void __launch_bounds__(kDecThreads, 2) k_kv_attn_decode(const __grid_
     __syncwarp();
   }
 
+  if (bad && p.error) atomicOr(p.error, kKvBadPage);
   // Join the warps, then the cluster's blocks: each state weighted by 2^(m - M).
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();  // every warp is done with its ring
@@ -360,13 +361,13 @@ __global__ void __launch_bounds__(kDecThreads, 2) k_kv_attn_decode(const __grid_
   }
   __syncthreads();
   bf16 *out = p.out + size_t(row) * p.out_stride + size_t(kvh) * G * D;
-  for (int e = tid; e < G * D; e += kDecThreads) {
+  for (int e = tid; e < G * D; e += Cfg::kThreads) {
     const int h = e / D;
     float M = -INFINITY, L = 0.f, O = 0.f;
 #pragma unroll
-    for (int w = 0; w < kDecWarps; ++w) M = fmaxf(M, wml[w][h][0]);
+    for (int w = 0; w < W; ++w) M = fmaxf(M, wml[w][h][0]);
 #pragma unroll
-    for (int w = 0; w < kDecWarps; ++w) {
+    for (int w = 0; w < W; ++w) {
       if (wml[w][h][1] == 0.f) continue;  // saw nothing (a sum that is NaN goes on)
       const float a = wml[w][h][0] == M ? 1.f : kv_ex2(wml[w][h][0] - M);
       L += a * wml[w][h][1];
@@ -374,15 +375,19 @@ __global__ void __launch_bounds__(kDecThreads, 2) k_kv_attn_decode(const __grid_
     }
     if (C == 1) {
       out[e] = f2bf(L == 0.f ? 0.f : O / L);
+    } else if (p.partials) {
+      float *dst = p.partials + ((size_t(row) * p.heads + kvh * G + h) * C + rank) * (D + 2);
+      dst[2 + e % D] = O;
+      if (e % D == 0) dst[0] = M, dst[1] = L;
     } else {
       part_o[e] = O;
       if (e % D == 0) part_ml[h][0] = M, part_ml[h][1] = L;
     }
   }
-  if (C == 1) return;
+  if (C == 1 || p.partials) return;
   cluster_sync();
   const uint32_t ml = kv_smem(part_ml), po = kv_smem(part_o);
-  for (int e = rank * kDecThreads + tid; e < G * D; e += C * kDecThreads) {
+  for (int e = rank * Cfg::kThreads + tid; e < G * D; e += C * Cfg::kThreads) {
     const int h = e / D;
     // Every load is issued before any is used: one round trip.
     float mv[kDecMaxCluster], lv[kDecMaxCluster], ov[kDecMaxCluster], M = -INFINITY, L = 0.f, O = 0.f;
@@ -409,12 +414,47 @@ __global__ void __launch_bounds__(kDecThreads, 2) k_kv_attn_decode(const __grid_
   cluster_sync();  // no block leaves while another reads its part
 }
 
-template <int D, int NT>
-void decode_launch(const KvAttnParams &p, int cluster, cudaStream_t st) {
+// Grid (heads, rows), one thread per dim: the parts' states [row][head][parts][D + 2] (m, l,
+// o) joined as the cluster's blocks are.
+template <int D>
+__global__ void __launch_bounds__(D) k_kv_attn_join(const __grid_constant__ KvAttnParams p, int parts) {
+  const int h = blockIdx.x, row = blockIdx.y, d = threadIdx.x;
+  pdl_wait();
+  const float *src = p.partials + (size_t(row) * p.heads + h) * parts * (D + 2);
+  constexpr int B = 8;  // parts read in one round trip
+  float M = -INFINITY, L = 0.f, O = 0.f;
+  for (int c0 = 0; c0 < parts; c0 += B) {
+    float mv[B], lv[B], ov[B], Mn = M;
+#pragma unroll
+    for (int c = 0; c < B; ++c) {
+      mv[c] = -INFINITY, lv[c] = ov[c] = 0.f;
+      if (c0 + c < parts) {
+        const float *s = src + (c0 + c) * (D + 2);
+        mv[c] = s[0], lv[c] = s[1], ov[c] = s[2 + d];
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < B; ++c) Mn = fmaxf(Mn, mv[c]);
+    const float r = M == Mn ? 1.f : kv_ex2(M - Mn);
+    L *= r, O *= r, M = Mn;
+#pragma unroll
+    for (int c = 0; c < B; ++c) {
+      if (lv[c] == 0.f) continue;
+      const float a = mv[c] == M ? 1.f : kv_ex2(mv[c] - M);
+      L += a * lv[c], O += a * ov[c];
+    }
+  }
+  p.out[size_t(row) * p.out_stride + size_t(h) * D + d] = f2bf(L == 0.f ? 0.f : O / L);
+}
+
+// `split` blocks per (row, kv head): a cluster, or (p.partials) parts for k_kv_attn_join.
+template <int D, int NT, int W>
+void decode_launch(const KvAttnParams &p, int split, cudaStream_t st) {
+  const int cluster = p.partials ? 1 : split;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(cluster, p.kv_heads, p.rows);
-  cfg.blockDim = dim3(kDecThreads);
-  cfg.dynamicSmemBytes = DecCfg<D>::kRing;
+  cfg.gridDim = dim3(split, p.kv_heads, p.rows);
+  cfg.blockDim = dim3(32 * W);
+  cfg.dynamicSmemBytes = DecCfg<D, W>::kRing;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -422,37 +462,88 @@ void decode_launch(const KvAttnParams &p, int cluster, cudaStream_t st) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  YAR_CUDA(cudaLaunchKernelEx(&cfg, k_kv_attn_decode<D, NT>, p));
+  YAR_CUDA(cudaLaunchKernelEx(&cfg, k_kv_attn_decode<D, NT, W>, p));
+  if (!p.partials) return;
+  cudaLaunchConfig_t join = {};
+  join.gridDim = dim3(p.heads, p.rows);
+  join.blockDim = dim3(D);
+  join.stream = st;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  join.attrs = attr;
+  join.numAttrs = 1;
+  YAR_CUDA(cudaLaunchKernelEx(&join, k_kv_attn_join<D>, p, split));
+}
+
+template <int D, int NT, int W>
+void decode_configure() {
+  const auto k = k_kv_attn_decode<D, NT, W>;
+  YAR_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, DecCfg<D, W>::kRing));
+  YAR_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
 }
 
 template <int D, int NT>
-void decode_configure() {
-  YAR_CUDA(cudaFuncSetAttribute(k_kv_attn_decode<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, DecCfg<D>::kRing));
-  YAR_CUDA(cudaFuncSetAttribute(k_kv_attn_decode<D, NT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+void decode_pick(const KvAttnParams &p, int split, int warps, cudaStream_t st) {
+  warps == 4 ? decode_launch<D, NT, 4>(p, split, st) : decode_launch<D, NT, 8>(p, split, st);
 }
+
+// Blocks of clusters of 2^i that run at once (the occupancy query's answers on this part:
+// large clusters leave SMs of a GPC unused).
+constexpr int kSlots4[5] = {296, 296, 284, 264, 224}, kSlots8[5] = {148, 148, 132, 120, 112};
 }  // namespace
 
+size_t kv_attn_decode_workspace(int heads, int kv_heads, int head_dim) {
+  return size_t(kSlots8[0]) * (heads / kv_heads) * (head_dim + 2) * sizeof(float);
+}
+
 void launch_kv_attn_decode(const KvAttnParams &p, int head_dim, cudaStream_t st) {
-  // Blocks per (row, kv head): as many as one wave holds (two blocks per SM), but no block
-  // with fewer than two passes of its four warps (128 positions).
   const long long cap = (long long)p.pages_per_row << p.page_shift;
   long long most = p.max_length > 0 ? std::min<long long>(p.max_length, cap) : cap;
   if (p.window) most = std::min<long long>(most, (long long)p.window + p.sinks);
-  const long long units = (long long)p.rows * p.kv_heads;
-  int cluster = 1;
-  while (cluster < kDecMaxCluster && units * cluster * 2 <= 2 * 148 && most > cluster * 128) cluster *= 2;
+  const long long units = (long long)p.rows * p.kv_heads, slices = (most + kDecSlice - 1) / kDecSlice;
+  // The form with the smallest estimated time in us: `split` blocks per unit, a block streaming
+  // at most at the rate that one was measured at alone (four warps 45 GB/s, eight 66), all of
+  // them at HBM's; ~3.5 us to start and end a launch, 1.3 more to join a cluster, 2 for the
+  // join kernel, 2.5 for each further wave of clusters (their blocks start together).
+  const double bytes = 2.0 * kDecSlice * head_dim * 2;
+  int split = 1, warps = 4;
+  bool parts = false;
+  double best = 1e30;
+  auto consider = [&](int w, int c, int slots, double fixed) {
+    const double blocks = double(units) * c, at_once = std::min(blocks, double(slots));
+    const double rate = std::min(w == 4 ? 45e3 : 66e3, 6500e3 / at_once);  // bytes per us
+    const double waves = std::max(1.0, blocks / slots);
+    const double t = fixed + waves * double((slices + c - 1) / c) * bytes / rate +
+                     (c > 1 && waves > 1 ? 2.5 * waves : 0.0);
+    if (t >= best) return false;
+    best = t, split = c, warps = w;
+    return true;
+  };
+  for (int i = 0; i < 5; ++i) {
+    const double fixed = i ? 4.8 : 3.5;
+    consider(4, 1 << i, kSlots4[i], fixed);
+    if (i < 4) consider(8, 1 << i, kSlots8[i], fixed);  // (16 blocks of eight warps: half as many run)
+  }
+  if (p.partials && 2 * units <= kSlots8[0])
+    parts = consider(8, int(kSlots8[0] / units), kSlots8[0], 5.5);
+  KvAttnParams d = p;
+  if (!parts) d.partials = nullptr;
   const int group = p.heads / p.kv_heads;
   if (head_dim == 128)
-    group <= 8 ? decode_launch<128, 1>(p, cluster, st) : decode_launch<128, 2>(p, cluster, st);
+    group <= 8 ? decode_pick<128, 1>(d, split, warps, st) : decode_pick<128, 2>(d, split, warps, st);
   else
-    group <= 8 ? decode_launch<64, 1>(p, cluster, st) : decode_launch<64, 2>(p, cluster, st);
+    group <= 8 ? decode_pick<64, 1>(d, split, warps, st) : decode_pick<64, 2>(d, split, warps, st);
 }
 
 void configure_kv_attn_kernels() {
-  decode_configure<128, 1>();
-  decode_configure<128, 2>();
-  decode_configure<64, 1>();
-  decode_configure<64, 2>();
+  decode_configure<128, 1, 4>();
+  decode_configure<128, 2, 4>();
+  decode_configure<64, 1, 4>();
+  decode_configure<64, 2, 4>();
+  decode_configure<128, 1, 8>();
+  decode_configure<128, 2, 8>();
+  decode_configure<64, 1, 8>();
+  decode_configure<64, 2, 8>();
 }
 
 void launch_kv_attn_prefill(const KvPool &pool, int layer, const KvAttnParams &p, cudaStream_t st) {

@@ -134,15 +134,19 @@ KvAttnParams attn_params(const KvPool &pool, int layer, const ::yar_kv_rows *row
 
 void kv_attn_decode(const ::yar_kv_pool *c_pool, int layer, const ::yar_kv_rows *rows, const void *q, int64_t q_stride,
                     int heads, void *out, int64_t out_stride, int window, int sinks, double scale, int max_length,
-                    int32_t *error, cudaStream_t st) {
+                    void *workspace, int64_t workspace_bytes, int32_t *error, cudaStream_t st) {
   const KvPool pool = checked_pool(c_pool);
   KvAttnParams p = attn_params(pool, layer, rows, q, q_stride, heads, out, out_stride, window, sinks, scale, error);
   need(max_length >= 0, "max_length must not be negative");
+  need(workspace_bytes >= 0 && (workspace || workspace_bytes == 0) && aligned(workspace, 4),
+       "workspace must be a 4-byte aligned buffer of workspace_bytes (or NULL and 0)");
   p.max_length = max_length;
+  if (workspace && size_t(workspace_bytes) >= kv_attn_decode_workspace(heads, pool.kv_heads, pool.head_dim))
+    p.partials = static_cast<float *>(workspace);
   if (p.rows == 0) return;
   need(q && out, "q and out are required");
   const int device = device_of({{"the pool", pool.data}, {"the page table", p.table}, {"lengths", p.lengths}, {"q", q},
-                                {"out", out}, {"error", error}});
+                                {"out", out}, {"workspace", workspace}, {"error", error}});
   DeviceGuard guard(device);
   configure_device(device);
   launch_kv_attn_decode(p, pool.head_dim, st);

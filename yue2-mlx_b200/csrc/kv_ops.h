@@ -38,9 +38,11 @@ struct KvAttnParams {
   int window = 0, sinks = 0;
   float scale = 1.f;
   int max_length = 0;  // decode: a bound of the lengths, for the choice of splits only (0: the table's)
+  float *partials = nullptr;  // decode: workspace of kv_attn_decode_workspace bytes (may be null)
   int *error = nullptr;
 };
 
+size_t kv_attn_decode_workspace(int heads, int kv_heads, int head_dim);
 void launch_kv_attn_decode(const KvAttnParams &p, int head_dim, cudaStream_t st);
 // `pool`: the whole pool (the tensor map covers it); p.kv lies in it.
 void launch_kv_attn_prefill(const KvPool &pool, int layer, const KvAttnParams &p, cudaStream_t st);
