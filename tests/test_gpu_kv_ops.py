@@ -204,6 +204,43 @@ def test_large_scores_and_a_given_scale(yar, torch):
         check(torch, got, np.stack([p[0] for p in pairs]), np.stack([p[1] for p in pairs]))
 
 
+@pytest.mark.parametrize("dim,window,sinks", [(128, 0, 0), (64, 90, 3), (128, 300, 0)])
+def test_values_that_are_not_finite_reach_only_the_queries_that_see_them(yar, torch, dim, window, sinks):
+    """V rows holding infinities and NaN, keys with NaN: a query that does not see them is as
+    without them (bit for bit), one that sees them gets what the sum gives."""
+    n, heads = 400, 4
+    c = Cache(torch, [n], 2, dim, 64, seed=31)
+    q, _ = queries(torch, n, heads, dim, 8)
+    offs = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    clean = yar.kv_attn_prefill(c.pool, 1, c.table, c.lengths, offs, q, window=window, sinks=sinks)
+    at = 270
+    page, slot = int(c.table[0, at // 64]), at % 64
+    sees = torch.tensor([at in visible(n, i, window, sinks) for i in range(n)], device="cuda")
+    assert 0 < sees.sum() < n
+    for what, value in (("v", float("inf")), ("v", float("nan")), ("k", float("nan"))):
+        pool = c.pool.clone()
+        pool[1, page, 0 if what == "k" else 1, 0, slot, 7] = value  # KV head 0: heads 0 and 1
+        got = yar.kv_attn_prefill(pool, 1, c.table, c.lengths, offs, q, window=window, sinks=sinks)
+        err = (got.float() - clean.float()).abs()
+        assert torch.equal(got[:, 2:], clean[:, 2:])
+        hidden = err[~sees][:, :2]  # recomputed sums may round differently
+        assert torch.isfinite(hidden).all() and (hidden <= 2.0 ** -6 * (clean[~sees][:, :2].float().abs() + 1)).all()
+        seen = got[sees][:, :2].float()
+        if what == "k":
+            assert torch.isnan(seen).all()
+        else:
+            assert not torch.isfinite(seen[..., 7]).any()
+            rest = torch.ones(dim, dtype=torch.bool)
+            rest[7] = False
+            assert torch.isfinite(seen[..., rest]).all()
+        one = yar.kv_attn_decode(pool, 1, c.table, c.lengths, q[-1:], window=window, sinks=sinks)
+        before = yar.kv_attn_decode(c.pool, 1, c.table, c.lengths, q[-1:], window=window, sinks=sinks)
+        if not sees[-1]:
+            assert torch.equal(one, before)
+        else:
+            assert not torch.isfinite(one[0, :2].float()).all() and torch.equal(one[:, 2:], before[:, 2:])
+
+
 def test_strided_tensors_and_rows_behind_the_last(yar, torch):
     c = Cache(torch, [40, 90], 2, 64, 16, seed=8)
     wide = torch.randn(6, 9, 64, device="cuda").bfloat16()

@@ -179,9 +179,9 @@ bool gemm_tc_supported(const bf16 *A, int M, int K, const bf16 *W, int N, const 
 void launch_gemm_tc(const bf16 *A, int M, int K, const bf16 *W, int N, bf16 *C, int ldc, int epilogue, int *error,
                     float *ws, size_t ws_floats, cudaStream_t st, int split_n = 0);
 void configure_gemm_tc_kernels();
-// A 2-D TMA map of `rows` rows of 128 BF16 at `base` (256-byte pitch), {64, 64} boxes,
+// A 2-D TMA map of `rows` dense rows of `width` BF16 at `base`, {64, box_rows} boxes,
 // 128-byte swizzle; false when the driver's encoder is unavailable or refuses it.
-bool encode_rows128_map(CUtensorMap *map, const bf16 *base, uint64_t rows);
+bool encode_rows_map(CUtensorMap *map, const bf16 *base, uint64_t rows, int width, int box_rows);
 void launch_qkv_post_prefill(const Model &m, Session &s, int layer, int row, int start, int T,
                              cudaStream_t st);
 void launch_attn_prefill(const Model &m, Session &s, int layer, int row, int start, int T,

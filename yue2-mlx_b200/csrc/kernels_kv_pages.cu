@@ -217,6 +217,7 @@ void launch_kv_compact(const KvPool &pool, const int *table, long long table_str
 
 void configure_kv_kernels() {
   configure_kv_attn_kernels();
+  configure_kv_prefill_kernels();
   YAR_CUDA(cudaFuncSetAttribute(k_kv_compact_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, kKvMaxPages / 8));
 }
 

@@ -1,0 +1,718 @@
+// kernels_kv_prefill.cu — causal attention of prompt chunks over a paged cache (any group of
+// query heads, full or a sliding window with sinks), on the 5th-generation tensor cores.
+//
+// softmax(scale q K^T) V per query over the visible positions. The queries of one row and KV
+// head are flattened to M rows (query-major: row m is query m / G, head m % G), so a group
+// shares every K and V tile and short chunks fill their tiles. A block takes 256 M rows as
+// two tiles A and B of 128, and walks the 128-key tiles that any of its queries sees (the
+// sinks' tiles, then the window's). Its warps (10 and 11 idle):
+//   * warp 9 brings K and V tiles by TMA through a ring (one box per page piece; pieces that
+//     nothing sees, or whose page is bad, are fetched out of bounds: zeros);
+//   * lane 0 of warp 8 issues the products: S = Q K^T into TMEM (128 columns for each of A
+//     and B), and O += P V with P read from TMEM, where the softmax warps left it in S's own
+//     columns. While A's softmax runs the tensor pipe works for B, and the other way round;
+//   * warps 0..3 (A) and 4..7 (B): a thread owns one M row (= TMEM lane). It reads its 128
+//     scores, masks them (tiles on an edge only), raises its running maximum m when the tile
+//     exceeds it by more than 8 (in log2 units; O in TMEM is rescaled only then: O / l is
+//     the same quotient whichever m the terms share), writes P = 2^(s - m) as BF16 and adds
+//     P to l in FP32.
+// P in BF16 costs 2^-9 of each weight at random, below the rounding of the BF16 result; two
+// BF16 parts would cost half as much tensor work again. Scores, m, l and O are FP32.
+// Masked positions cannot leak: hidden keys' scores are replaced, V rows that nothing in the
+// block sees are zeroed in shared memory, and when a tile that only some queries see holds
+// a V value that is not finite (0 x inf), the block recomputes its sums key by key.
+//
+// Few blocks (a chunk of one prompt) are split along the keys over a cluster of 2 or 4, whose
+// states are joined through distributed shared memory, each block finishing D / C columns.
+#include <cuda.h>
+
+#include <algorithm>
+#include <string>
+
+#include "common.cuh"
+#include "kv_ops.h"
+#include "tcgen05.cuh"
+
+namespace yar {
+
+namespace {
+constexpr int kPreM = 128, kPreN = 128;  // M rows of a tile, keys of a tile
+// Three warpgroups, launched with 168 registers a thread: the third (copies, products) gives
+// up 96 of them and the two softmax ones take 48 each: 2 x 216 + 72 = 3 x 168.
+constexpr int kPreThreads = 384, kPreRegs = 168, kPreRegsSoftmax = 216, kPreRegsIssue = 72;
+static_assert(2 * kPreRegsSoftmax + kPreRegsIssue == 3 * kPreRegs, "no more registers than the launch holds");
+
+template <int D>
+struct PreCfg {
+  static constexpr int kSlice = 128 * 128;           // 128 rows of 64 values
+  static constexpr int kTile = (D / 64) * kSlice;    // a Q, K or V tile
+  static constexpr int kStages = D == 128 ? 5 : 10;  // K and V tiles in flight: 160 KB
+  static constexpr int kSmem = 2 * kTile + kStages * kTile + 1024;
+  // kind::f16, FP32 accumulator, BF16 A and B, A K-major, N >> 3 at bit 17, M >> 4 at bit 24;
+  // P V reads B (V) MN-major (bit 16).
+  static constexpr uint32_t kIdescS =
+      (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(kPreN >> 3) << 17) | (uint32_t(kPreM >> 4) << 24);
+  static constexpr uint32_t kIdescO =
+      (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (uint32_t(D >> 3) << 17) | (uint32_t(kPreM >> 4) << 24);
+};
+constexpr uint32_t kPreColO = 256, kPreCols = 512;  // S (and P) of A, B at columns 0, 128; O at 256, 384
+constexpr float kPreRescale = 8.f;
+
+struct PrefillExtra {
+  int row0;        // the layer's first cached row in the pool seen as [rows][D]
+  int total_rows;  // rows of the pool: the out-of-bounds coordinate
+  int box_rows;    // keys of one box
+  int pairs;       // upper bound of the blocks' M-row pairs
+};
+
+// A bounded wait that also ends when another role gave up.
+__device__ __forceinline__ bool pre_wait(uint64_t *bar, unsigned parity, const volatile int *fail) {
+  for (long long i = 0; i < kAtWaitLimit; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(done)
+        : "r"(at_smem(bar)), "r"(parity)
+        : "memory");
+    if (done) return true;
+    if ((i & 255) == 255 && *fail) return false;
+  }
+  return false;
+}
+// 2^x by the approximate base-2 exponential, results below 2^-126 as 0 (relative error below
+// 2^-22): without that flush each exponential costs three more instructions.
+__device__ __forceinline__ float pre_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Store 32 columns of this warp's lanes (not waited for).
+__device__ __forceinline__ void st32_async(uint32_t addr, const uint32_t *v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
+      "%13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
+      "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
+      "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+__device__ __forceinline__ void pre_cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t pre_mapa(uint32_t a, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+  return r;
+}
+
+// Where a block's work lies.
+struct PreBlock {
+  int row, first, n, len;  // the row, its first query, its queries, its cached positions
+  int pair;
+  int p0, p1;                // positions of its first and last query
+  int kend, lo, sinks;       // keys seen by any query: [0, sinks) and [lo, kend)
+  int sink_tiles, wfirst;    // key tile j: j < sink_tiles ? j : wfirst + j - sink_tiles
+  int j0, j1;                // this block's share of the key tiles
+};
+struct PreTile {  // one of A, B: positions of its first and last row (exists: has rows)
+  bool exists;
+  int pmin, pmax;
+};
+
+template <int D>
+__global__ void __launch_bounds__(kPreThreads, 1)
+    k_kv_attn_prefill(const __grid_constant__ CUtensorMap map, const __grid_constant__ KvAttnParams p,
+                      const __grid_constant__ PrefillExtra x) {
+  using Cfg = PreCfg<D>;
+  constexpr int NST = Cfg::kStages;
+  extern __shared__ unsigned char pre_raw[];
+  unsigned char *sm = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(pre_raw) + 1023) & ~uintptr_t(1023));
+  unsigned char *ring = sm + 2 * Cfg::kTile;
+  __shared__ __align__(8) uint64_t kv_full[NST], kv_empty[NST], s_full[2], p_ready[2], o_done[2], drain;
+  __shared__ PreBlock blk;
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int s_fail, s_poison[2], s_bad;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, kvh = blockIdx.y, G = p.heads / p.kv_heads;
+  uint32_t C, rank;
+  asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(C));
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+
+  // ---- which row and which 256 of its M rows: the last pairs (the longest) first -----------
+  if (warp == 0) {
+    const int slot = x.pairs - 1 - int(blockIdx.x / C);
+    int row = -1, first = 0, n = 0, pair = 0;
+    if (!p.offsets) {
+      row = 0, n = p.n_queries, pair = slot;
+      if ((long long)pair * 256 >= (long long)n * G) row = -1;
+    } else {
+      int before = 0;
+      for (int r0 = 0; r0 < p.rows && row < 0; r0 += 32) {
+        const int r = r0 + lane;
+        int f = 0, k = 0;
+        if (r < p.rows) {
+          f = p.offsets[r];
+          const int e = p.offsets[r + 1];
+          if (f >= 0 && e >= f && e <= p.n_queries)
+            k = e - f;
+          else if (p.error)
+            atomicOr(p.error, kKvBadOffsets);
+        }
+        const int mine = int(((long long)k * G + 255) / 256);
+        int incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int v = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+          if (lane >= o) incl += v;
+        }
+        const unsigned hit = __ballot_sync(0xFFFFFFFFu, slot - before < incl);
+        if (hit) {
+          const int src = __ffs(hit) - 1;
+          row = r0 + src;
+          first = __shfl_sync(0xFFFFFFFFu, f, src);
+          n = __shfl_sync(0xFFFFFFFFu, k, src);
+          pair = slot - before - __shfl_sync(0xFFFFFFFFu, incl - mine, src);
+        }
+        before += __shfl_sync(0xFFFFFFFFu, incl, 31);
+      }
+    }
+    if (lane == 0) {
+      PreBlock b;
+      b.row = row, b.first = first, b.n = n, b.pair = pair;
+      if (row >= 0) {
+        const int cap = p.pages_per_row << p.page_shift;
+        int len = p.lengths ? p.lengths[row] : p.length;
+        if (len > cap) {
+          if (p.error) atomicOr(p.error, kKvBadLength);
+          len = cap;
+        }
+        b.len = max(len, 0);
+        const long long m0 = (long long)pair * 256, m1 = min((long long)n * G, m0 + 256) - 1;
+        b.p0 = b.len - n + int(m0 / G);
+        b.p1 = b.len - n + int(m1 / G);
+        b.kend = b.p1 + 1;
+        b.lo = p.window ? max(0, b.p0 - p.window + 1) : 0;
+        b.sinks = p.window ? min(p.sinks, b.lo) : 0;
+        b.sink_tiles = (b.sinks + kPreN - 1) / kPreN;
+        b.wfirst = max(b.sink_tiles, b.lo / kPreN);
+        const int total = b.kend <= 0 ? 0 : b.sink_tiles + max(0, (b.kend + kPreN - 1) / kPreN - b.wfirst);
+        const int per = (total + int(C) - 1) / int(C);
+        b.j0 = min(total, int(rank) * per), b.j1 = min(total, b.j0 + per);
+      }
+      blk = b;
+      s_fail = 0, s_poison[0] = 0, s_poison[1] = 0, s_bad = 0;
+      for (int s = 0; s < NST; ++s) {
+        asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(at_smem(&kv_full[s])));
+        asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(at_smem(&kv_empty[s])));
+      }
+      for (int i = 0; i < 2; ++i) {
+        asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(at_smem(&s_full[i])));
+        asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(at_smem(&p_ready[i])), "r"(kPreM));
+        asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(at_smem(&o_done[i])));
+      }
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(at_smem(&drain)));
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+  }
+  __syncthreads();
+  const PreBlock b = blk;
+  if (b.row < 0) return;  // (a cluster's blocks share their pair: all of them leave)
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(at_smem(&tmem_slot)),
+                 "r"(kPreCols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+  }
+  const int *tab = p.table + size_t(b.row) * p.table_stride;
+  const int pieces = kPreN / x.box_rows;
+  auto key_tile = [&](int j) { return (j < b.sink_tiles ? j : b.wfirst + j - b.sink_tiles) * kPreN; };
+  // Whether some query of the block sees a key in [k0, k1).
+  auto needed = [&](int k0, int k1) { return k0 < b.kend && !(k0 >= b.sinks && k1 <= b.lo); };
+  // Bad pages among the keys to come (their pieces are then masked one by one).
+  for (int i = tid; i < (b.j1 - b.j0) * pieces; i += kPreThreads) {
+    const int k0 = key_tile(b.j0 + i / pieces) + (i % pieces) * x.box_rows;
+    if (needed(k0, k0 + x.box_rows)) {
+      const int page = tab[k0 >> p.page_shift];
+      if (page < 0 || page >= p.pages) {
+        s_bad = 1;
+        if (p.error) atomicOr(p.error, kKvBadPage);
+      }
+    }
+  }
+  const long long rows_m = (long long)b.n * G;
+  auto tile_of = [&](int t) {
+    PreTile r;
+    const long long m0 = (long long)b.pair * 256 + t * kPreM, m1 = min(rows_m, m0 + kPreM) - 1;
+    r.exists = m0 < rows_m;
+    r.pmin = b.len - b.n + int(m0 / G);
+    r.pmax = r.exists ? b.len - b.n + int(m1 / G) : -1;
+    return r;
+  };
+  auto live = [&](const PreTile &t, int j) {  // some row of the tile sees a key of key tile j
+    const int k0 = key_tile(j);
+    return t.exists && k0 <= t.pmax && (!p.window || k0 < p.sinks || k0 + kPreN - 1 > t.pmin - p.window);
+  };
+
+  // ---- Q: M row t of tile A or B into its swizzled slices -----------------------------------
+  const int wg = warp >> 2, t = tid & 127;
+  const long long m = (long long)b.pair * 256 + wg * kPreM + t;
+  const bool mine = warp < 8 && m < rows_m;
+  const int qi = mine ? int(m / G) : 0, head = kvh * G + (mine ? int(m % G) : 0);
+  const bf16 *q_row = p.q + size_t(b.first + qi) * p.q_stride + size_t(head) * D;
+  if (warp < 8) {
+#pragma unroll
+    for (int c = 0; c < D / 8; ++c) {
+      const uint4 v = mine ? *reinterpret_cast<const uint4 *>(q_row + c * 8) : make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4 *>(sm + wg * Cfg::kTile + (c >> 3) * Cfg::kSlice + at_sw(t, c & 7)) = v;
+    }
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = tmem_slot;
+  auto stage = [&](int it) { return ring + (it % NST) * Cfg::kTile; };  // K of tile j: it = 2 (j - j0), V: + 1
+
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPreRegsIssue));
+  if (warp == 9) {
+    // ---- copies ---------------------------------------------------------------------------
+    int issued = 0;
+    bool ok = true;
+    for (int j = b.j0; j < b.j1 && ok; ++j) {
+      int y = x.total_rows;  // K's row of this lane's piece; out of bounds: zeros
+      const int k0 = key_tile(j) + lane * x.box_rows;
+      if (lane < pieces && needed(k0, k0 + x.box_rows)) {
+        const int page = tab[k0 >> p.page_shift];
+        if (page >= 0 && page < p.pages)
+          y = x.row0 + (((page * 2 * p.kv_heads) + kvh) << p.page_shift) + (k0 & ((1 << p.page_shift) - 1));
+      }
+      for (int kv = 0; kv < 2; ++kv) {
+        const int it = 2 * (j - b.j0) + kv, s = it % NST;
+        if (it >= NST && !pre_wait(&kv_empty[s], unsigned(it / NST - 1) & 1u, &s_fail)) ok = false;
+        if (!__all_sync(0xFFFFFFFFu, ok)) {
+          ok = false;
+          break;
+        }
+        if (lane == 0)
+          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(at_smem(&kv_full[s])),
+                       "r"(Cfg::kTile)
+                       : "memory");
+        __syncwarp();
+        if (lane < pieces) {
+          const int yv = y == x.total_rows ? y : y + ((kv * p.kv_heads) << p.page_shift);
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c)
+            asm volatile(
+                "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, "
+                "%4}], [%2];" ::"r"(at_smem(stage(it) + c * Cfg::kSlice + lane * x.box_rows * 128)),
+                "l"(&map), "r"(at_smem(&kv_full[s])), "r"(c * 64), "r"(yv)
+                : "memory");
+        }
+        issued = it + 1;
+      }
+    }
+    if (!ok) {  // leave no copy in flight
+      s_fail = 1;
+      for (int i = issued > NST ? issued - NST : 0; i < issued; ++i)
+        at_wait(&kv_full[i % NST], unsigned(i / NST) & 1u);
+      if (lane == 0 && p.error) atomicOr(p.error, kKvExpired);
+    }
+  } else if (warp == 8) {
+    // ---- products -------------------------------------------------------------------------
+    const PreTile tl[2] = {tile_of(0), tile_of(1)};
+    bool ok = true, started[2] = {false, false};
+    unsigned n_p[2] = {0u, 0u};
+    auto wait_full = [&](int it) {
+      ok = ok && pre_wait(&kv_full[it % NST], unsigned(it / NST) & 1u, &s_fail);
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    };
+    auto issue_s = [&](int X, int it) {
+      if (lane == 0) {
+        const unsigned char *k = stage(it);
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks)
+          at_mma(tmem + X * kPreN, at_desc(sm + X * Cfg::kTile + (ks >> 2) * Cfg::kSlice) + 2 * (ks & 3),
+                 at_desc(k + (ks >> 2) * Cfg::kSlice) + 2 * (ks & 3), Cfg::kIdescS, uint32_t(ks != 0));
+        at_commit(&s_full[X]);
+      }
+      __syncwarp();
+    };
+    if (b.j0 < b.j1) {
+      wait_full(0);
+      if (ok) {
+        for (int X = 0; X < 2; ++X)
+          if (live(tl[X], b.j0)) issue_s(X, 0);
+        if (lane == 0) at_commit(&kv_empty[0]);
+      }
+    }
+    for (int j = b.j0; j < b.j1 && ok; ++j) {
+      const int it = 2 * (j - b.j0) + 1, k0 = key_tile(j);
+      wait_full(it);
+      if (!ok) break;
+      unsigned char *v = stage(it);
+      if (k0 + kPreN > b.kend || (k0 + kPreN > b.sinks && k0 < b.lo)) {
+        // V rows that nothing in the block sees: zeros (their P is 0, the rows may hold any bits).
+        for (int r = 0; r < kPreN; ++r)
+          if (k0 + r >= b.kend || (k0 + r >= b.sinks && k0 + r < b.lo))
+            if (lane < D / 8)
+              *reinterpret_cast<uint4 *>(v + (lane >> 3) * Cfg::kSlice + r * 128 + (lane & 7) * 16) =
+                  make_uint4(0, 0, 0, 0);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+      }
+      bool k_there = false;
+      for (int X = 0; X < 2 && ok; ++X) {
+        if (live(tl[X], j)) {
+          ok = pre_wait(&p_ready[X], n_p[X]++ & 1u, &s_fail);
+          ok = __all_sync(0xFFFFFFFFu, ok);
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          if (lane == 0) {
+#pragma unroll
+            for (int ks = 0; ks < kPreN / 16; ++ks)
+              at_mma_ts(tmem + kPreColO + X * 128, tmem + X * kPreN + 8 * ks,
+                        at_desc_mn(v, Cfg::kSlice) + uint64_t(ks) * (2048 >> 4), Cfg::kIdescO,
+                        uint32_t(started[X] || ks > 0));
+          }
+          started[X] = true;
+          bool more = false;
+          for (int i = j + 1; i < b.j1 && !more; ++i) more = live(tl[X], i);
+          if (!more && lane == 0) at_commit(&o_done[X]);
+        }
+        if (X == 1 && lane == 0) at_commit(&kv_empty[it % NST]);
+        if (j + 1 < b.j1 && live(tl[X], j + 1)) {
+          if (!k_there) wait_full(it + 1);
+          k_there = true;
+          if (ok) issue_s(X, it + 1);
+        }
+      }
+      if (ok && j + 1 < b.j1) {
+        if (!k_there) wait_full(it + 1);
+        if (lane == 0) at_commit(&kv_empty[(it + 1) % NST]);
+      }
+    }
+    // Every product issued has completed before the block's tensor memory goes.
+    if (lane == 0) at_commit(&drain);
+    __syncwarp();
+    if (!at_wait(&drain, 0u) || !ok) {
+      s_fail = 1;
+      if (lane == 0 && p.error) atomicOr(p.error, kKvExpired);
+    }
+  }
+  if (C > 1) {  // the softmax warps' two exchanges
+    pre_cluster_sync();
+    pre_cluster_sync();
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPreRegsSoftmax));
+    // ---- softmax: the thread's M row ------------------------------------------------------
+    const PreTile tl = tile_of(wg);
+    const int pos = mine ? max(b.len - b.n + qi, -1) : -1;
+    const float sl2 = p.scale * 1.4426950408889634f;
+    const uint32_t lanes = tmem + (uint32_t((warp & 3) * 32) << 16);
+    const uint32_t col_s = lanes + wg * kPreN, col_o = lanes + kPreColO + wg * 128;
+    unsigned n_s = 0u;
+    bool ok = true;
+    float row_m = -INFINITY, row_l = 0.f;  // running maximum and sum
+    for (int j = b.j0; j < b.j1; ++j) {
+      if (!live(tl, j)) continue;
+      ok = pre_wait(&s_full[wg], n_s & 1u, &s_fail);
+      if (!__all_sync(0xFFFFFFFFu, ok)) {
+        ok = false;
+        break;
+      }
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const int k0 = key_tile(j);
+      float s[kPreN];
+      at_ld64(col_s, s);
+      at_ld64(col_s + 64, s + 64);
+      const bool whole = k0 + kPreN - 1 <= tl.pmin &&
+                         (!p.window || k0 + kPreN - 1 < p.sinks || k0 > tl.pmax - p.window);
+      if (!whole || s_bad) {
+        // k visible: k <= hi and (k < sink or k > old).
+        const int hi = pos - k0, sink = p.window ? p.sinks - k0 : 1 << 30, old = pos - p.window - k0;
+#pragma unroll
+        for (int k = 0; k < kPreN; ++k) s[k] = k <= hi && (k < sink || k > old) ? s[k] : -INFINITY;
+        if (s_bad) {
+#pragma unroll
+          for (int c = 0; c < kPreN / 16; ++c) {
+            const int kk = k0 + 16 * c;
+            const int page = needed(kk, kk + 16) ? tab[kk >> p.page_shift] : 0;
+            if (page < 0 || page >= p.pages) {
+#pragma unroll
+              for (int k = 0; k < 16; ++k) s[16 * c + k] = -INFINITY;
+            }
+          }
+        }
+        // A V value that is not finite in a row that only some of the queries see: the product
+        // with P = 0 would carry it into the others (thread t looks at V row t).
+        const int it = 2 * (j - b.j0) + 1;
+        ok = pre_wait(&kv_full[it % NST], unsigned(it / NST) & 1u, &s_fail);
+        if (!__all_sync(0xFFFFFFFFu, ok)) {
+          ok = false;
+          break;
+        }
+        if (k0 + t < b.kend && !(k0 + t >= b.sinks && k0 + t < b.lo)) {
+          __nv_bfloat162 acc = __floats2bfloat162_rn(0.f, 0.f);
+          const __nv_bfloat162 zero = acc;
+          const unsigned char *v = stage(it) + t * 128;
+#pragma unroll
+          for (int c = 0; c < D / 8; ++c) {
+            const uint4 w = *reinterpret_cast<const uint4 *>(v + (c >> 3) * Cfg::kSlice + (c & 7) * 16);
+            const uint32_t e[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc = __hfma2(*reinterpret_cast<const __nv_bfloat162 *>(&e[i]), zero, acc);
+          }
+          const float2 f = __bfloat1622float2(acc);
+          if (f.x != 0.f || f.y != 0.f) s_poison[wg] = 1;
+        }
+      }
+      float mx8[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mx8[i] = s[i];
+#pragma unroll
+      for (int k = 8; k < kPreN; ++k) mx8[k & 7] = fmaxf(mx8[k & 7], s[k]);
+      const float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])),
+                             fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7]))) *
+                       sl2;
+      const bool raise = mx > row_m + kPreRescale;  // false while both are -inf
+      if (__any_sync(0xFFFFFFFFu, raise)) {
+        const float c = raise ? pre_ex2(row_m - mx) : 1.f;  // 0 when m was -inf
+        row_l *= c;
+        row_m = raise ? mx : row_m;
+        // S of this tile was issued behind the last P V, so O is complete and still.
+        if (n_s > 0) {
+#pragma unroll
+          for (int cb = 0; cb < D; cb += 32) {
+            float v[32];
+            at_ld32(col_o + cb, v);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] *= c;
+            at_st32(col_o + cb, v);
+          }
+        }
+      }
+      ++n_s;
+      const float nm = row_m == -INFINITY ? 0.f : -row_m;
+      float ps[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t w[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const float e0 = pre_ex2(fmaf(s[64 * c + 2 * i], sl2, nm)), e1 = pre_ex2(fmaf(s[64 * c + 2 * i + 1], sl2, nm));
+          ps[i & 1] += e0, ps[2 + (i & 1)] += e1;
+          const __nv_bfloat162 h = __floats2bfloat162_rn(e0, e1);
+          w[i] = *reinterpret_cast<const uint32_t *>(&h);
+        }
+        st32_async(col_s + 32 * c, w);
+      }
+      row_l += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      at_arrive(&p_ready[wg]);
+    }
+    if (ok && n_s > 0) ok = pre_wait(&o_done[wg], 0u, &s_fail);
+    if (!__all_sync(0xFFFFFFFFu, ok)) {
+      s_fail = 1;
+      if (lane == 0 && p.error) atomicOr(p.error, kKvExpired);
+    }
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + wg), "n"(kPreM) : "memory");  // the tile's flags are complete
+    // ---- the result ---------------------------------------------------------------------------
+    const bool failed = s_fail != 0;
+    if (s_poison[wg] && !failed) {
+      // Key by key with the statistics from above (V does not enter them), 32 columns at a time.
+      const float nm = row_m == -INFINITY ? 0.f : -row_m;
+      for (int cb = 0; cb < D; cb += 32) {
+        float o[32];
+  #pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = 0.f;
+        for (int j = b.j0; j < b.j1; ++j)
+          for (int k = key_tile(j); k < key_tile(j) + kPreN; ++k) {
+            if (!mine || row_l == 0.f || k > pos || (p.window && k >= p.sinks && k <= pos - p.window)) continue;
+            const int page = tab[k >> p.page_shift];
+            if (page < 0 || page >= p.pages) continue;
+            const bf16 *kr = p.kv + size_t(page) * p.page_elems +
+                             ((size_t(kvh) << p.page_shift) + (k & ((1 << p.page_shift) - 1))) * D;
+            float s = 0.f;
+            for (int d = 0; d < D; ++d) s = fmaf(bf2f(q_row[d]), bf2f(kr[d]), s);
+            const float e = pre_ex2(fmaf(s, sl2, nm));
+  #pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = fmaf(e, bf2f(kr[p.page_elems / 2 + cb + i]), o[i]);
+          }
+        __syncwarp();
+        at_st32(col_o + cb, o);
+      }
+    }
+    if (C == 1) {
+      if (!failed) {
+        const float inv = row_l == 0.f ? 0.f : 1.0f / row_l;
+        bf16 *dst = p.out + size_t(b.first + qi) * p.out_stride + size_t(head) * D;
+  #pragma unroll
+        for (int cb = 0; cb < D; cb += 32) {
+          float v[32];
+          at_ld32(col_o + cb, v);
+          if (mine) {
+  #pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              uint32_t w[4];
+  #pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                // (a row that saw nothing: O was never written)
+                const __nv_bfloat162 o2 = row_l == 0.f ? __floats2bfloat162_rn(0.f, 0.f)
+                                                       : __floats2bfloat162_rn(v[c * 8 + 2 * e] * inv, v[c * 8 + 2 * e + 1] * inv);
+                w[e] = *reinterpret_cast<const uint32_t *>(&o2);
+              }
+              *reinterpret_cast<uint4 *>(dst + cb + c * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+        }
+      }
+    } else {
+      // The cluster's states of a row weighted by 2^(m - M); block r finishes columns
+      // [r D / C, (r + 1) D / C): the others send it theirs ([sender][4 columns][M row], 16 bytes
+      // each) into its ring, which no copy or product uses any more.
+      // (m and l go where the tile's Q was: its products are complete.)
+      float2 *ml = reinterpret_cast<float2 *>(sm + wg * Cfg::kTile) + t;
+      *ml = make_float2(row_m, row_l);
+      pre_cluster_sync();
+      float M = -INFINITY, L = 0.f, w = 0.f;
+      {
+        float mv[4], lv[4];
+  #pragma unroll
+        for (uint32_t c = 0; c < 4; ++c) {
+          mv[c] = -INFINITY, lv[c] = 0.f;
+          if (c < C) {
+            const uint32_t a = pre_mapa(at_smem(ml), c);
+            asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(mv[c]), "=f"(lv[c]) : "r"(a) : "memory");
+          }
+          M = fmaxf(M, mv[c]);
+        }
+  #pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (lv[c] != 0.f) L += lv[c] * (mv[c] == M ? 1.f : pre_ex2(mv[c] - M));
+        w = row_l == 0.f ? 0.f : row_m == M ? 1.f : pre_ex2(row_m - M);
+      }
+      const int cols = D / int(C), own = int(rank) * cols;
+      float mine_o[D / 2];  // this block's columns (C >= 2)
+      if (warp < 8) {
+  #pragma unroll
+        for (int cb = 0; cb < D; cb += 32) {
+          float v[32];
+          at_ld32(col_o + cb, v);
+  #pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = row_l == 0.f ? 0.f : v[i] * w;
+  #pragma unroll
+          for (int h = 0; h < 2; ++h) {  // 16 columns: all of one block's (cols is 16, 32 or 64)
+            const int r = (cb + 16 * h) / cols, at = (cb + 16 * h) % cols;
+            if (r == int(rank)) {
+  #pragma unroll
+              for (int q4 = 0; q4 < D / 32; ++q4)  // at = 16 q4 (static indexes only)
+                if (at == 16 * q4) {
+  #pragma unroll
+                  for (int i = 0; i < 16; ++i) mine_o[16 * q4 + i] = v[16 * h + i];
+                }
+            } else {
+              const int sender = int(rank) < r ? int(rank) : int(rank) - 1;
+  #pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                const uint32_t a =
+                    pre_mapa(at_smem(ring + ((size_t(sender) * (cols / 4) + at / 4 + c) * 256 + wg * kPreM + t) * 16), r);
+                asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(a), "f"(v[16 * h + 4 * c]),
+                             "f"(v[16 * h + 4 * c + 1]), "f"(v[16 * h + 4 * c + 2]), "f"(v[16 * h + 4 * c + 3])
+                             : "memory");
+              }
+            }
+          }
+        }
+      }
+      pre_cluster_sync();
+      if (mine && !failed) {
+        const float inv = L == 0.f ? 0.f : 1.0f / L;
+        bf16 *dst = p.out + size_t(b.first + qi) * p.out_stride + size_t(head) * D + own;
+  #pragma unroll
+        for (int c8 = 0; c8 < D / 16; ++c8) {
+          if (c8 * 8 < cols) {
+            float v[8];
+  #pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = mine_o[8 * c8 + i];
+            for (int s = 0; s + 1 < int(C); ++s)
+  #pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const float4 f = *reinterpret_cast<const float4 *>(
+                    ring + ((size_t(s) * (cols / 4) + 2 * c8 + h) * 256 + wg * kPreM + t) * 16);
+                v[4 * h] += f.x, v[4 * h + 1] += f.y, v[4 * h + 2] += f.z, v[4 * h + 3] += f.w;
+              }
+            uint32_t o[4];
+  #pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const __nv_bfloat162 o2 = __floats2bfloat162_rn(v[2 * e] * inv, v[2 * e + 1] * inv);
+              o[e] = *reinterpret_cast<const uint32_t *>(&o2);
+            }
+            *reinterpret_cast<uint4 *>(dst + 8 * c8) = make_uint4(o[0], o[1], o[2], o[3]);
+          }
+        }
+      }
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kPreCols));
+}
+
+template <int D>
+void prefill_launch(const CUtensorMap &map, const KvAttnParams &p, const PrefillExtra &x, int cluster, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(x.pairs) * cluster, p.kv_heads);
+  cfg.blockDim = dim3(kPreThreads);
+  cfg.dynamicSmemBytes = PreCfg<D>::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  YAR_CUDA(cudaLaunchKernelEx(&cfg, k_kv_attn_prefill<D>, map, p, x));
+}
+}  // namespace
+
+void launch_kv_attn_prefill(const KvPool &pool, int layer, const KvAttnParams &p, cudaStream_t st) {
+  if (p.n_queries <= 0 || p.rows <= 0) return;
+  PrefillExtra x;
+  const long long layer_rows = 2ll * pool.pages * pool.kv_heads * pool.page_tokens;
+  x.row0 = int(layer * layer_rows);
+  x.total_rows = int(pool.layers * layer_rows);
+  x.box_rows = std::min(pool.page_tokens, kPreN);
+  const long long G = p.heads / p.kv_heads;
+  // Pairs of 256 M rows: exactly, or rounded up for each row of queries.
+  const long long pairs = (p.n_queries * G + 255) / 256 + (p.offsets ? p.rows - 1 : 0);
+  if (pairs > (1 << 28)) throw Error("ValueError", "too many queries for one call");
+  x.pairs = int(pairs);
+  CUtensorMap map;
+  if (!encode_rows_map(&map, pool.data, uint64_t(x.total_rows), pool.head_dim, x.box_rows))
+    throw Error("RuntimeError", "cuTensorMapEncodeTiled failed for the cache pool");
+  const int cluster = 1;
+  if (pool.head_dim == 128)
+    prefill_launch<128>(map, p, x, cluster, st);
+  else
+    prefill_launch<64>(map, p, x, cluster, st);
+}
+
+template <int D>
+static void prefill_configure() {
+  YAR_CUDA(cudaFuncSetAttribute(k_kv_attn_prefill<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, PreCfg<D>::kSmem));
+  // The register split waits for ever when the launch holds fewer registers than it hands out.
+  cudaFuncAttributes a;
+  YAR_CUDA(cudaFuncGetAttributes(&a, k_kv_attn_prefill<D>));
+  if (a.numRegs != kPreRegs)
+    throw Error("RuntimeError", "prefill attention built with " + std::to_string(a.numRegs) + " registers, not 168");
+}
+void configure_kv_prefill_kernels() {
+  prefill_configure<128>();
+  prefill_configure<64>();
+}
+
+}  // namespace yar

@@ -3,7 +3,7 @@
 // Nothing here allocates or waits.
 #include "kv_ops.h"
 
-#include <climits>
+#include <algorithm>
 #include <cmath>
 #include <mutex>
 #include <string>
@@ -124,8 +124,8 @@ KvAttnParams attn_params(const KvPool &pool, int layer, const ::yar_kv_rows *row
   p.q_stride = q_stride;
   p.out = static_cast<bf16 *>(out);
   p.out_stride = out_stride;
-  p.window = window;
-  p.sinks = sinks;
+  p.window = std::min(window, kKvMaxPositions - 1);  // (no row holds more: position arithmetic stays in 32 bits)
+  p.sinks = std::min(sinks, kKvMaxPositions - 1);
   p.scale = float(scale);
   p.error = error;
   return p;

@@ -56,6 +56,7 @@ void launch_kv_compact(const KvPool &pool, const int *table, long long table_str
                        const int *counts, int *new_table, long long new_stride, int *remap, int *used, int *work,
                        int *error, cudaStream_t st);
 void configure_kv_attn_kernels();
+void configure_kv_prefill_kernels();
 void configure_kv_kernels();
 
 }  // namespace yar
