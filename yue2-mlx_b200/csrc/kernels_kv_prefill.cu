@@ -4,14 +4,14 @@
 // softmax(scale q K^T) V per query over the visible positions. The queries of one row and KV
 // head are flattened to M rows (query-major: row m is query m / G, head m % G), so a group
 // shares every K and V tile and short chunks fill their tiles. A block takes 256 M rows as
-// two tiles A and B of 128, and walks the 128-key tiles that any of its queries sees (the
-// sinks' tiles, then the window's). Its warps (10 and 11 idle):
-//   * warp 9 brings K and V tiles by TMA through a ring (one box per page piece; pieces that
+// two tiles A and B of 128, and walks the 64-key tiles that any of its queries sees (the
+// sinks' tiles, then the window's). Its warps (11 idle):
+//   * warp 10 brings K and V tiles by TMA through a ring (one box per page piece; pieces that
 //     nothing sees, or whose page is bad, are fetched out of bounds: zeros);
-//   * lane 0 of warp 8 issues the products: S = Q K^T into TMEM (128 columns for each of A
-//     and B), and O += P V with P read from TMEM, where the softmax warps left it in S's own
-//     columns. While A's softmax runs the tensor pipe works for B, and the other way round;
-//   * warps 0..3 (A) and 4..7 (B): a thread owns one M row (= TMEM lane). It reads its 128
+//   * one lane of warp 8 (A) and of warp 9 (B) issues the products: S = Q K^T into one of two
+//     TMEM buffers of 64 columns, two key tiles ahead, and O += P V with P read from TMEM,
+//     where the softmax warps left it in S's own columns;
+//   * warps 0..3 (A) and 4..7 (B): a thread owns one M row (= TMEM lane). It reads its 64
 //     scores, masks them (tiles on an edge only), raises its running maximum m when the tile
 //     exceeds it by more than 8 (in log2 units; O in TMEM is rescaled only then: O / l is
 //     the same quotient whichever m the terms share), writes P = 2^(s - m) as BF16 and adds
@@ -36,7 +36,7 @@
 namespace yar {
 
 namespace {
-constexpr int kPreM = 128, kPreN = 128;  // M rows of a tile, keys of a tile
+constexpr int kPreM = 128, kPreN = 64;  // M rows of a tile, keys of a tile
 // Three warpgroups, launched with 168 registers a thread: the third (copies, products) gives
 // up 96 of them and the two softmax ones take 48 each: 2 x 216 + 72 = 3 x 168.
 constexpr int kPreThreads = 384, kPreRegs = 168, kPreRegsSoftmax = 216, kPreRegsIssue = 72;
@@ -44,10 +44,10 @@ static_assert(2 * kPreRegsSoftmax + kPreRegsIssue == 3 * kPreRegs, "no more regi
 
 template <int D>
 struct PreCfg {
-  static constexpr int kSlice = 128 * 128;           // 128 rows of 64 values
-  static constexpr int kTile = (D / 64) * kSlice;    // a Q, K or V tile
-  static constexpr int kStages = D == 128 ? 5 : 10;  // K and V tiles in flight: 160 KB
-  static constexpr int kSmem = 2 * kTile + kStages * kTile + 1024;
+  static constexpr int kQSlice = kPreM * 128, kQ = (D / 64) * kQSlice;    // 128 rows of 64 values; a Q tile
+  static constexpr int kSlice = kPreN * 128, kTile = (D / 64) * kSlice;  // the same of a K or V tile
+  static constexpr int kStages = D == 128 ? 10 : 20;                     // K and V tiles in flight: 160 KB
+  static constexpr int kSmem = 2 * kQ + kStages * kTile + 1024;
   // kind::f16, FP32 accumulator, BF16 A and B, A K-major, N >> 3 at bit 17, M >> 4 at bit 24;
   // P V reads B (V) MN-major (bit 16).
   static constexpr uint32_t kIdescS =
@@ -55,7 +55,8 @@ struct PreCfg {
   static constexpr uint32_t kIdescO =
       (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (uint32_t(D >> 3) << 17) | (uint32_t(kPreM >> 4) << 24);
 };
-constexpr uint32_t kPreColO = 256, kPreCols = 512;  // S (and P) of A, B at columns 0, 128; O at 256, 384
+// Tensor memory: two S (and P) buffers of A at columns 0 and 64, of B at 128 and 192, O at 256, 384.
+constexpr uint32_t kPreColO = 256, kPreCols = 512;
 constexpr float kPreRescale = 8.f;
 
 struct PrefillExtra {
@@ -86,6 +87,30 @@ __device__ __forceinline__ float pre_ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// Two FP32 values in one operation (each rounded as the single one is).
+__device__ __forceinline__ uint64_t pair64(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void split64(uint64_t v, float &lo, float &hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 // Store 32 columns of this warp's lanes (not waited for).
 __device__ __forceinline__ void st32_async(uint32_t addr, const uint32_t *v) {
   asm volatile(
@@ -115,9 +140,9 @@ struct PreBlock {
   int sink_tiles, wfirst;    // key tile j: j < sink_tiles ? j : wfirst + j - sink_tiles
   int j0, j1;                // this block's share of the key tiles
 };
-struct PreTile {  // one of A, B: positions of its first and last row (exists: has rows)
-  bool exists;
-  int pmin, pmax;
+struct PreTile {  // one of A, B
+  int pmin, pmax;  // positions of its first and last row (pmax -1: it has no rows)
+  int s1, w0, w1;  // the block's key tiles that it sees: [0, s1) (sinks) and [w0, w1)
 };
 
 template <int D>
@@ -128,8 +153,8 @@ __global__ void __launch_bounds__(kPreThreads, 1)
   constexpr int NST = Cfg::kStages;
   extern __shared__ unsigned char pre_raw[];
   unsigned char *sm = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(pre_raw) + 1023) & ~uintptr_t(1023));
-  unsigned char *ring = sm + 2 * Cfg::kTile;
-  __shared__ __align__(8) uint64_t kv_full[NST], kv_empty[NST], s_full[2], p_ready[2], o_done[2], drain;
+  unsigned char *ring = sm + 2 * Cfg::kQ;
+  __shared__ __align__(8) uint64_t kv_full[NST], kv_empty[NST], s_full[2][2], p_ready[2][2], o_done[2][2], drain[2];
   __shared__ PreBlock blk;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int s_fail, s_poison[2], s_bad;
@@ -203,14 +228,14 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       s_fail = 0, s_poison[0] = 0, s_poison[1] = 0, s_bad = 0;
       for (int s = 0; s < NST; ++s) {
         asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(at_smem(&kv_full[s])));
-        asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(at_smem(&kv_empty[s])));
+        asm volatile("mbarrier.init.shared::cta.b64 [%0], 2;" ::"r"(at_smem(&kv_empty[s])));
       }
-      for (int i = 0; i < 2; ++i) {
-        asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(at_smem(&s_full[i])));
-        asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(at_smem(&p_ready[i])), "r"(kPreM));
-        asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(at_smem(&o_done[i])));
+      for (int i = 0; i < 4; ++i) {
+        asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(at_smem(&s_full[i >> 1][i & 1])));
+        asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(at_smem(&p_ready[i >> 1][i & 1])), "r"(kPreM));
+        asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(at_smem(&o_done[i >> 1][i & 1])));
       }
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(at_smem(&drain)));
+      for (int i = 0; i < 2; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(at_smem(&drain[i])));
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
   }
@@ -239,18 +264,22 @@ __global__ void __launch_bounds__(kPreThreads, 1)
     }
   }
   const long long rows_m = (long long)b.n * G;
+  const int nt = b.j1 - b.j0;
   auto tile_of = [&](int t) {
     PreTile r;
     const long long m0 = (long long)b.pair * 256 + t * kPreM, m1 = min(rows_m, m0 + kPreM) - 1;
-    r.exists = m0 < rows_m;
     r.pmin = b.len - b.n + int(m0 / G);
-    r.pmax = r.exists ? b.len - b.n + int(m1 / G) : -1;
+    r.pmax = m0 < rows_m ? b.len - b.n + int(m1 / G) : -1;
+    // As key tiles of the row: the sinks' before `sunk`, the window's [first, last].
+    const int last = r.pmax >> 6, first = p.window ? max(r.pmin - p.window + 1, 0) >> 6 : 0;
+    const int sunk = p.window ? min((p.sinks + kPreN - 1) / kPreN, last + 1) : 0;
+    r.s1 = max(0, min(nt, (sunk <= b.wfirst ? min(sunk, b.sink_tiles) : b.sink_tiles + sunk - b.wfirst) - b.j0));
+    r.w0 = max(0, max(first, b.wfirst) - b.wfirst + b.sink_tiles - b.j0);
+    r.w1 = min(nt, last + 1 - b.wfirst + b.sink_tiles - b.j0);
     return r;
   };
-  auto live = [&](const PreTile &t, int j) {  // some row of the tile sees a key of key tile j
-    const int k0 = key_tile(j);
-    return t.exists && k0 <= t.pmax && (!p.window || k0 < p.sinks || k0 + kPreN - 1 > t.pmin - p.window);
-  };
+  // Key tiles (by the block's index i) that some row of the tile sees: i < t.s1, and t.w0 <= i < t.w1.
+  auto live = [&](const PreTile &t, int i) { return i < t.s1 || (i >= t.w0 && i < t.w1); };
 
   // ---- Q: M row t of tile A or B into its swizzled slices -----------------------------------
   const int wg = warp >> 2, t = tid & 127;
@@ -262,7 +291,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
 #pragma unroll
     for (int c = 0; c < D / 8; ++c) {
       const uint4 v = mine ? *reinterpret_cast<const uint4 *>(q_row + c * 8) : make_uint4(0, 0, 0, 0);
-      *reinterpret_cast<uint4 *>(sm + wg * Cfg::kTile + (c >> 3) * Cfg::kSlice + at_sw(t, c & 7)) = v;
+      *reinterpret_cast<uint4 *>(sm + wg * Cfg::kQ + (c >> 3) * Cfg::kQSlice + at_sw(t, c & 7)) = v;
     }
   }
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -270,46 +299,63 @@ __global__ void __launch_bounds__(kPreThreads, 1)
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = tmem_slot;
-  auto stage = [&](int it) { return ring + (it % NST) * Cfg::kTile; };  // K of tile j: it = 2 (j - j0), V: + 1
+  // Ring order K0 K1 V0 K2 V1 ... (the order of use): the place of V of the block's i-th tile.
+  auto at_v = [&](int i) { return i == nt - 1 ? 2 * i + 1 : 2 * i + 2; };
+  auto stage = [&](int it) { return ring + (it % NST) * Cfg::kTile; };
 
   if (warp >= 8) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPreRegsIssue));
-  if (warp == 9) {
+  if (warp == 10) {
     // ---- copies ---------------------------------------------------------------------------
+    // The pool rows of the pieces' keys, a batch of 32 pieces at a time (lane l: piece l % pieces
+    // of the batch's tile l / pieces), read a batch ahead: no copy waits for the page table.
+    const int tpb = 32 / pieces;
+    auto load_rows = [&](int batch) {
+      int y = x.total_rows;  // out of bounds: zeros
+      const int i = batch * tpb + lane / pieces;
+      if (i < nt) {
+        const int k0 = key_tile(b.j0 + i) + (lane % pieces) * x.box_rows;
+        if (needed(k0, k0 + x.box_rows)) {
+          const int page = tab[k0 >> p.page_shift];
+          if (page >= 0 && page < p.pages)
+            y = x.row0 + ((page * 2 * p.kv_heads + kvh) << p.page_shift) + (k0 & ((1 << p.page_shift) - 1));
+        }
+      }
+      return y;
+    };
+    int rows_prev = 0, rows_cur = load_rows(0), rows_next = load_rows(1), batch = 0;
     int issued = 0;
     bool ok = true;
-    for (int j = b.j0; j < b.j1 && ok; ++j) {
-      int y = x.total_rows;  // K's row of this lane's piece; out of bounds: zeros
-      const int k0 = key_tile(j) + lane * x.box_rows;
-      if (lane < pieces && needed(k0, k0 + x.box_rows)) {
-        const int page = tab[k0 >> p.page_shift];
-        if (page >= 0 && page < p.pages)
-          y = x.row0 + (((page * 2 * p.kv_heads) + kvh) << p.page_shift) + (k0 & ((1 << p.page_shift) - 1));
+    for (int it = 0; it < 2 * nt && ok; ++it) {
+      // K of tile i and then V of tile i - 1 (K0 first, the last V alone).
+      const bool is_v = it >= 2 && ((it & 1) == 0 || it == 2 * nt - 1);
+      const bool v_one = nt == 1 && it == 1;
+      const int i = v_one ? 0 : is_v ? (it == 2 * nt - 1 ? nt - 1 : it / 2 - 1) : it < 2 ? it : (it + 1) / 2;
+      const int kv = is_v || v_one, s = it % NST;
+      if (i / tpb > batch) {
+        rows_prev = rows_cur, rows_cur = rows_next;
+        rows_next = load_rows(++batch + 1);
       }
-      for (int kv = 0; kv < 2; ++kv) {
-        const int it = 2 * (j - b.j0) + kv, s = it % NST;
-        if (it >= NST && !pre_wait(&kv_empty[s], unsigned(it / NST - 1) & 1u, &s_fail)) ok = false;
-        if (!__all_sync(0xFFFFFFFFu, ok)) {
-          ok = false;
-          break;
-        }
-        if (lane == 0)
-          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(at_smem(&kv_full[s])),
-                       "r"(Cfg::kTile)
-                       : "memory");
-        __syncwarp();
-        if (lane < pieces) {
-          const int yv = y == x.total_rows ? y : y + ((kv * p.kv_heads) << p.page_shift);
+      int y = __shfl_sync(0xFFFFFFFFu, i / tpb == batch ? rows_cur : rows_prev, (i % tpb) * pieces + lane % pieces);
+      if (kv && y != x.total_rows) y += p.kv_heads << p.page_shift;
+      if (it >= NST && !pre_wait(&kv_empty[s], unsigned(it / NST - 1) & 1u, &s_fail)) ok = false;
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      if (!ok) break;
+      if (lane == 0)
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(at_smem(&kv_full[s])),
+                     "r"(Cfg::kTile)
+                     : "memory");
+      __syncwarp();
+      if (lane < pieces) {
 #pragma unroll
-          for (int c = 0; c < D / 64; ++c)
-            asm volatile(
-                "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, "
-                "%4}], [%2];" ::"r"(at_smem(stage(it) + c * Cfg::kSlice + lane * x.box_rows * 128)),
-                "l"(&map), "r"(at_smem(&kv_full[s])), "r"(c * 64), "r"(yv)
-                : "memory");
-        }
-        issued = it + 1;
+        for (int c = 0; c < D / 64; ++c)
+          asm volatile(
+              "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, "
+              "%4}], [%2];" ::"r"(at_smem(stage(it) + c * Cfg::kSlice + lane * x.box_rows * 128)),
+              "l"(&map), "r"(at_smem(&kv_full[s])), "r"(c * 64), "r"(y)
+              : "memory");
       }
+      issued = it + 1;
     }
     if (!ok) {  // leave no copy in flight
       s_fail = 1;
@@ -317,42 +363,66 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         at_wait(&kv_full[i % NST], unsigned(i / NST) & 1u);
       if (lane == 0 && p.error) atomicOr(p.error, kKvExpired);
     }
-  } else if (warp == 8) {
-    // ---- products -------------------------------------------------------------------------
-    const PreTile tl[2] = {tile_of(0), tile_of(1)};
-    bool ok = true, started[2] = {false, false};
-    unsigned n_p[2] = {0u, 0u};
-    auto wait_full = [&](int it) {
-      ok = ok && pre_wait(&kv_full[it % NST], unsigned(it / NST) & 1u, &s_fail);
-      ok = __all_sync(0xFFFFFFFFu, ok);
+  } else if (warp < 10) {
+    // ---- products of tile X = A (warp 8) or B (warp 9) ---------------------------------------
+    const int X = warp - 8;
+    const PreTile tl = tile_of(X);
+    bool ok = true;
+    int n_s = 0, n_p = 0;  // the tile's key tiles whose S, whose P V was issued
+    // A place in the ring: its slot and the parity of its use.
+    struct Place {
+      int slot;
+      unsigned ph;
+      __device__ void next2() {
+        slot += 2;
+        if (slot >= NST) slot -= NST, ph ^= 1u;
+      }
+    };
+    Place k_at = {0, 0}, v_at = {2, 0};
+    auto wait_full = [&](const Place &a) {
+      ok = __all_sync(0xFFFFFFFFu, pre_wait(&kv_full[a.slot], a.ph, &s_fail));
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     };
-    auto issue_s = [&](int X, int it) {
-      if (lane == 0) {
-        const unsigned char *k = stage(it);
+    // Operands' descriptors, the same on every lane (the shuffles tell the compiler so).
+    auto uniform = [](uint32_t v) { return __shfl_sync(0xFFFFFFFFu, v, 0); };
+    const uint32_t tm = uniform(tmem + X * 128), q_lo = uniform(at_desc_lo(at_smem(sm + X * Cfg::kQ)));
+    const uint32_t ring_a = uniform(at_smem(ring));
+    // S of tile i if some row sees some of it; the K tile's slot is then free for this tile.
+    auto issue_s = [&](int i) {
+      wait_full(k_at);
+      if (!ok) return;
+      const bool on = live(tl, i);
+      const uint32_t buf = uniform(n_s & 1), k = uniform(at_desc_lo(ring_a + k_at.slot * Cfg::kTile));
+      if (at_elect()) {
+        if (on) {
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks)
-          at_mma(tmem + X * kPreN, at_desc(sm + X * Cfg::kTile + (ks >> 2) * Cfg::kSlice) + 2 * (ks & 3),
-                 at_desc(k + (ks >> 2) * Cfg::kSlice) + 2 * (ks & 3), Cfg::kIdescS, uint32_t(ks != 0));
-        at_commit(&s_full[X]);
+          for (int ks = 0; ks < D / 16; ++ks)
+            at_mma_ss(tm + buf * 64, q_lo + (((ks >> 2) * Cfg::kQSlice) >> 4) + 2 * (ks & 3),
+                      k + (((ks >> 2) * Cfg::kSlice) >> 4) + 2 * (ks & 3), Cfg::kIdescS, uint32_t(ks != 0));
+          at_commit(&s_full[X][buf]);
+        }
+        at_commit(&kv_empty[k_at.slot]);
       }
       __syncwarp();
+      n_s += on;
+      if (i == 0)
+        k_at.slot = 1;
+      else
+        k_at.next2();
     };
-    if (b.j0 < b.j1) {
-      wait_full(0);
-      if (ok) {
-        for (int X = 0; X < 2; ++X)
-          if (live(tl[X], b.j0)) issue_s(X, 0);
-        if (lane == 0) at_commit(&kv_empty[0]);
+    for (int i = 0; i < 2 && i < nt && ok; ++i) issue_s(i);
+    for (int i = 0; i < nt && ok; ++i) {
+      const int k0 = key_tile(b.j0 + i);
+      if (i == nt - 1) {  // the last V follows the last K's place by one, not two
+        v_at.ph ^= v_at.slot == 0;
+        v_at.slot = v_at.slot == 0 ? NST - 1 : v_at.slot - 1;
       }
-    }
-    for (int j = b.j0; j < b.j1 && ok; ++j) {
-      const int it = 2 * (j - b.j0) + 1, k0 = key_tile(j);
-      wait_full(it);
+      wait_full(v_at);
       if (!ok) break;
-      unsigned char *v = stage(it);
       if (k0 + kPreN > b.kend || (k0 + kPreN > b.sinks && k0 < b.lo)) {
-        // V rows that nothing in the block sees: zeros (their P is 0, the rows may hold any bits).
+        // V rows that nothing in the block sees: zeros (their P is 0, the rows may hold any
+        // bits). Both tiles' warps do so, each before its own product.
+        unsigned char *v = ring + v_at.slot * Cfg::kTile;
         for (int r = 0; r < kPreN; ++r)
           if (k0 + r >= b.kend || (k0 + r >= b.sinks && k0 + r < b.lo))
             if (lane < D / 8)
@@ -361,41 +431,32 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
       }
-      bool k_there = false;
-      for (int X = 0; X < 2 && ok; ++X) {
-        if (live(tl[X], j)) {
-          ok = pre_wait(&p_ready[X], n_p[X]++ & 1u, &s_fail);
-          ok = __all_sync(0xFFFFFFFFu, ok);
-          if (!ok) break;
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          if (lane == 0) {
+      const bool on = live(tl, i);
+      const uint32_t buf = uniform(n_p & 1), acc = uniform(n_p > 0);
+      const uint32_t vd = uniform(at_desc_mn_lo(ring_a + v_at.slot * Cfg::kTile, Cfg::kSlice));
+      if (on) {
+        ok = __all_sync(0xFFFFFFFFu, pre_wait(&p_ready[X][buf], unsigned(n_p >> 1) & 1u, &s_fail));
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      }
+      if (at_elect()) {
+        if (on) {
 #pragma unroll
-            for (int ks = 0; ks < kPreN / 16; ++ks)
-              at_mma_ts(tmem + kPreColO + X * 128, tmem + X * kPreN + 8 * ks,
-                        at_desc_mn(v, Cfg::kSlice) + uint64_t(ks) * (2048 >> 4), Cfg::kIdescO,
-                        uint32_t(started[X] || ks > 0));
-          }
-          started[X] = true;
-          bool more = false;
-          for (int i = j + 1; i < b.j1 && !more; ++i) more = live(tl[X], i);
-          if (!more && lane == 0) at_commit(&o_done[X]);
+          for (int ks = 0; ks < kPreN / 16; ++ks)
+            at_mma_ts(tm + kPreColO, tm + buf * 64 + 8 * ks, vd + ks * (2048 >> 4), Cfg::kIdescO, ks > 0 ? 1u : acc);
+          at_commit(&o_done[X][buf]);
         }
-        if (X == 1 && lane == 0) at_commit(&kv_empty[it % NST]);
-        if (j + 1 < b.j1 && live(tl[X], j + 1)) {
-          if (!k_there) wait_full(it + 1);
-          k_there = true;
-          if (ok) issue_s(X, it + 1);
-        }
+        at_commit(&kv_empty[v_at.slot]);
       }
-      if (ok && j + 1 < b.j1) {
-        if (!k_there) wait_full(it + 1);
-        if (lane == 0) at_commit(&kv_empty[(it + 1) % NST]);
-      }
+      __syncwarp();
+      n_p += on;
+      v_at.next2();
+      if (i + 2 < nt) issue_s(i + 2);
     }
     // Every product issued has completed before the block's tensor memory goes.
-    if (lane == 0) at_commit(&drain);
+    if (at_elect()) at_commit(&drain[X]);
     __syncwarp();
-    if (!at_wait(&drain, 0u) || !ok) {
+    if (!at_wait(&drain[X], 0u) || !ok) {
       s_fail = 1;
       if (lane == 0 && p.error) atomicOr(p.error, kKvExpired);
     }
@@ -411,13 +472,15 @@ __global__ void __launch_bounds__(kPreThreads, 1)
     const int pos = mine ? max(b.len - b.n + qi, -1) : -1;
     const float sl2 = p.scale * 1.4426950408889634f;
     const uint32_t lanes = tmem + (uint32_t((warp & 3) * 32) << 16);
-    const uint32_t col_s = lanes + wg * kPreN, col_o = lanes + kPreColO + wg * 128;
-    unsigned n_s = 0u;
+    const uint32_t col_s = lanes + wg * 128, col_o = lanes + kPreColO + wg * 128;
+    int n_s = 0;  // the tile's key tiles so far
     bool ok = true;
     float row_m = -INFINITY, row_l = 0.f;  // running maximum and sum
-    for (int j = b.j0; j < b.j1; ++j) {
-      if (!live(tl, j)) continue;
-      ok = pre_wait(&s_full[wg], n_s & 1u, &s_fail);
+    for (int i = 0; i < nt; ++i) {
+      const int j = b.j0 + i;
+      if (!live(tl, i)) continue;
+      const int buf = n_s & 1;
+      ok = pre_wait(&s_full[wg][buf], unsigned(n_s >> 1) & 1u, &s_fail);
       if (!__all_sync(0xFFFFFFFFu, ok)) {
         ok = false;
         break;
@@ -425,8 +488,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const int k0 = key_tile(j);
       float s[kPreN];
-      at_ld64(col_s, s);
-      at_ld64(col_s + 64, s + 64);
+      at_ld64(col_s + buf * 64, s);
       const bool whole = k0 + kPreN - 1 <= tl.pmin &&
                          (!p.window || k0 + kPreN - 1 < p.sinks || k0 > tl.pmax - p.window);
       if (!whole || s_bad) {
@@ -446,74 +508,83 @@ __global__ void __launch_bounds__(kPreThreads, 1)
           }
         }
         // A V value that is not finite in a row that only some of the queries see: the product
-        // with P = 0 would carry it into the others (thread t looks at V row t).
-        const int it = 2 * (j - b.j0) + 1;
+        // with P = 0 would carry it into the others (a thread looks at half a V row).
+        const int it = at_v(i), r = t & (kPreN - 1);
         ok = pre_wait(&kv_full[it % NST], unsigned(it / NST) & 1u, &s_fail);
         if (!__all_sync(0xFFFFFFFFu, ok)) {
           ok = false;
           break;
         }
-        if (k0 + t < b.kend && !(k0 + t >= b.sinks && k0 + t < b.lo)) {
+        if (k0 + r < b.kend && !(k0 + r >= b.sinks && k0 + r < b.lo)) {
           __nv_bfloat162 acc = __floats2bfloat162_rn(0.f, 0.f);
           const __nv_bfloat162 zero = acc;
-          const unsigned char *v = stage(it) + t * 128;
+          const unsigned char *v = stage(it) + r * 128;
 #pragma unroll
-          for (int c = 0; c < D / 8; ++c) {
+          for (int c0 = 0; c0 < D / 16; ++c0) {
+            const int c = c0 + (t >> 6) * (D / 16);
             const uint4 w = *reinterpret_cast<const uint4 *>(v + (c >> 3) * Cfg::kSlice + (c & 7) * 16);
             const uint32_t e[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc = __hfma2(*reinterpret_cast<const __nv_bfloat162 *>(&e[i]), zero, acc);
+            for (int n = 0; n < 4; ++n) acc = __hfma2(*reinterpret_cast<const __nv_bfloat162 *>(&e[n]), zero, acc);
           }
           const float2 f = __bfloat1622float2(acc);
           if (f.x != 0.f || f.y != 0.f) s_poison[wg] = 1;
         }
       }
-      float mx8[8];
+      float mx4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) mx8[i] = s[i];
+      for (int k = 4; k + 8 <= kPreN; k += 8)
 #pragma unroll
-      for (int k = 8; k < kPreN; ++k) mx8[k & 7] = fmaxf(mx8[k & 7], s[k]);
-      const float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])),
-                             fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7]))) *
-                       sl2;
+        for (int c = 0; c < 4; ++c) mx4[c] = max3(mx4[c], s[k + c], s[k + 4 + c]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) mx4[c] = fmaxf(mx4[c], s[kPreN - 4 + c]);
+      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sl2;
       const bool raise = mx > row_m + kPreRescale;  // false while both are -inf
       if (__any_sync(0xFFFFFFFFu, raise)) {
         const float c = raise ? pre_ex2(row_m - mx) : 1.f;  // 0 when m was -inf
         row_l *= c;
         row_m = raise ? mx : row_m;
-        // S of this tile was issued behind the last P V, so O is complete and still.
-        if (n_s > 0) {
+        if (n_s > 0) {  // O, once the last P V has landed (the next one waits for this tile's P)
+          ok = pre_wait(&o_done[wg][buf ^ 1], unsigned((n_s - 1) >> 1) & 1u, &s_fail);
+          if (!__all_sync(0xFFFFFFFFu, ok)) {
+            ok = false;
+            break;
+          }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
           for (int cb = 0; cb < D; cb += 32) {
             float v[32];
             at_ld32(col_o + cb, v);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] *= c;
+            for (int e = 0; e < 32; ++e) v[e] *= c;
             at_st32(col_o + cb, v);
           }
         }
       }
       ++n_s;
+      // P = 2^(s scale log2(e) - m): pairs of values in one FMA and one addition.
       const float nm = row_m == -INFINITY ? 0.f : -row_m;
-      float ps[4] = {0.f, 0.f, 0.f, 0.f};
+      const uint64_t sl2x2 = pair64(sl2, sl2), nmx2 = pair64(nm, nm);
+      uint64_t sum[2] = {0, 0};
+      uint32_t w[kPreN / 2];
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t w[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float e0 = pre_ex2(fmaf(s[64 * c + 2 * i], sl2, nm)), e1 = pre_ex2(fmaf(s[64 * c + 2 * i + 1], sl2, nm));
-          ps[i & 1] += e0, ps[2 + (i & 1)] += e1;
-          const __nv_bfloat162 h = __floats2bfloat162_rn(e0, e1);
-          w[i] = *reinterpret_cast<const uint32_t *>(&h);
-        }
-        st32_async(col_s + 32 * c, w);
+      for (int k = 0; k < kPreN / 2; ++k) {
+        float e0, e1;
+        split64(fma2(pair64(s[2 * k], s[2 * k + 1]), sl2x2, nmx2), e0, e1);
+        e0 = pre_ex2(e0), e1 = pre_ex2(e1);
+        sum[k & 1] = add2(sum[k & 1], pair64(e0, e1));
+        const __nv_bfloat162 h = __floats2bfloat162_rn(e0, e1);
+        w[k] = *reinterpret_cast<const uint32_t *>(&h);
       }
-      row_l += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+      st32_async(col_s + buf * 64, w);
+      float l0, l1;
+      split64(add2(sum[0], sum[1]), l0, l1);
+      row_l += l0 + l1;
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      at_arrive(&p_ready[wg]);
+      at_arrive(&p_ready[wg][buf]);
     }
-    if (ok && n_s > 0) ok = pre_wait(&o_done[wg], 0u, &s_fail);
+    if (ok && n_s > 0) ok = pre_wait(&o_done[wg][(n_s - 1) & 1], unsigned((n_s - 1) >> 1) & 1u, &s_fail);
     if (!__all_sync(0xFFFFFFFFu, ok)) {
       s_fail = 1;
       if (lane == 0 && p.error) atomicOr(p.error, kKvExpired);
@@ -575,7 +646,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       // [r D / C, (r + 1) D / C): the others send it theirs ([sender][4 columns][M row], 16 bytes
       // each) into its ring, which no copy or product uses any more.
       // (m and l go where the tile's Q was: its products are complete.)
-      float2 *ml = reinterpret_cast<float2 *>(sm + wg * Cfg::kTile) + t;
+      float2 *ml = reinterpret_cast<float2 *>(sm + wg * Cfg::kQ) + t;
       *ml = make_float2(row_m, row_l);
       pre_cluster_sync();
       float M = -INFINITY, L = 0.f, w = 0.f;

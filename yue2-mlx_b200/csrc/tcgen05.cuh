@@ -52,12 +52,35 @@ __device__ __forceinline__ void at_mma(uint32_t tmem, uint64_t a, uint64_t b, ui
       "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
       : "memory");
 }
-// The same with A in tensor memory (row = lane, two BF16 values of k per 32-bit column).
-__device__ __forceinline__ void at_mma_ts(uint32_t tmem, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// True on one lane of a converged warp, always the same one. Inside a branch on it (unlike
+// one on the lane's number) the issued instructions' operands stay in uniform registers:
+// one tcgen05.mma then costs a few issue cycles instead of ~150.
+__device__ __forceinline__ bool at_elect() {
+  uint32_t r;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xFFFFFFFF;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(r));
+  return r != 0;
+}
+// Low words of at_desc / at_desc_mn of the operand at shared address `a` (the high word is
+// kAtDescHi); a step of n bytes adds n / 16.
+constexpr uint32_t kAtDescHi = (1024 >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t at_desc_lo(uint32_t a) { return ((a >> 4) & 0x3FFFu) | (1u << 16); }
+__device__ __forceinline__ uint32_t at_desc_mn_lo(uint32_t a, int slice_bytes) {
+  return ((a >> 4) & 0x3FFFu) | (uint32_t(slice_bytes >> 4) << 16);
+}
+// D (tensor memory) = A B (+ D when acc): A and B by the low words of their descriptors.
+__device__ __forceinline__ void at_mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n}" ::"r"(tmem),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
+      "{\n .reg .pred p;\n .reg .b64 da, db;\n setp.ne.b32 p, %4, 0;\n mov.b64 da, {%1, %5};\n mov.b64 db, {%2, %5};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(kAtDescHi)
+      : "memory");
+}
+// The same with A in tensor memory (row = lane, two BF16 values of k per 32-bit column).
+__device__ __forceinline__ void at_mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n .reg .b64 db;\n setp.ne.b32 p, %4, 0;\n mov.b64 db, {%2, %5};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(kAtDescHi)
       : "memory");
 }
 __device__ __forceinline__ void at_commit(uint64_t *bar) {
