@@ -8,7 +8,8 @@ S = max_j scale sum_d |q_d k_jd|.
 * the exponential itself, and the sums over the keys in FP32 (partial sums of positive terms,
   rescaled per block): 2^-18 covers 2^-22 per exponential and 64 rounded blocks;
 * the weights enter the second product as BF16 (off by 2^-8 each at most) in the prompt form,
-  as two BF16 parts (2^-16) in the single-token form;
+  as two BF16 parts (2^-16) in the single-token form; some of the prompt form's exponentials
+  come from a polynomial (2.6e-6 < 2^-18 off in a weight and in their sum);
 * the result is rounded to BF16 once: 2^-8 of it.
 """
 import math
@@ -20,7 +21,7 @@ from tests.conftest import load_package
 
 pytestmark = pytest.mark.gpu
 
-P_ROUND = {"decode": 2.0 ** -16, "prefill": 2.0 ** -8}
+P_ROUND = {"decode": 2.0 ** -16, "prefill": 2.0 ** -8 + 2.0 ** -17}
 
 
 @pytest.fixture(scope="module")

@@ -28,6 +28,7 @@
 
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kv_ops.h"
@@ -46,8 +47,10 @@ template <int D>
 struct PreCfg {
   static constexpr int kQSlice = kPreM * 128, kQ = (D / 64) * kQSlice;    // 128 rows of 64 values; a Q tile
   static constexpr int kSlice = kPreN * 128, kTile = (D / 64) * kSlice;  // the same of a K or V tile
-  static constexpr int kStages = D == 128 ? 10 : 20;                     // K and V tiles in flight: 160 KB
-  static constexpr int kSmem = 2 * kQ + kStages * kTile + 1024;
+  // A ring stage: V of tile i, then K of tile i + 2 (the products that follow P of tile i);
+  // stage 0 of the walk: K of tiles 0 and 1. 160 KB in flight.
+  static constexpr int kStages = D == 128 ? 5 : 10;
+  static constexpr int kSmem = 2 * kQ + 2 * kStages * kTile + 1024;
   // kind::f16, FP32 accumulator, BF16 A and B, A K-major, N >> 3 at bit 17, M >> 4 at bit 24;
   // P V reads B (V) MN-major (bit 16).
   static constexpr uint32_t kIdescS =
@@ -58,6 +61,7 @@ struct PreCfg {
 // Tensor memory: two S (and P) buffers of A at columns 0 and 64, of B at 128 and 192, O at 256, 384.
 constexpr uint32_t kPreColO = 256, kPreCols = 512;
 constexpr float kPreRescale = 8.f;
+constexpr int kPrePoly = 3;  // of 8 pairs of exponentials, those on the FMA units
 
 struct PrefillExtra {
   int row0;        // the layer's first cached row in the pool seen as [rows][D]
@@ -66,19 +70,27 @@ struct PrefillExtra {
   int pairs;       // upper bound of the blocks' M-row pairs
 };
 
-// A bounded wait that also ends when another role gave up.
-__device__ __forceinline__ bool pre_wait(uint64_t *bar, unsigned parity, const volatile int *fail) {
-  for (long long i = 0; i < kAtWaitLimit; ++i) {
-    uint32_t done;
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
-        : "=r"(done)
-        : "r"(at_smem(bar)), "r"(parity)
-        : "memory");
-    if (done) return true;
-    if ((i & 255) == 255 && *fail) return false;
+// A bounded wait (2^16 polls of up to 20 us each) that also ends when another role gave up.
+__device__ __forceinline__ bool pre_poll(uint64_t *bar, unsigned parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(done)
+      : "r"(at_smem(bar)), "r"(parity), "r"(20000u)
+      : "memory");
+  return done != 0;
+}
+__device__ __forceinline__ bool pre_wait_slow(uint64_t *bar, unsigned parity, const volatile int *fail) {
+  for (int i = 0; i < 1 << 16; ++i) {
+    if (pre_poll(bar, parity)) return true;
+    if (*fail) return false;
   }
   return false;
+}
+// True on every lane of the (converged) warp when the phase is over.
+__device__ __forceinline__ bool pre_wait(uint64_t *bar, unsigned parity, const volatile int *fail) {
+  if (__all_sync(0xFFFFFFFFu, pre_poll(bar, parity))) return true;
+  return __all_sync(0xFFFFFFFFu, pre_wait_slow(bar, parity, fail));
 }
 // 2^x by the approximate base-2 exponential, results below 2^-126 as 0 (relative error below
 // 2^-22): without that flush each exponential costs three more instructions.
@@ -110,6 +122,26 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
+}
+// 2^t of two values t <= 100 on the FMA units (t below -125 gives 2^-125): t = n + f with f in
+// [-1/2, 1/2], 2^f by the degree-4 polynomial of least maximal relative error on that interval
+// (2.6e-6, Remez exchange), n added to its exponent.
+__device__ __forceinline__ void exp2_poly2(uint64_t t, float &e0, float &e1) {
+  float t0, t1, r0, r1, p0, p1;
+  split64(t, t0, t1);
+  t = pair64(fmaxf(t0, -125.f), fmaxf(t1, -125.f));
+  const uint64_t big = pair64(12582912.f, 12582912.f);  // 1.5 x 2^23: the sum's last bit is one
+  const uint64_t r = add2(t, big);
+  const uint64_t f = fma2(add2(r, pair64(-12582912.f, -12582912.f)), pair64(-1.f, -1.f), t);
+  uint64_t p = fma2(f, pair64(0.009570102207362652f, 0.009570102207362652f),
+                    pair64(0.05591785907745361f, 0.05591785907745361f));
+  p = fma2(f, p, pair64(0.240247443318367f, 0.240247443318367f));
+  p = fma2(f, p, pair64(0.6931217908859253f, 0.6931217908859253f));
+  p = fma2(f, p, pair64(0.9999992847442627f, 0.9999992847442627f));
+  split64(r, r0, r1);
+  split64(p, p0, p1);
+  e0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(r0) << 23));
+  e1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(r1) << 23));
 }
 // Store 32 columns of this warp's lanes (not waited for).
 __device__ __forceinline__ void st32_async(uint32_t addr, const uint32_t *v) {
@@ -232,7 +264,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       }
       for (int i = 0; i < 4; ++i) {
         asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(at_smem(&s_full[i >> 1][i & 1])));
-        asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(at_smem(&p_ready[i >> 1][i & 1])), "r"(kPreM));
+        asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(at_smem(&p_ready[i >> 1][i & 1])), "r"(kPreM / 32));
         asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(at_smem(&o_done[i >> 1][i & 1])));
       }
       for (int i = 0; i < 2; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(at_smem(&drain[i])));
@@ -299,9 +331,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = tmem_slot;
-  // Ring order K0 K1 V0 K2 V1 ... (the order of use): the place of V of the block's i-th tile.
-  auto at_v = [&](int i) { return i == nt - 1 ? 2 * i + 1 : 2 * i + 2; };
-  auto stage = [&](int it) { return ring + (it % NST) * Cfg::kTile; };
+  auto stage = [&](int it) { return ring + (it % NST) * 2 * Cfg::kTile; };  // (V of tile i: it = i + 1)
 
   if (warp >= 8) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPreRegsIssue));
@@ -324,38 +354,41 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       return y;
     };
     int rows_prev = 0, rows_cur = load_rows(0), rows_next = load_rows(1), batch = 0;
-    int issued = 0;
-    bool ok = true;
-    for (int it = 0; it < 2 * nt && ok; ++it) {
-      // K of tile i and then V of tile i - 1 (K0 first, the last V alone).
-      const bool is_v = it >= 2 && ((it & 1) == 0 || it == 2 * nt - 1);
-      const bool v_one = nt == 1 && it == 1;
-      const int i = v_one ? 0 : is_v ? (it == 2 * nt - 1 ? nt - 1 : it / 2 - 1) : it < 2 ? it : (it + 1) / 2;
-      const int kv = is_v || v_one, s = it % NST;
-      if (i / tpb > batch) {
-        rows_prev = rows_cur, rows_cur = rows_next;
-        rows_next = load_rows(++batch + 1);
-      }
+    // Tile i's K (kv = 0) or V into `dst`, this lane's piece of it.
+    auto put = [&](int i, int kv, unsigned char *dst, uint64_t *bar) {
       int y = __shfl_sync(0xFFFFFFFFu, i / tpb == batch ? rows_cur : rows_prev, (i % tpb) * pieces + lane % pieces);
       if (kv && y != x.total_rows) y += p.kv_heads << p.page_shift;
-      if (it >= NST && !pre_wait(&kv_empty[s], unsigned(it / NST - 1) & 1u, &s_fail)) ok = false;
-      ok = __all_sync(0xFFFFFFFFu, ok);
-      if (!ok) break;
-      if (lane == 0)
-        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(at_smem(&kv_full[s])),
-                     "r"(Cfg::kTile)
-                     : "memory");
-      __syncwarp();
       if (lane < pieces) {
 #pragma unroll
         for (int c = 0; c < D / 64; ++c)
           asm volatile(
               "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, "
-              "%4}], [%2];" ::"r"(at_smem(stage(it) + c * Cfg::kSlice + lane * x.box_rows * 128)),
-              "l"(&map), "r"(at_smem(&kv_full[s])), "r"(c * 64), "r"(y)
+              "%4}], [%2];" ::"r"(at_smem(dst + c * Cfg::kSlice + lane * x.box_rows * 128)),
+              "l"(&map), "r"(at_smem(bar)), "r"(c * 64), "r"(y)
               : "memory");
       }
+    };
+    int issued = 0;
+    bool ok = true;
+    for (int it = 0; it <= nt && nt > 0; ++it) {
+      const int s = it % NST, i = it + 1;  // the stage's K tile (it = 0: tiles 0 and 1)
+      if (it >= NST) ok = pre_wait(&kv_empty[s], unsigned(it / NST - 1) & 1u, &s_fail);
+      if (!ok) break;
+      const int tiles = it == 0 ? min(nt, 2) : 1 + (i < nt);
+      if (lane == 0)
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(at_smem(&kv_full[s])),
+                     "r"(tiles * Cfg::kTile)
+                     : "memory");
+      __syncwarp();
       issued = it + 1;
+      put(it == 0 ? 0 : it - 1, it > 0, stage(it), &kv_full[s]);
+      if (i < nt) {
+        if (i / tpb > batch) {
+          rows_prev = rows_cur, rows_cur = rows_next;
+          rows_next = load_rows(++batch + 1);
+        }
+        put(i, 0, stage(it) + Cfg::kTile, &kv_full[s]);
+      }
     }
     if (!ok) {  // leave no copy in flight
       s_fail = 1;
@@ -365,64 +398,61 @@ __global__ void __launch_bounds__(kPreThreads, 1)
     }
   } else if (warp < 10) {
     // ---- products of tile X = A (warp 8) or B (warp 9) ---------------------------------------
-    const int X = warp - 8;
-    const PreTile tl = tile_of(X);
+    // The loop's control values are the same on every lane; the shuffles tell the compiler so,
+    // and it keeps them, and the operands made from them, in uniform registers (each tcgen05
+    // operand copied from a thread's register would cost more than the product).
+    auto uniform = [](int v) { return __shfl_sync(0xFFFFFFFFu, v, 0); };
+    const int X = uniform(warp - 8), n_tiles = uniform(nt);
+    const PreTile mine_t = tile_of(X);
+    const PreTile tl = {0, 0, uniform(mine_t.s1), uniform(mine_t.w0), uniform(mine_t.w1)};
+    // Key tiles [e0, e1) and from e2 on hold V rows that nothing in the block sees.
+    const int hide0 = uniform(max(0, b.sinks / kPreN - b.j0));
+    const int hide1 = uniform(b.sinks < b.lo ? b.sink_tiles + (b.lo % kPreN && b.lo / kPreN >= b.sink_tiles) - b.j0 : 0);
+    const int hide2 = uniform(b.kend % kPreN ? b.sink_tiles + b.kend / kPreN - b.wfirst - b.j0 : 1 << 30);
+    const uint32_t tm = uniform(tmem + X * 128), q_lo = uniform(at_desc_lo(at_smem(sm + X * Cfg::kQ)));
+    const uint32_t k_lo = uniform(at_desc_lo(at_smem(ring))), v_lo = uniform(at_desc_mn_lo(at_smem(ring), Cfg::kSlice));
     bool ok = true;
-    int n_s = 0, n_p = 0;  // the tile's key tiles whose S, whose P V was issued
-    // A place in the ring: its slot and the parity of its use.
-    struct Place {
-      int slot;
-      unsigned ph;
-      __device__ void next2() {
-        slot += 2;
-        if (slot >= NST) slot -= NST, ph ^= 1u;
-      }
-    };
-    Place k_at = {0, 0}, v_at = {2, 0};
-    auto wait_full = [&](const Place &a) {
-      ok = __all_sync(0xFFFFFFFFu, pre_wait(&kv_full[a.slot], a.ph, &s_fail));
+    int n_s = 0, n_p = 0;    // the tile's key tiles whose S, whose P V was issued
+    int slot = 0, ph = 0;    // the place in the ring and the parity of its use
+    auto wait = [&](uint64_t *bar, int parity) {
+      ok = pre_wait(bar, unsigned(parity), &s_fail);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     };
-    // Operands' descriptors, the same on every lane (the shuffles tell the compiler so).
-    auto uniform = [](uint32_t v) { return __shfl_sync(0xFFFFFFFFu, v, 0); };
-    const uint32_t tm = uniform(tmem + X * 128), q_lo = uniform(at_desc_lo(at_smem(sm + X * Cfg::kQ)));
-    const uint32_t ring_a = uniform(at_smem(ring));
-    // S of tile i if some row sees some of it; the K tile's slot is then free for this tile.
-    auto issue_s = [&](int i) {
-      wait_full(k_at);
-      if (!ok) return;
-      const bool on = live(tl, i);
-      const uint32_t buf = uniform(n_s & 1), k = uniform(at_desc_lo(ring_a + k_at.slot * Cfg::kTile));
-      if (at_elect()) {
-        if (on) {
+    auto next = [&] {
+      if (++slot == NST) slot = 0, ph ^= 1;
+    };
+    // S of the tile's next key tile, whose K starts at descriptor k (by the elected lane).
+    auto put_s = [&](uint32_t k, int n) {
+      const int buf = n & 1;
 #pragma unroll
-          for (int ks = 0; ks < D / 16; ++ks)
-            at_mma_ss(tm + buf * 64, q_lo + (((ks >> 2) * Cfg::kQSlice) >> 4) + 2 * (ks & 3),
-                      k + (((ks >> 2) * Cfg::kSlice) >> 4) + 2 * (ks & 3), Cfg::kIdescS, uint32_t(ks != 0));
-          at_commit(&s_full[X][buf]);
-        }
-        at_commit(&kv_empty[k_at.slot]);
+      for (int ks = 0; ks < D / 16; ++ks)
+        at_mma_ss(tm + buf * 64, q_lo + (((ks >> 2) * Cfg::kQSlice) >> 4) + 2 * (ks & 3),
+                  k + (((ks >> 2) * Cfg::kSlice) >> 4) + 2 * (ks & 3), Cfg::kIdescS, uint32_t(ks != 0));
+      at_commit(&s_full[X][buf]);
+    };
+    if (n_tiles > 0) {
+      wait(&kv_full[0], 0);
+      const bool on0 = live(tl, 0), on1 = n_tiles > 1 && live(tl, 1);
+      if (ok && at_elect()) {
+        if (on0) put_s(k_lo, 0);
+        if (on1) put_s(k_lo + (Cfg::kTile >> 4), on0);
+        at_commit(&kv_empty[0]);
       }
       __syncwarp();
-      n_s += on;
-      if (i == 0)
-        k_at.slot = 1;
-      else
-        k_at.next2();
-    };
-    for (int i = 0; i < 2 && i < nt && ok; ++i) issue_s(i);
-    for (int i = 0; i < nt && ok; ++i) {
-      const int k0 = key_tile(b.j0 + i);
-      if (i == nt - 1) {  // the last V follows the last K's place by one, not two
-        v_at.ph ^= v_at.slot == 0;
-        v_at.slot = v_at.slot == 0 ? NST - 1 : v_at.slot - 1;
-      }
-      wait_full(v_at);
+      n_s = on0 + on1;
+      next();
+    }
+    for (int i = 0; i < n_tiles && ok; ++i) {
+      const bool on = live(tl, i), on_s = i + 2 < n_tiles && live(tl, i + 2);
+      const int buf = n_p & 1;
+      // The stage has landed long before P is written: both products follow P at once.
+      wait(&kv_full[slot], ph);
       if (!ok) break;
-      if (k0 + kPreN > b.kend || (k0 + kPreN > b.sinks && k0 < b.lo)) {
+      if ((i >= hide0 && i < hide1) || i >= hide2) {
         // V rows that nothing in the block sees: zeros (their P is 0, the rows may hold any
         // bits). Both tiles' warps do so, each before its own product.
-        unsigned char *v = ring + v_at.slot * Cfg::kTile;
+        const int k0 = key_tile(b.j0 + i);
+        unsigned char *v = ring + slot * 2 * Cfg::kTile;
         for (int r = 0; r < kPreN; ++r)
           if (k0 + r >= b.kend || (k0 + r >= b.sinks && k0 + r < b.lo))
             if (lane < D / 8)
@@ -431,27 +461,26 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
       }
-      const bool on = live(tl, i);
-      const uint32_t buf = uniform(n_p & 1), acc = uniform(n_p > 0);
-      const uint32_t vd = uniform(at_desc_mn_lo(ring_a + v_at.slot * Cfg::kTile, Cfg::kSlice));
+      const uint32_t at = slot * (2 * Cfg::kTile >> 4), acc = n_p > 0;
       if (on) {
-        ok = __all_sync(0xFFFFFFFFu, pre_wait(&p_ready[X][buf], unsigned(n_p >> 1) & 1u, &s_fail));
+        wait(&p_ready[X][buf], (n_p >> 1) & 1);
         if (!ok) break;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       }
       if (at_elect()) {
         if (on) {
 #pragma unroll
           for (int ks = 0; ks < kPreN / 16; ++ks)
-            at_mma_ts(tm + kPreColO, tm + buf * 64 + 8 * ks, vd + ks * (2048 >> 4), Cfg::kIdescO, ks > 0 ? 1u : acc);
+            at_mma_ts(tm + kPreColO, tm + buf * 64 + 8 * ks, v_lo + at + ks * (2048 >> 4), Cfg::kIdescO,
+                      ks > 0 ? 1u : acc);
           at_commit(&o_done[X][buf]);
         }
-        at_commit(&kv_empty[v_at.slot]);
+        if (on_s) put_s(k_lo + at + (Cfg::kTile >> 4), n_s);
+        at_commit(&kv_empty[slot]);
       }
       __syncwarp();
       n_p += on;
-      v_at.next2();
-      if (i + 2 < nt) issue_s(i + 2);
+      n_s += on_s;
+      next();
     }
     // Every product issued has completed before the block's tensor memory goes.
     if (at_elect()) at_commit(&drain[X]);
@@ -481,17 +510,14 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       if (!live(tl, i)) continue;
       const int buf = n_s & 1;
       ok = pre_wait(&s_full[wg][buf], unsigned(n_s >> 1) & 1u, &s_fail);
-      if (!__all_sync(0xFFFFFFFFu, ok)) {
-        ok = false;
-        break;
-      }
+      if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const int k0 = key_tile(j);
       float s[kPreN];
       at_ld64(col_s + buf * 64, s);
-      const bool whole = k0 + kPreN - 1 <= tl.pmin &&
-                         (!p.window || k0 + kPreN - 1 < p.sinks || k0 > tl.pmax - p.window);
-      if (!whole || s_bad) {
+      const bool edge = s_bad || k0 + kPreN - 1 > tl.pmin ||
+                        (p.window && k0 + kPreN - 1 >= p.sinks && k0 <= tl.pmax - p.window);
+      if (edge) {
         // k visible: k <= hi and (k < sink or k > old).
         const int hi = pos - k0, sink = p.window ? p.sinks - k0 : 1 << 30, old = pos - p.window - k0;
 #pragma unroll
@@ -509,12 +535,9 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         }
         // A V value that is not finite in a row that only some of the queries see: the product
         // with P = 0 would carry it into the others (a thread looks at half a V row).
-        const int it = at_v(i), r = t & (kPreN - 1);
+        const int it = i + 1, r = t & (kPreN - 1);
         ok = pre_wait(&kv_full[it % NST], unsigned(it / NST) & 1u, &s_fail);
-        if (!__all_sync(0xFFFFFFFFu, ok)) {
-          ok = false;
-          break;
-        }
+        if (!ok) break;
         if (k0 + r < b.kend && !(k0 + r >= b.sinks && k0 + r < b.lo)) {
           __nv_bfloat162 acc = __floats2bfloat162_rn(0.f, 0.f);
           const __nv_bfloat162 zero = acc;
@@ -546,10 +569,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         row_m = raise ? mx : row_m;
         if (n_s > 0) {  // O, once the last P V has landed (the next one waits for this tile's P)
           ok = pre_wait(&o_done[wg][buf ^ 1], unsigned((n_s - 1) >> 1) & 1u, &s_fail);
-          if (!__all_sync(0xFFFFFFFFu, ok)) {
-            ok = false;
-            break;
-          }
+          if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
           for (int cb = 0; cb < D; cb += 32) {
@@ -567,25 +587,39 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       const uint64_t sl2x2 = pair64(sl2, sl2), nmx2 = pair64(nm, nm);
       uint64_t sum[2] = {0, 0};
       uint32_t w[kPreN / 2];
+      auto weights = [&](auto some_poly) {
 #pragma unroll
-      for (int k = 0; k < kPreN / 2; ++k) {
-        float e0, e1;
-        split64(fma2(pair64(s[2 * k], s[2 * k + 1]), sl2x2, nmx2), e0, e1);
-        e0 = pre_ex2(e0), e1 = pre_ex2(e1);
-        sum[k & 1] = add2(sum[k & 1], pair64(e0, e1));
-        const __nv_bfloat162 h = __floats2bfloat162_rn(e0, e1);
-        w[k] = *reinterpret_cast<const uint32_t *>(&h);
-      }
+        for (int k = 0; k < kPreN / 2; ++k) {
+          float e0, e1;
+          const uint64_t t2 = fma2(pair64(s[2 * k], s[2 * k + 1]), sl2x2, nmx2);
+          if (some_poly && k % 8 < kPrePoly) {
+            exp2_poly2(t2, e0, e1);
+          } else {
+            split64(t2, e0, e1);
+            e0 = pre_ex2(e0), e1 = pre_ex2(e1);
+          }
+          sum[k & 1] = add2(sum[k & 1], pair64(e0, e1));
+          const __nv_bfloat162 h = __floats2bfloat162_rn(e0, e1);
+          w[k] = *reinterpret_cast<const uint32_t *>(&h);
+        }
+      };
+      // Tiles with masked scores take the exponential unit only: 2^-inf has to be 0.
+      if (edge)
+        weights(std::false_type{});
+      else
+        weights(std::true_type{});
       st32_async(col_s + buf * 64, w);
       float l0, l1;
       split64(add2(sum[0], sum[1]), l0, l1);
       row_l += l0 + l1;
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      at_arrive(&p_ready[wg][buf]);
+      // One arrival a warp: 32 lanes' arrivals on one barrier would take turns.
+      __syncwarp();
+      if (lane == 0) at_arrive(&p_ready[wg][buf]);
     }
     if (ok && n_s > 0) ok = pre_wait(&o_done[wg][(n_s - 1) & 1], unsigned((n_s - 1) >> 1) & 1u, &s_fail);
-    if (!__all_sync(0xFFFFFFFFu, ok)) {
+    if (!ok) {
       s_fail = 1;
       if (lane == 0 && p.error) atomicOr(p.error, kKvExpired);
     }
