@@ -502,6 +502,13 @@ __global__ void __launch_bounds__(kPreThreads, 1)
     const float sl2 = p.scale * 1.4426950408889634f;
     const uint32_t lanes = tmem + (uint32_t((warp & 3) * 32) << 16);
     const uint32_t col_s = lanes + wg * 128, col_o = lanes + kPreColO + wg * 128;
+    // Key tiles that every row sees whole: i < sunk and [whole0, whole1) (none with a bad page).
+    const bool bad = s_bad != 0;
+    const int shift = b.sink_tiles - b.wfirst - b.j0;  // a window tile's index i = its key tile + shift
+    const int sunk = bad || !p.window || tl.pmin < 0 ? 0 : min(min(p.sinks, tl.pmin + 1) / kPreN, b.sink_tiles) - b.j0;
+    const int whole0 = !p.window || tl.pmax < p.window ? b.sink_tiles - b.j0
+                                                       : max((tl.pmax - p.window) / kPreN + 1, b.wfirst) + shift;
+    const int whole1 = bad || tl.pmin < 0 ? 0 : (tl.pmin + 1) / kPreN + shift;
     int n_s = 0;  // the tile's key tiles so far
     bool ok = true;
     float row_m = -INFINITY, row_l = 0.f;  // running maximum and sum
@@ -512,27 +519,24 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       ok = pre_wait(&s_full[wg][buf], unsigned(n_s >> 1) & 1u, &s_fail);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const int k0 = key_tile(j);
       float s[kPreN];
       at_ld64(col_s + buf * 64, s);
-      const bool edge = s_bad || k0 + kPreN - 1 > tl.pmin ||
-                        (p.window && k0 + kPreN - 1 >= p.sinks && k0 <= tl.pmax - p.window);
+      const bool edge = i >= sunk && (i < whole0 || i >= whole1);
       if (edge) {
-        // k visible: k <= hi and (k < sink or k > old).
-        const int hi = pos - k0, sink = p.window ? p.sinks - k0 : 1 << 30, old = pos - p.window - k0;
-#pragma unroll
-        for (int k = 0; k < kPreN; ++k) s[k] = k <= hi && (k < sink || k > old) ? s[k] : -INFINITY;
-        if (s_bad) {
-#pragma unroll
-          for (int c = 0; c < kPreN / 16; ++c) {
-            const int kk = k0 + 16 * c;
-            const int page = needed(kk, kk + 16) ? tab[kk >> p.page_shift] : 0;
-            if (page < 0 || page >= p.pages) {
-#pragma unroll
-              for (int k = 0; k < 16; ++k) s[16 * c + k] = -INFINITY;
-            }
+        const int k0 = key_tile(j);
+        // Bit k: key k0 + k is visible (k <= hi, and k < sink or k > old).
+        auto below = [](int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1ull; };
+        unsigned long long seen = below(pos - k0 + 1);
+        if (p.window) seen &= below(p.sinks - k0) | ~below(pos - p.window - k0 + 1);
+        if (bad)
+          for (int c = 0; c < kPreN; c += 16) {
+            const int page = needed(k0 + c, k0 + c + 16) ? tab[(k0 + c) >> p.page_shift] : 0;
+            if (page < 0 || page >= p.pages) seen &= ~(0xFFFFull << c);
           }
-        }
+        const uint32_t seen_lo = uint32_t(seen), seen_hi = uint32_t(seen >> 32);
+#pragma unroll
+        for (int k = 0; k < kPreN; ++k)
+          s[k] = ((k < 32 ? seen_lo : seen_hi) >> (k & 31)) & 1u ? s[k] : -INFINITY;
         // A V value that is not finite in a row that only some of the queries see: the product
         // with P = 0 would carry it into the others (a thread looks at half a V row).
         const int it = i + 1, r = t & (kPreN - 1);
@@ -542,7 +546,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
           __nv_bfloat162 acc = __floats2bfloat162_rn(0.f, 0.f);
           const __nv_bfloat162 zero = acc;
           const unsigned char *v = stage(it) + r * 128;
-#pragma unroll
+#pragma unroll 2
           for (int c0 = 0; c0 < D / 16; ++c0) {
             const int c = c0 + (t >> 6) * (D / 16);
             const uint4 w = *reinterpret_cast<const uint4 *>(v + (c >> 3) * Cfg::kSlice + (c & 7) * 16);
@@ -571,7 +575,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
           ok = pre_wait(&o_done[wg][buf ^ 1], unsigned((n_s - 1) >> 1) & 1u, &s_fail);
           if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll
+#pragma unroll 1
           for (int cb = 0; cb < D; cb += 32) {
             float v[32];
             at_ld32(col_o + cb, v);
@@ -632,7 +636,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       const float nm = row_m == -INFINITY ? 0.f : -row_m;
       for (int cb = 0; cb < D; cb += 32) {
         float o[32];
-  #pragma unroll
+#pragma unroll
         for (int i = 0; i < 32; ++i) o[i] = 0.f;
         for (int j = b.j0; j < b.j1; ++j)
           for (int k = key_tile(j); k < key_tile(j) + kPreN; ++k) {
@@ -642,9 +646,10 @@ __global__ void __launch_bounds__(kPreThreads, 1)
             const bf16 *kr = p.kv + size_t(page) * p.page_elems +
                              ((size_t(kvh) << p.page_shift) + (k & ((1 << p.page_shift) - 1))) * D;
             float s = 0.f;
+#pragma unroll 4
             for (int d = 0; d < D; ++d) s = fmaf(bf2f(q_row[d]), bf2f(kr[d]), s);
             const float e = pre_ex2(fmaf(s, sl2, nm));
-  #pragma unroll
+#pragma unroll
             for (int i = 0; i < 32; ++i) o[i] = fmaf(e, bf2f(kr[p.page_elems / 2 + cb + i]), o[i]);
           }
         __syncwarp();
@@ -655,15 +660,15 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       if (!failed) {
         const float inv = row_l == 0.f ? 0.f : 1.0f / row_l;
         bf16 *dst = p.out + size_t(b.first + qi) * p.out_stride + size_t(head) * D;
-  #pragma unroll
+#pragma unroll 1
         for (int cb = 0; cb < D; cb += 32) {
           float v[32];
           at_ld32(col_o + cb, v);
           if (mine) {
-  #pragma unroll
+#pragma unroll
             for (int c = 0; c < 4; ++c) {
               uint32_t w[4];
-  #pragma unroll
+#pragma unroll
               for (int e = 0; e < 4; ++e) {
                 // (a row that saw nothing: O was never written)
                 const __nv_bfloat162 o2 = row_l == 0.f ? __floats2bfloat162_rn(0.f, 0.f)
@@ -686,7 +691,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       float M = -INFINITY, L = 0.f, w = 0.f;
       {
         float mv[4], lv[4];
-  #pragma unroll
+#pragma unroll
         for (uint32_t c = 0; c < 4; ++c) {
           mv[c] = -INFINITY, lv[c] = 0.f;
           if (c < C) {
@@ -695,7 +700,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
           }
           M = fmaxf(M, mv[c]);
         }
-  #pragma unroll
+#pragma unroll
         for (int c = 0; c < 4; ++c)
           if (lv[c] != 0.f) L += lv[c] * (mv[c] == M ? 1.f : pre_ex2(mv[c] - M));
         w = row_l == 0.f ? 0.f : row_m == M ? 1.f : pre_ex2(row_m - M);
@@ -703,25 +708,25 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       const int cols = D / int(C), own = int(rank) * cols;
       float mine_o[D / 2];  // this block's columns (C >= 2)
       if (warp < 8) {
-  #pragma unroll
+#pragma unroll
         for (int cb = 0; cb < D; cb += 32) {
           float v[32];
           at_ld32(col_o + cb, v);
-  #pragma unroll
+#pragma unroll
           for (int i = 0; i < 32; ++i) v[i] = row_l == 0.f ? 0.f : v[i] * w;
-  #pragma unroll
+#pragma unroll
           for (int h = 0; h < 2; ++h) {  // 16 columns: all of one block's (cols is 16, 32 or 64)
             const int r = (cb + 16 * h) / cols, at = (cb + 16 * h) % cols;
             if (r == int(rank)) {
-  #pragma unroll
+#pragma unroll
               for (int q4 = 0; q4 < D / 32; ++q4)  // at = 16 q4 (static indexes only)
                 if (at == 16 * q4) {
-  #pragma unroll
+#pragma unroll
                   for (int i = 0; i < 16; ++i) mine_o[16 * q4 + i] = v[16 * h + i];
                 }
             } else {
               const int sender = int(rank) < r ? int(rank) : int(rank) - 1;
-  #pragma unroll
+#pragma unroll
               for (int c = 0; c < 4; ++c) {
                 const uint32_t a =
                     pre_mapa(at_smem(ring + ((size_t(sender) * (cols / 4) + at / 4 + c) * 256 + wg * kPreM + t) * 16), r);
@@ -737,21 +742,21 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       if (mine && !failed) {
         const float inv = L == 0.f ? 0.f : 1.0f / L;
         bf16 *dst = p.out + size_t(b.first + qi) * p.out_stride + size_t(head) * D + own;
-  #pragma unroll
+#pragma unroll
         for (int c8 = 0; c8 < D / 16; ++c8) {
           if (c8 * 8 < cols) {
             float v[8];
-  #pragma unroll
+#pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = mine_o[8 * c8 + i];
             for (int s = 0; s + 1 < int(C); ++s)
-  #pragma unroll
+#pragma unroll
               for (int h = 0; h < 2; ++h) {
                 const float4 f = *reinterpret_cast<const float4 *>(
                     ring + ((size_t(s) * (cols / 4) + 2 * c8 + h) * 256 + wg * kPreM + t) * 16);
                 v[4 * h] += f.x, v[4 * h + 1] += f.y, v[4 * h + 2] += f.z, v[4 * h + 3] += f.w;
               }
             uint32_t o[4];
-  #pragma unroll
+#pragma unroll
             for (int e = 0; e < 4; ++e) {
               const __nv_bfloat162 o2 = __floats2bfloat162_rn(v[2 * e] * inv, v[2 * e + 1] * inv);
               o[e] = *reinterpret_cast<const uint32_t *>(&o2);
@@ -799,7 +804,13 @@ void launch_kv_attn_prefill(const KvPool &pool, int layer, const KvAttnParams &p
   CUtensorMap map;
   if (!encode_rows_map(&map, pool.data, uint64_t(x.total_rows), pool.head_dim, x.box_rows))
     throw Error("RuntimeError", "cuTensorMapEncodeTiled failed for the cache pool");
-  const int cluster = 1;
+  // Blocks of one prompt's chunk that leave SMs idle are split along the keys (over 2, then 4
+  // blocks), as long as each keeps four key tiles.
+  const long long blocks = pairs * p.kv_heads;
+  const long long positions = p.offsets ? (long long)p.pages_per_row << p.page_shift : p.length;
+  const long long keys = p.window ? std::min<long long>(positions, (long long)p.window + p.sinks) : positions;
+  int cluster = 1;
+  while (cluster < 4 && blocks * cluster * 2 <= 148 && keys >= cluster * 2 * 4 * kPreN) cluster *= 2;
   if (pool.head_dim == 128)
     prefill_launch<128>(map, p, x, cluster, st);
   else
