@@ -319,11 +319,20 @@ __global__ void __launch_bounds__(kPreThreads, 1)
   const bool mine = warp < 8 && m < rows_m;
   const int qi = mine ? int(m / G) : 0, head = kvh * G + (mine ? int(m % G) : 0);
   const bf16 *q_row = p.q + size_t(b.first + qi) * p.q_stride + size_t(head) * D;
+  // A warp moves its 32 rows row by row (D / 8 lanes each): whole lines of global memory.
+  constexpr int CPR = D / 8;
   if (warp < 8) {
+    uint4 v[CPR];
 #pragma unroll
-    for (int c = 0; c < D / 8; ++c) {
-      const uint4 v = mine ? *reinterpret_cast<const uint4 *>(q_row + c * 8) : make_uint4(0, 0, 0, 0);
-      *reinterpret_cast<uint4 *>(sm + wg * Cfg::kQ + (c >> 3) * Cfg::kQSlice + at_sw(t, c & 7)) = v;
+    for (int i = 0; i < CPR; ++i) {
+      const int r = (i * 32 + lane) / CPR, c = lane % CPR;
+      const bf16 *src = reinterpret_cast<const bf16 *>(__shfl_sync(0xFFFFFFFFu, (unsigned long long)q_row, r));
+      v[i] = __shfl_sync(0xFFFFFFFFu, int(mine), r) ? *reinterpret_cast<const uint4 *>(src + c * 8) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < CPR; ++i) {
+      const int r = (warp & 3) * 32 + (i * 32 + lane) / CPR, c = lane % CPR;
+      *reinterpret_cast<uint4 *>(sm + wg * Cfg::kQ + (c >> 3) * Cfg::kQSlice + at_sw(r, c & 7)) = v[i];
     }
   }
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -656,29 +665,43 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         at_st32(col_o + cb, o);
       }
     }
+    // The rows' results [cols] go through shared memory (the warp's 32 rows of the tile's Q, whose
+    // products are complete) and leave row by row: whole lines of global memory.
+    unsigned char *stash = sm + wg * Cfg::kQ + (warp & 3) * (32 * D * 2);
+    auto stash_at = [&](int r, int c, int chunks) { return stash + (r * chunks + (c ^ (r & 7 & (chunks - 1)))) * 16; };
+    bf16 *out_row = p.out + size_t(b.first + qi) * p.out_stride + size_t(head) * D;
+    auto flush = [&](int cols, int col0) {
+      __syncwarp();
+      const int chunks = cols / 8;
+#pragma unroll 4
+      for (int i = 0; i < chunks; ++i) {
+        const int r = (i * 32 + lane) / chunks, c = (i * 32 + lane) % chunks;
+        bf16 *dst = reinterpret_cast<bf16 *>(__shfl_sync(0xFFFFFFFFu, (unsigned long long)out_row, r));
+        if (__shfl_sync(0xFFFFFFFFu, int(mine), r))
+          *reinterpret_cast<uint4 *>(dst + col0 + c * 8) = *reinterpret_cast<const uint4 *>(stash_at(r, c, chunks));
+      }
+    };
     if (C == 1) {
       if (!failed) {
         const float inv = row_l == 0.f ? 0.f : 1.0f / row_l;
-        bf16 *dst = p.out + size_t(b.first + qi) * p.out_stride + size_t(head) * D;
 #pragma unroll 1
         for (int cb = 0; cb < D; cb += 32) {
           float v[32];
           at_ld32(col_o + cb, v);
-          if (mine) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              uint32_t w[4];
+          for (int c = 0; c < 4; ++c) {
+            uint32_t w[4];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                // (a row that saw nothing: O was never written)
-                const __nv_bfloat162 o2 = row_l == 0.f ? __floats2bfloat162_rn(0.f, 0.f)
-                                                       : __floats2bfloat162_rn(v[c * 8 + 2 * e] * inv, v[c * 8 + 2 * e + 1] * inv);
-                w[e] = *reinterpret_cast<const uint32_t *>(&o2);
-              }
-              *reinterpret_cast<uint4 *>(dst + cb + c * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+            for (int e = 0; e < 4; ++e) {
+              // (a row that saw nothing: O was never written)
+              const __nv_bfloat162 o2 = row_l == 0.f ? __floats2bfloat162_rn(0.f, 0.f)
+                                                     : __floats2bfloat162_rn(v[c * 8 + 2 * e] * inv, v[c * 8 + 2 * e + 1] * inv);
+              w[e] = *reinterpret_cast<const uint32_t *>(&o2);
             }
+            *reinterpret_cast<uint4 *>(stash_at(lane, cb / 8 + c, D / 8)) = make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
+        flush(D, 0);
       }
     } else {
       // The cluster's states of a row weighted by 2^(m - M); block r finishes columns
@@ -739,9 +762,8 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         }
       }
       pre_cluster_sync();
-      if (mine && !failed) {
+      if (!failed) {
         const float inv = L == 0.f ? 0.f : 1.0f / L;
-        bf16 *dst = p.out + size_t(b.first + qi) * p.out_stride + size_t(head) * D + own;
 #pragma unroll
         for (int c8 = 0; c8 < D / 16; ++c8) {
           if (c8 * 8 < cols) {
@@ -761,9 +783,10 @@ __global__ void __launch_bounds__(kPreThreads, 1)
               const __nv_bfloat162 o2 = __floats2bfloat162_rn(v[2 * e] * inv, v[2 * e + 1] * inv);
               o[e] = *reinterpret_cast<const uint32_t *>(&o2);
             }
-            *reinterpret_cast<uint4 *>(dst + 8 * c8) = make_uint4(o[0], o[1], o[2], o[3]);
+            *reinterpret_cast<uint4 *>(stash_at(lane, c8, cols / 8)) = make_uint4(o[0], o[1], o[2], o[3]);
           }
         }
+        flush(cols, own);
       }
     }
   }
