@@ -462,11 +462,13 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         // bits). Both tiles' warps do so, each before its own product.
         const int k0 = key_tile(b.j0 + i);
         unsigned char *v = ring + slot * 2 * Cfg::kTile;
-        for (int r = 0; r < kPreN; ++r)
-          if (k0 + r >= b.kend || (k0 + r >= b.sinks && k0 + r < b.lo))
-            if (lane < D / 8)
-              *reinterpret_cast<uint4 *>(v + (lane >> 3) * Cfg::kSlice + r * 128 + (lane & 7) * 16) =
-                  make_uint4(0, 0, 0, 0);
+        auto zero = [&](int r0, int r1) {
+          for (int c = max(r0, 0) * (D / 8) + lane; c < min(r1, kPreN) * (D / 8); c += 32)
+            *reinterpret_cast<uint4 *>(v + (c % (D / 8) >> 3) * Cfg::kSlice + c / (D / 8) * 128 + (c & 7) * 16) =
+                make_uint4(0, 0, 0, 0);
+        };
+        zero(b.sinks - k0, b.lo - k0);
+        zero(b.kend - k0, kPreN);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
       }
