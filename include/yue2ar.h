@@ -122,6 +122,12 @@ int yar_model_dims(const yar_model *model, int64_t *dims10);
  * activations, logits, sampler state and the captured decode-step graph. */
 int yar_session_create(yar_model *model, int max_rows, int max_ctx, int page_tokens,
                        yar_session **out);
+/* The same with a pool of `pool_pages` pages (0: enough for every row's max_ctx): rows then
+ * compete for them, and yar_row_reset (so yar_generate too) is refused when they run out.
+ * Rows that share pages (yar_row_fork) or give back what their window hides
+ * (yar_row_release) let fewer pages serve more rows. */
+int yar_session_create_pool(yar_model *model, int max_rows, int max_ctx, int page_tokens, int pool_pages,
+                            yar_session **out);
 int yar_session_free(yar_session *session);
 
 /* Session options. YAR_OPT_PERSISTENT (default 1): run each decode forward of one or two
@@ -136,11 +142,16 @@ int yar_session_free(yar_session *session);
  * 32 KB stages per SM the persistent kernel pulls into L2 ahead of its shared-memory ring
  * (its lookahead while the step waits at operation boundaries). */
 enum { YAR_OPT_PERSISTENT = 1, YAR_OPT_TRACE = 2, YAR_OPT_PREFETCH_STAGES = 3, YAR_OPT_MAX_SPLITS = 4,
-       YAR_OPT_LAYER_DUMP = 5, YAR_OPT_FAULT_INJECT = 6, YAR_OPT_PREFILL_ATTN_TC = 7 };
+       YAR_OPT_LAYER_DUMP = 5, YAR_OPT_FAULT_INJECT = 6, YAR_OPT_PREFILL_ATTN_TC = 7,
+       YAR_OPT_BATCHED_ATTN = 8 };
 /* YAR_OPT_PREFILL_ATTN_TC (default 1): prefill attention for head_dim 128 on tcgen05 tensor
  * cores with TMEM accumulators and TMA-fed K/V; 0 selects the mma.sync kernel (the same
  * quotient; the two differ by rounding: summation order, exp2 of log2-scaled scores and a
- * running maximum raised in steps on the tcgen05 side). */
+ * running maximum raised in steps on the tcgen05 side); 2 selects the kernel of
+ * yar_kv_attn_prefill (faster; weights in BF16 instead of two BF16 parts), which a session
+ * with a sliding window uses in any case. YAR_OPT_BATCHED_ATTN (default 0): 1 runs the
+ * attention of decode steps of 16 and more rows on the kernel of yar_kv_attn_decode (reads
+ * the cache at HBM's rate; another order of summation). */
 /* YAR_OPT_MAX_SPLITS (default 0 = automatic, else 1..32): the number of splits each (row,
  * kv head) of the decode attention is cut into at most — 1 puts a row's whole context in
  * one unit (the longest chain of chunks), for parity tests of the split-KV rescaling.
@@ -226,6 +237,32 @@ int yar_row_position(yar_session *session, int row, int *pos);
  * BF16 values) at `slot` — 0 the embedding, l + 1 the output of layer l. The hidden state
  * between layers of ARModel::hidden (native/src/ar.cpp:262-299), exposed for parity. */
 int yar_row_hidden(yar_session *session, int row, int slot, uint16_t *out, int n);
+
+/* Sliding-window attention for every row of the session (no counterpart in the reference):
+ * from now on the query at position p sees the last `window` positions, its own included,
+ * and the row's first `sinks` (window 0: everything, the default). It holds for prefill and
+ * every decode path. One GPU only. Refused while a row has released pages that the new
+ * window would need. */
+int yar_session_set_window(yar_session *session, int window, int sinks);
+/* Rows as lists of cache pages (no counterpart in the reference). yar_row_fork makes `dst` a
+ * copy of `src` at its present position (cache and last logits) with room for `capacity`
+ * positions; full pages are shared, the one that is part full is copied, and what dst held
+ * is dropped. yar_row_truncate cuts a row back to its first n positions (its logits stay
+ * those of the last forward). yar_row_free gives a row's pages back; it needs yar_row_reset
+ * or a fork before it is used again. yar_row_release gives back the pages that no later
+ * query of the row can see through the session's window (`released`: how many; may be
+ * NULL). A call that would need more pages than the pool has left changes nothing
+ * (YAR_INVALID_INPUT). */
+int yar_row_fork(yar_session *session, int src, int dst, int capacity);
+int yar_row_truncate(yar_session *session, int row, int n);
+int yar_row_free(yar_session *session, int row);
+int yar_row_release(yar_session *session, int row, int *released);
+/* Move the rows' pages to the front of the pool (yar_kv_compact on it); `used` (may be NULL)
+ * receives how many there are. Results do not change. */
+int yar_session_compact(yar_session *session, int *used);
+/* Pages of the pool, those that no row holds, and the highest index that one holds (-1:
+ * none); each may be NULL. */
+int yar_session_pages(yar_session *session, int *total, int *unused, int *highest);
 
 /* The device sampler on host logits (one step), exposed for parity tests of the filter
  * chain and the draw contract. cond/uncond are phase-local BF16 bits of width n

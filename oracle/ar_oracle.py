@@ -132,7 +132,12 @@ class LazyBf16Weights:
 
 
 class OracleAR:
-    """The AR decoder on float32 arrays, with BF16 rounding points when ``bf16``."""
+    """The AR decoder on float32 arrays, with BF16 rounding points when ``bf16``.
+
+    ``window`` / ``sinks``: sliding-window attention — the query at position p sees j <= p with
+    j < sinks or j > p - window (0, the upstream model: every j <= p)."""
+
+    window, sinks = 0, 0
 
     def __init__(self, tensors: dict, dims, bf16: bool = True, prerounded: bool = False, lazy: bool = False):
         self.d = dims
@@ -206,7 +211,10 @@ class OracleAR:
         cos, sin = rope_cos_sin(np.arange(start, end), d.head_dim, d.theta)
         group = d.heads // d.kv_heads
         scale = F32(float(d.head_dim) ** -0.5)
-        visible = np.arange(end)[None, :] <= np.arange(start, end)[:, None]
+        key, query = np.arange(end)[None, :], np.arange(start, end)[:, None]
+        visible = key <= query
+        if self.window:
+            visible &= (key < self.sinks) | (key > query - self.window)
         p = f"model.layers.{i}."
         h = self.rms_norm(x, self.w[p + "input_layernorm.weight"])
         q = self.linear(h, p + "self_attn.q_proj.weight").reshape(T, d.heads, d.head_dim)

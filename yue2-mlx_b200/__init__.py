@@ -90,7 +90,15 @@ def _load_library(path: str = LIB_PATH) -> ctypes.CDLL:
         "yar_model_free": (I, [P]),
         "yar_model_dims": (I, [P, ctypes.POINTER(ctypes.c_int64)]),
         "yar_session_create": (I, [P, I, I, I, ctypes.POINTER(P)]),
+        "yar_session_create_pool": (I, [P, I, I, I, I, ctypes.POINTER(P)]),
         "yar_session_free": (I, [P]),
+        "yar_session_set_window": (I, [P, I, I]),
+        "yar_session_compact": (I, [P, ctypes.POINTER(I)]),
+        "yar_session_pages": (I, [P, ctypes.POINTER(I), ctypes.POINTER(I), ctypes.POINTER(I)]),
+        "yar_row_fork": (I, [P, I, I, I]),
+        "yar_row_truncate": (I, [P, I, I]),
+        "yar_row_free": (I, [P, I]),
+        "yar_row_release": (I, [P, I, ctypes.POINTER(I)]),
         "yar_session_set_option": (I, [P, I, I]),
         "yar_session_trace": (I, [P, ctypes.POINTER(ctypes.c_uint64), ctypes.c_size_t, ctypes.POINTER(ctypes.c_size_t)]),
         "yar_generate": (I, [P, i32p, I, ctypes.POINTER(_Sampling), U64, I, i32p, I, D, I, CANCEL_FN, P,
@@ -222,8 +230,9 @@ class ARModel:
         _check(lib.yar_model_precision_bits(h, ctypes.byref(b)))
         self.precision = {8: "8bit", 4: "4bit"}.get(b.value, "bf16")
 
-    def session(self, max_rows: int = 2, max_ctx: int = 4096, page_tokens: int = 256) -> "Session":
-        return Session(self, max_rows, max_ctx, page_tokens)
+    def session(self, max_rows: int = 2, max_ctx: int = 4096, page_tokens: int = 256,
+                pool_pages: int = 0) -> "Session":
+        return Session(self, max_rows, max_ctx, page_tokens, pool_pages)
 
     def close(self):
         if getattr(self, "_h", None):
@@ -263,9 +272,9 @@ class ARModel:
 class Session:
     """Paged KV cache and decode state for up to ``max_rows`` rows on the model's GPU."""
 
-    def __init__(self, model: ARModel, max_rows: int, max_ctx: int, page_tokens: int):
+    def __init__(self, model: ARModel, max_rows: int, max_ctx: int, page_tokens: int, pool_pages: int = 0):
         h = ctypes.c_void_p()
-        _check(lib.yar_session_create(model._h, max_rows, max_ctx, page_tokens, ctypes.byref(h)))
+        _check(lib.yar_session_create_pool(model._h, max_rows, max_ctx, page_tokens, pool_pages, ctypes.byref(h)))
         self._h, self.model = h, model
         self.max_rows, self.max_ctx = max_rows, max_ctx
 
@@ -313,9 +322,50 @@ class Session:
         """L2 prefetch distance of the persistent decode kernel, in 32 KB stages per SM."""
         _check(lib.yar_session_set_option(self._h, 3, int(n)))
 
-    def set_prefill_attention_tc(self, on: bool):
-        """Prefill attention (head_dim 128) on tcgen05 tensor cores (default) or, off, the mma.sync kernel."""
-        _check(lib.yar_session_set_option(self._h, 7, int(bool(on))))
+    def set_prefill_attention_tc(self, on):
+        """Prefill attention (head_dim 128) on tcgen05 tensor cores (default) or, off, the mma.sync
+        kernel; 2: the kernel of ``kv_attn_prefill``."""
+        _check(lib.yar_session_set_option(self._h, 7, 2 if on == 2 else int(bool(on))))
+
+    def set_batched_attention(self, on: bool):
+        """Attention of decode steps of 16 and more rows on the kernel of ``kv_attn_decode``."""
+        _check(lib.yar_session_set_option(self._h, 8, int(bool(on))))
+
+    def set_window(self, window: int, sinks: int = 0):
+        """Sliding-window attention: a query sees the last ``window`` positions and the first
+        ``sinks`` (0: everything) (yar_session_set_window)."""
+        _check(lib.yar_session_set_window(self._h, window, sinks))
+
+    def fork(self, src: int, dst: int, capacity: int):
+        """Make row ``dst`` a copy of row ``src`` with room for ``capacity`` positions; full pages
+        are shared."""
+        _check(lib.yar_row_fork(self._h, src, dst, capacity))
+
+    def truncate(self, row: int, n: int):
+        """Cut the row back to its first ``n`` positions."""
+        _check(lib.yar_row_truncate(self._h, row, n))
+
+    def free(self, row: int):
+        """Give the row's pages back."""
+        _check(lib.yar_row_free(self._h, row))
+
+    def release(self, row: int) -> int:
+        """Give back the row's pages that its window hides for good; returns how many."""
+        n = ctypes.c_int()
+        _check(lib.yar_row_release(self._h, row, ctypes.byref(n)))
+        return n.value
+
+    def compact(self) -> int:
+        """Move the rows' pages to the front of the pool; returns how many there are."""
+        n = ctypes.c_int()
+        _check(lib.yar_session_compact(self._h, ctypes.byref(n)))
+        return n.value
+
+    def pages(self) -> tuple[int, int, int]:
+        """(pages of the pool, unused ones, the highest index in use or -1)."""
+        t, u, h = ctypes.c_int(), ctypes.c_int(), ctypes.c_int()
+        _check(lib.yar_session_pages(self._h, ctypes.byref(t), ctypes.byref(u), ctypes.byref(h)))
+        return t.value, u.value, h.value
 
     def set_max_splits(self, n: int):
         """Cap the decode attention's splits per (row, kv head); 0 restores the automatic plan."""

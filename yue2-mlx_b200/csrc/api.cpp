@@ -12,7 +12,7 @@ namespace yar {
 Model *load_model(const std::string &dir, int device, uint32_t flags, int tp_rank = 0, int tp_world = 1,
                   const uint8_t *nccl_id = nullptr);
 void free_model(Model *m);
-Session *create_session(Model *m, int max_rows, int max_ctx, int page_tokens);
+Session *create_session(Model *m, int max_rows, int max_ctx, int page_tokens, int pool_pages);
 void free_session(Session *s);
 void row_reset(Session &s, int row, int capacity);
 void row_prefill(Session &s, int row, const int32_t *ids, int n, int phase, int chunk, int (*cancel)(void *),
@@ -197,12 +197,17 @@ int yar_model_dims(const yar_model *model, int64_t *dims) {
   });
 }
 
-int yar_session_create(yar_model *model, int max_rows, int max_ctx, int page_tokens, yar_session **out) {
+int yar_session_create_pool(yar_model *model, int max_rows, int max_ctx, int page_tokens, int pool_pages,
+                            yar_session **out) {
   return guarded([&] {
     need(model && out, "model and out are required");
     *out = nullptr;
-    *out = new yar_session{yar::create_session(model->m, max_rows, max_ctx, page_tokens)};
+    *out = new yar_session{yar::create_session(model->m, max_rows, max_ctx, page_tokens, pool_pages)};
   });
+}
+
+int yar_session_create(yar_model *model, int max_rows, int max_ctx, int page_tokens, yar_session **out) {
+  return yar_session_create_pool(model, max_rows, max_ctx, page_tokens, 0, out);
 }
 
 int yar_session_free(yar_session *session) {
@@ -255,7 +260,13 @@ int yar_session_set_option(yar_session *session, int option, int value) {
       s.graphs.clear();
       s.inject_op = value;
     } else if (option == YAR_OPT_PREFILL_ATTN_TC) {
-      s.prefill_attn_tc = value != 0;
+      s.prefill_attn_tc = value == 2 ? 2 : value != 0;
+    } else if (option == YAR_OPT_BATCHED_ATTN) {
+      YAR_CUDA(cudaSetDevice(s.m->device));
+      YAR_CUDA(cudaStreamSynchronize(s.stream));
+      for (auto &g : s.graphs) cudaGraphExecDestroy(g.exec);  // graphs captured the other kernel
+      s.graphs.clear();
+      s.batched_attn = value != 0;
     } else if (option == YAR_OPT_LAYER_DUMP) {
       YAR_CUDA(cudaSetDevice(s.m->device));
       YAR_CUDA(cudaStreamSynchronize(s.stream));
@@ -379,6 +390,8 @@ int yar_row_kv(yar_session *session, int row, int layer, int start, int count, u
     const auto &d = s.m->d;
     need(row >= 0 && row < s.max_rows && layer >= 0 && layer < d.layers, "row or layer outside the session");
     need(start >= 0 && count >= 0 && start + count <= s.pos[row], "positions outside the row's cache");
+    for (int i = start; i < start + count && size_t(i / s.page_tokens) < s.row_pages[row].size(); ++i)
+      need(s.row_pages[row][i / s.page_tokens] >= 0, "positions outside the row's cache: they have been released");
     YAR_CUDA(cudaSetDevice(s.m->device));
     YAR_CUDA(cudaStreamSynchronize(s.stream));
     std::vector<int> table(s.pages_per_row);
@@ -419,6 +432,64 @@ int yar_row_position(yar_session *session, int row, int *pos) {
     need(session && pos, "session and pos are required");
     need(row >= 0 && row < session->s->max_rows, "row outside the session");
     *pos = session->s->pos[row];
+  });
+}
+
+int yar_row_fork(yar_session *session, int src, int dst, int capacity) {
+  return guarded([&] {
+    need(session, "session is required");
+    yar::row_fork(*session->s, src, dst, capacity);
+  });
+}
+
+int yar_row_truncate(yar_session *session, int row, int n) {
+  return guarded([&] {
+    need(session, "session is required");
+    yar::row_truncate(*session->s, row, n);
+  });
+}
+
+int yar_row_free(yar_session *session, int row) {
+  return guarded([&] {
+    need(session, "session is required");
+    yar::row_free(*session->s, row);
+  });
+}
+
+int yar_row_release(yar_session *session, int row, int *released) {
+  return guarded([&] {
+    need(session, "session is required");
+    const int n = yar::row_release(*session->s, row);
+    if (released) *released = n;
+  });
+}
+
+int yar_session_compact(yar_session *session, int *used) {
+  return guarded([&] {
+    need(session, "session is required");
+    const int n = yar::session_compact(*session->s);
+    if (used) *used = n;
+  });
+}
+
+int yar_session_pages(yar_session *session, int *total, int *unused, int *highest) {
+  return guarded([&] {
+    need(session, "session is required");
+    const auto &s = *session->s;
+    if (total) *total = s.num_pages;
+    if (unused) *unused = int(s.free_pages.size());
+    if (highest) {
+      *highest = -1;
+      for (int p = 0; p < s.num_pages; ++p)
+        if (s.page_refs[p] > 0) *highest = p;
+    }
+  });
+}
+
+int yar_session_set_window(yar_session *session, int window, int sinks) {
+  return guarded([&] {
+    need(session, "session is required");
+    yar::session_set_window(*session->s, window, sinks);
   });
 }
 

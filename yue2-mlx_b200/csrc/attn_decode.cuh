@@ -24,6 +24,9 @@ struct AttnGeom {
   int heads, kv_heads, head_dim, qdim, kvdim, page_tokens, page_shift, pages_per_row, num_pages;
   size_t page_elems;  // kv_heads * P * D
   float eps, scale;
+  // Sliding window (0: everything is visible): the query at position p sees the last `window`
+  // positions, its own included, and the first `sinks`.
+  int window = 0, sinks = 0;
 };
 
 // Address of (layer, kv, kv_head, position) for a row's page table.
@@ -113,12 +116,35 @@ constexpr int kKvChunk = 64;  // positions per KV chunk
 
 // The split plan of a row whose context holds L positions (the new one included): split s
 // covers chunks [s * cps, min((s + 1) * cps, nchunks)); the last split holds the new position.
+// Of a windowed row only the chunks with a visible position count: those of the sinks, then
+// those from the window's start on (attn_chunk_base).
 struct SplitPlan {
   int nchunks, cps, n_splits;
 };
-__host__ __device__ __forceinline__ SplitPlan split_plan(int L, int max_splits) {
+// The hidden positions [h0, h1) of a row of L positions (h0 >= h1: none).
+struct HiddenRange {
+  int h0, h1;
+};
+__host__ __device__ __forceinline__ HiddenRange attn_hidden(const AttnGeom &g, int L) {
+  const int lo = g.window > 0 && L > g.window ? L - g.window : 0;
+  return {g.sinks < lo ? g.sinks : lo, lo};
+}
+// Whole chunks without a visible position, and the first of them.
+__host__ __device__ __forceinline__ int attn_skipped(const HiddenRange &h, int &first) {
+  first = (h.h0 + kKvChunk - 1) / kKvChunk;
+  const int end = h.h1 / kKvChunk;
+  return end > first ? end - first : 0;
+}
+// First position of the row's c-th counted chunk.
+__host__ __device__ __forceinline__ int attn_chunk_base(const AttnGeom &g, int L, int c) {
+  int first;
+  const int skipped = attn_skipped(attn_hidden(g, L), first);
+  return (c < first ? c : c + skipped) * kKvChunk;
+}
+__host__ __device__ __forceinline__ SplitPlan split_plan(const AttnGeom &g, int L, int max_splits) {
   SplitPlan r;
-  r.nchunks = (L + kKvChunk - 1) / kKvChunk;
+  int first;
+  r.nchunks = (L + kKvChunk - 1) / kKvChunk - attn_skipped(attn_hidden(g, L), first);
   r.cps = (r.nchunks + max_splits - 1) / max_splits;
   r.n_splits = (r.nchunks + r.cps - 1) / r.cps;
   return r;
@@ -374,20 +400,21 @@ __device__ __forceinline__ int attn_kchunk(int lane, int j) {
 }
 
 // One chunk for this warp: positions [8w, 8w + 8) of rows [0, n_main) of Ks/Vs (shared
-// memory, row pitch D) and, when `extra`, the new position (knew/vnew) as row n_main.
+// memory, row pitch D) and, when `extra`, the new position (knew/vnew) as row n_main; rows
+// [hide0, hide1) are not visible (a sliding window's) and their contents not used.
 // FP32 scores (mixed-precision BF16 FMAs), the warp's running max/sum/output rescaled by
 // exp(m_old - m_new); only this warp's rows are read.
 // q comes from shared memory (q_b, after attn_qk) chunk by chunk in the same rotated order
 // as the K loads (conflict-free too), which keeps 32 registers free in the caller.
 template <int D, int G>
 __device__ __forceinline__ void attn_chunk(const bf16 (&q_b)[G][D], const bf16 *knew, const bf16 *vnew,
-                                           const bf16 *Ks, const bf16 *Vs, int n_main, bool extra, float scale,
-                                           AttnWarpAcc<D, G> &acc, int tid) {
+                                           const bf16 *Ks, const bf16 *Vs, int n_main, bool extra, int hide0,
+                                           int hide1, float scale, AttnWarpAcc<D, G> &acc, int tid) {
   constexpr int CPP = D / 32, DL = D / 32;
   const int lane = tid & 31, warp = tid >> 5;
   const int n = n_main + (extra ? 1 : 0);
   const int i = warp * 8 + (lane >> 2);
-  const bool valid = i < n;
+  const bool valid = i < n && !(i >= hide0 && i < hide1);
   float sc[G];
   {
     float lo[G], hi[G];
@@ -443,8 +470,8 @@ __device__ __forceinline__ void attn_chunk(const bf16 (&q_b)[G][D], const bf16 *
     float w[G];
 #pragma unroll
     for (int h = 0; h < G; ++h) w[h] = __shfl_sync(0xFFFFFFFFu, pv[h], pp * 4);
-    if (pp < nw) {
-      const int r = warp * 8 + pp;
+    const int r = warp * 8 + pp;
+    if (pp < nw && !(r >= hide0 && r < hide1)) {
       const bf16 *vr = (r < n_main ? Vs + size_t(r) * D : vnew) + lane * DL;
       float v[DL];
       if constexpr (DL == 4) {

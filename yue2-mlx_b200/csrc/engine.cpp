@@ -29,13 +29,16 @@ static T *dmalloc(size_t n) {
   return p;
 }
 
-Session *create_session(Model *m, int max_rows, int max_ctx, int page_tokens) {
+Session *create_session(Model *m, int max_rows, int max_ctx, int page_tokens, int pool_pages) {
   if (max_rows < 1 || max_rows > 256) throw Error("ValueError", "max_rows must be in [1, 256]");
   if (max_ctx < 1 || max_ctx > m->d.context)
     throw Error("ValueError", "KV cache capacity must be in [1, " + std::to_string(m->d.context) + "]");
   if (page_tokens == 0) page_tokens = 256;
   if (page_tokens < 16 || page_tokens > 4096 || (page_tokens & (page_tokens - 1)))
     throw Error("ValueError", "page_tokens must be a power of two in [16, 4096]");
+  const int row_most = (max_ctx + page_tokens - 1) / page_tokens;
+  if (pool_pages < 0 || pool_pages > row_most * max_rows)
+    throw Error("ValueError", "pool_pages must be in [1, " + std::to_string(row_most * max_rows) + "] (0: all of them)");
   YAR_CUDA(cudaSetDevice(m->device));
   auto *s = new Session();
   try {
@@ -44,12 +47,13 @@ Session *create_session(Model *m, int max_rows, int max_ctx, int page_tokens) {
     s->max_rows = max_rows;
     s->max_ctx = max_ctx;
     s->page_tokens = page_tokens;
-    s->pages_per_row = (max_ctx + page_tokens - 1) / page_tokens;
-    s->num_pages = s->pages_per_row * max_rows;
+    s->pages_per_row = row_most;
+    s->num_pages = pool_pages ? pool_pages : s->pages_per_row * max_rows;
     s->kv_page_elems = size_t(d.kv_heads) * page_tokens * d.head_dim;
     YAR_CUDA(cudaStreamCreateWithFlags(&s->stream, cudaStreamNonBlocking));
     s->kv = dmalloc<bf16>(size_t(d.layers) * s->num_pages * 2 * s->kv_page_elems);
     s->row_pages.assign(max_rows, {});
+    s->page_refs.assign(s->num_pages, 0);
     for (int p = s->num_pages - 1; p >= 0; --p) s->free_pages.push_back(p);
     s->d_page_table = dmalloc<int>(size_t(max_rows) * s->pages_per_row);
     YAR_CUDA(cudaMemset(s->d_page_table, 0, size_t(max_rows) * s->pages_per_row * sizeof(int)));
@@ -59,6 +63,7 @@ Session *create_session(Model *m, int max_rows, int max_ctx, int page_tokens) {
     s->d_token = dmalloc<int>(max_rows);
     s->d_active = dmalloc<int>(max_rows);
     s->d_error = dmalloc<int>(1);
+    s->d_len = dmalloc<int>(max_rows);
     for (int *p : {s->d_pos, s->d_cur_pos, s->d_capacity, s->d_token, s->d_active})
       YAR_CUDA(cudaMemset(p, 0, max_rows * sizeof(int)));
     YAR_CUDA(cudaMemset(s->d_error, 0, sizeof(int)));
@@ -151,7 +156,7 @@ void free_session(Session *s) {
   for (auto &g : s->graphs) cudaGraphExecDestroy(g.exec);
   tp_unmap_peers(s->tp_peer_regions);
   for (void *p : std::initializer_list<void *>{s->kv, s->d_page_table, s->d_pos, s->d_cur_pos, s->d_capacity,
-                                               s->d_token, s->d_active, s->d_error, s->xregion, s->qkv,
+                                               s->d_token, s->d_active, s->d_error, s->d_len, s->xregion, s->qkv,
                                                s->attn_part, s->attn_count, s->px, s->ph, s->pqkv, s->pq,
                                                s->pattn, s->pmlp, s->pids, s->d_req, s->d_out_tokens,
                                                s->d_scores, s->d_epoch, s->d_trace, s->gemm_ws, s->tp_send,
@@ -162,7 +167,7 @@ void free_session(Session *s) {
   delete s;
 }
 
-static void check_row(const Session &s, int row) {
+void check_row(const Session &s, int row) {
   if (row < 0 || row >= s.max_rows) throw Error("ValueError", "row outside the session");
 }
 
@@ -171,25 +176,13 @@ void row_reset(Session &s, int row, int capacity) {
   if (capacity < 1 || capacity > s.max_ctx)
     throw Error("ValueError", "KV cache capacity must be in [1, " + std::to_string(s.max_ctx) + "]");
   YAR_CUDA(cudaStreamSynchronize(s.stream));
-  for (int p : s.row_pages[row]) s.free_pages.push_back(p);
-  s.row_pages[row].clear();
   const int need = (capacity + s.page_tokens - 1) / s.page_tokens;
-  if (int(s.free_pages.size()) < need) throw Error("ValueError", "KV page pool exhausted; generation was not shortened");
-  std::vector<int> table(s.pages_per_row, 0);
-  for (int i = 0; i < need; ++i) {
-    table[i] = s.free_pages.back();
-    s.row_pages[row].push_back(table[i]);
-    s.free_pages.pop_back();
-  }
-  YAR_CUDA(cudaMemcpyAsync(s.d_page_table + size_t(row) * s.pages_per_row, table.data(),
-                           table.size() * sizeof(int), cudaMemcpyHostToDevice, s.stream));
-  const int zero = 0;
-  YAR_CUDA(cudaMemcpyAsync(s.d_pos + row, &zero, sizeof(int), cudaMemcpyHostToDevice, s.stream));
-  YAR_CUDA(cudaMemcpyAsync(s.d_capacity + row, &capacity, sizeof(int), cudaMemcpyHostToDevice, s.stream));
-  YAR_CUDA(cudaMemcpyAsync(s.d_active + row, &zero, sizeof(int), cudaMemcpyHostToDevice, s.stream));
-  YAR_CUDA(cudaStreamSynchronize(s.stream));
+  if (pages_after_drop(s, row) < need) throw Error("ValueError", "KV page pool exhausted; generation was not shortened");
+  drop_pages(s, row);
+  for (int i = 0; i < need; ++i) s.row_pages[row].push_back(take_page(s));
   s.capacity[row] = capacity;
   s.pos[row] = 0;
+  upload_row(s, row);
 }
 
 // Phase columns [c0, c1) of the LM head for `n_rows` input rows into out ([n_rows][stride],
@@ -409,7 +402,10 @@ static void decode_forward_batched(Session &s, int n_rows, int phase) {
     const LayerWeights &w = m.layers[l];
     launch_rmsnorm_rows(s.x, w.ln1, n_rows, H, d.eps, s.ph, st);
     gemm(s.ph, H, w.qkv, d.qkv_rows(), s.qkv, d.qkv_rows(), kEpiStore);
-    launch_attn_decode(m, s, l, n_rows, st, splits);
+    if (s.batched_attn)
+      launch_attn_decode_batched(m, s, l, n_rows, st);
+    else
+      launch_attn_decode(m, s, l, n_rows, st, splits);
     tp_gather(m, s, s.attn, n_rows, ls.Qf, ls.Ql);
     gemm(s.attn, ls.Qf, w.o, ls.Hs, s.x + ls.h0, H, kEpiResidual);
     tp_gather(m, s, s.x, n_rows, H, ls.Hs);
@@ -680,8 +676,7 @@ std::string generate(Session &s, const int32_t *prefix, int n_prefix, const ::ya
   *truncated = eos ? 0 : 1;
   // Release the request's pages (caches are request-local, sampling.cpp:208-210).
   for (int r = 0; r < rows; ++r) {
-    for (int p : s.row_pages[r]) s.free_pages.push_back(p);
-    s.row_pages[r].clear();
+    drop_pages(s, r);
     s.capacity[r] = 0;
   }
   nlohmann::json timing = {{"seconds", seconds},
@@ -860,8 +855,7 @@ std::string generate_requests(Session &s, int n_req, int slots, const int32_t *p
         truncated[r] = pg[0] > dn ? 0 : 1;  // a sampled end token is counted in step, not stored
         total += dn;
         ++finished;
-        for (int p : s.row_pages[row]) s.free_pages.push_back(p);
-        s.row_pages[row].clear();
+        drop_pages(s, row);
         s.capacity[row] = 0;
         slot_req[row] = -1;
         if (next < n_req) {

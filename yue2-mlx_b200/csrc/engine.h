@@ -163,6 +163,9 @@ void launch_gemv(const bf16 *W, int N, int K, const bf16 *in, int in_stride, con
 // `max_splits` (0: the session's) caps the splits per (row, kv head); fewer, longer splits
 // suit large batches.
 void launch_attn_decode(const Model &m, Session &s, int layer, int n_rows, cudaStream_t st, int max_splits = 0);
+// The same for steps of many rows: q/k norm, RoPE and the KV append of every row, then the paged
+// attention operator (kernels_kv_attn.cu).
+void launch_attn_decode_batched(const Model &m, Session &s, int layer, int n_rows, cudaStream_t st);
 void launch_sampler(const Model &m, Session &s, int n_requests, cudaStream_t st);
 // Prefill (T tokens of one row).
 void launch_embed_tokens(const bf16 *embed, const int *ids, int T, int H, bf16 *x, cudaStream_t st);
@@ -197,6 +200,7 @@ void configure_attn_tc_kernels();
 void configure_gemv_tma_kernels();
 void configure_persistent_kernels();
 void configure_sampler_kernels();
+void configure_kv_kernels();
 bool persistent_supported(const Model &m, int n_rows);
 // Encodes m.d_wmaps (after the weights are uploaded); leaves it null when a K is not a
 // multiple of 2048.
@@ -221,7 +225,10 @@ struct Session {
   // Paged KV pool: [layer][page][k|v][kv_head][page_tokens][head_dim] BF16.
   bf16 *kv = nullptr;
   size_t kv_page_elems = 0;  // elements of one (layer, page, k|v) block: kv_heads*P*D
+  // A row's pages in order (-1: released, behind its window), the number of rows that hold
+  // each page, and the pages that none holds.
   std::vector<std::vector<int>> row_pages;
+  std::vector<int> page_refs;
   std::vector<int> free_pages;
   int *d_page_table = nullptr;  // [max_rows][pages_per_row]
   int *d_pos = nullptr;         // [max_rows] next position (== tokens in cache)
@@ -230,6 +237,7 @@ struct Session {
   int *d_token = nullptr;       // [max_rows]
   int *d_active = nullptr;      // [max_rows]
   int *d_error = nullptr;       // sticky device error flags
+  int *d_len = nullptr;         // [max_rows] cached positions of a batched step's rows (0: inactive)
   std::vector<int> capacity;    // host mirror
   std::vector<int> pos;         // host mirror
   // Decode activations.
@@ -259,7 +267,12 @@ struct Session {
   int *h_pinned = nullptr;  // pinned staging for small D2H reads
   // Persistent decode kernel: operation counters and the completed-step epoch.
   bool use_persistent = true;
-  bool prefill_attn_tc = true;  // head_dim 128 prefill attention on tcgen05 (else mma.sync)
+  // Prefill attention: 1 tcgen05 for head_dim 128, 0 mma.sync, 2 the paged operator (kernels_kv_prefill.cu).
+  int prefill_attn_tc = 1;
+  // Sliding-window attention (0: off): a query sees the last attn_window positions, its own
+  // included, and the row's first attn_sinks.
+  int attn_window = 0, attn_sinks = 0;
+  bool batched_attn = false;  // steps of 16+ rows: attention by the paged operator (kernels_kv_attn.cu)
   int persistent_ok[3] = {-1, -1, -1};  // per row count: unknown / no / yes
   int *d_ctr = nullptr;
   int *d_epoch = nullptr;
@@ -295,6 +308,19 @@ struct Session {
   long long tp_epoch_steps = 0;  // persistent steps since the counters were last zeroed
   size_t trace_elems = 0;
 };
+
+// A row's pages (kv_rows.cpp). Pages are counted: a forked row shares its parent's full pages.
+void check_row(const Session &s, int row);
+int take_page(Session &s);                             // an unused page (the caller has checked that there is one)
+void drop_pages(Session &s, int row);                  // the row holds no page any more
+int pages_after_drop(const Session &s, int row);       // unused pages, the row's own included
+void upload_row(Session &s, int row);                  // the row's table, position and capacity to the device; inactive
+void row_fork(Session &s, int src, int dst, int capacity);
+void row_truncate(Session &s, int row, int n);
+void row_free(Session &s, int row);
+int row_release(Session &s, int row);
+int session_compact(Session &s);
+void session_set_window(Session &s, int window, int sinks);
 
 constexpr int kCandCap = 2048;
 

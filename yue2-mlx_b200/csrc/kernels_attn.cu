@@ -7,6 +7,7 @@
 // table maps logical page i (positions i*P .. i*P+P-1) to a physical page. Physical slot
 // = RoPE position (modeling_yue2.py:383-393: StaticKVCache writes slot pos).
 #include "attn_decode.cuh"
+#include "kv_ops.h"
 #include "tma_ring.cuh"
 
 namespace yar {
@@ -26,6 +27,8 @@ static AttnGeom geom(const Model &m, const Session &s) {
   g.page_elems = s.kv_page_elems;
   g.eps = m.d.eps;
   g.scale = float(1.0 / std::sqrt(double(m.d.head_dim)));
+  g.window = s.attn_window;
+  g.sinks = s.attn_sinks;
   return g;
 }
 
@@ -63,13 +66,14 @@ __global__ void __launch_bounds__(kAttnThreads) k_attn_decode(DecodeAttnParams p
   __syncthreads();
   if (!rs.active) return;
   const int pos = rs.pos;
-  const SplitPlan sp = split_plan(pos + 1, p.max_splits);
+  const SplitPlan sp = split_plan(p.g, pos + 1, p.max_splits);
+  const HiddenRange hide = attn_hidden(p.g, pos + 1);
   if (split >= sp.n_splits) return;  // beyond the context: no work, no arrival
   const int c0 = split * sp.cps, c1 = min((split + 1) * sp.cps, sp.nchunks);
   // Chunk c's cached K and V rows (positions < pos: the new one is appended by attn_qk and
   // read from shared memory) into buffer `slot`, as one cp.async group.
   auto issue = [&](int c, int slot) {
-    const int base = c * kKvChunk, n_main = min(kKvChunk, pos - base);
+    const int base = attn_chunk_base(p.g, pos + 1, c), n_main = min(kKvChunk, pos - base);
     bf16 *kb = kvbuf + size_t(slot) * 2 * kKvChunk * D, *vb = kb + kKvChunk * D;
     if (bulk) {
       if (tid == 0) {
@@ -84,6 +88,7 @@ __global__ void __launch_bounds__(kAttnThreads) k_attn_decode(DecodeAttnParams p
     }
     for (int idx = tid; idx < n_main * (D / 8); idx += kAttnThreads) {
       const int r = idx / (D / 8), cc = idx % (D / 8);
+      if (base + r >= hide.h0 && base + r < hide.h1) continue;  // (its page may be another row's by now)
       const bf16 *ks = kv_row_ptr<D>(p, rs, row, p.layer, 0, kvh, base + r) + cc * 8;
       const bf16 *vs = kv_row_ptr<D>(p, rs, row, p.layer, 1, kvh, base + r) + cc * 8;
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(
@@ -111,7 +116,7 @@ __global__ void __launch_bounds__(kAttnThreads) k_attn_decode(DecodeAttnParams p
   bool bad = false;
   int done = 0;  // chunks whose copies completed
   for (int c = c0; c < c1; ++c) {
-    const int slot = (c - c0) & 1, base = c * kKvChunk, n_main = min(kKvChunk, pos - base);
+    const int slot = (c - c0) & 1, base = attn_chunk_base(p.g, pos + 1, c), n_main = min(kKvChunk, pos - base);
     // The other buffer was last read by chunk c - 1, which every warp had finished at the
     // barrier ending that iteration: it is free for chunk c + 1.
     if (c + 1 < c1 && !bad) {
@@ -133,8 +138,8 @@ __global__ void __launch_bounds__(kAttnThreads) k_attn_decode(DecodeAttnParams p
     }
     team_sync(1);
     const bf16 *kb = kvbuf + size_t(slot) * 2 * kKvChunk * D;
-    attn_chunk<D, G>(sm.q_b, sm.knew, sm.vnew, kb, kb + kKvChunk * D, n_main, pos - base < kKvChunk, p.g.scale,
-                     wacc, tid);
+    attn_chunk<D, G>(sm.q_b, sm.knew, sm.vnew, kb, kb + kKvChunk * D, n_main, pos - base < kKvChunk, hide.h0 - base,
+                     hide.h1 - base, p.g.scale, wacc, tid);
     team_sync(1);
   }
   if (bad)
@@ -230,6 +235,90 @@ __global__ void __launch_bounds__(256) k_qkv_post(QkvPostParams p) {
     for (int d = lane; d < D; d += 32) dst[d] = f2bf(v[d]);
     __syncwarp();
   }
+}
+
+// The same for a decode step of many rows: one CTA per row, at its latched position; an
+// inactive row gets a length of 0.
+struct QkvRowsParams {
+  QkvPostParams q;
+  const int *page_table, *cur_pos, *active;
+  int *len;
+};
+
+template <int D>
+__global__ void __launch_bounds__(256) k_qkv_post_rows(QkvRowsParams p) {
+  __shared__ float buf[8][D];
+  const AttnGeom &g = p.q.g;
+  const int row = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int pos = p.cur_pos[row], on = p.active[row];
+  if (threadIdx.x == 0) p.len[row] = on ? pos + 1 : 0;
+  if (!on) return;
+  const int *ptab = p.page_table + size_t(row) * g.pages_per_row;
+  const bf16 *src = p.q.qkv + size_t(row) * (g.qdim + 2 * g.kvdim);
+  const float *cosr = p.q.cos_tab + size_t(pos) * (D / 2), *sinr = p.q.sin_tab + size_t(pos) * (D / 2);
+  for (int h = warp; h < g.heads + 2 * g.kv_heads; h += 8) {
+    const bf16 *hs = src + h * D;
+    if (h >= g.heads + g.kv_heads) {
+      bf16 *dst = kv_addr(p.q.pool, g, ptab, p.q.layer, 1, h - g.heads - g.kv_heads, pos);
+      for (int d = lane; d < D; d += 32) dst[d] = hs[d];
+      continue;
+    }
+    float *v = buf[warp];
+    for (int d = lane; d < D; d += 32) v[d] = bf2f(hs[d]);
+    __syncwarp();
+    const bool is_k = h >= g.heads;
+    norm_rope_head<D>(v, is_k ? p.q.kn : p.q.qn, cosr, sinr, g.eps, lane);
+    bf16 *dst = is_k ? kv_addr(p.q.pool, g, ptab, p.q.layer, 0, h - g.heads, pos)
+                     : p.q.q_out + (size_t(row) * g.heads + h) * D;
+    for (int d = lane; d < D; d += 32) dst[d] = f2bf(v[d]);
+    __syncwarp();
+  }
+}
+
+// A layer's pool as the paged operators take it.
+static KvAttnParams paged_params(const Model &m, const Session &s, const AttnGeom &g, int layer) {
+  KvAttnParams a;
+  a.page_elems = 2 * g.page_elems;
+  a.kv = s.kv + size_t(layer) * s.num_pages * a.page_elems;
+  a.pages = s.num_pages;
+  a.heads = m.d.heads, a.kv_heads = m.d.kv_heads;
+  a.page_shift = g.page_shift;
+  a.table_stride = a.pages_per_row = s.pages_per_row;
+  a.q = s.pq;
+  a.q_stride = m.d.qdim();
+  a.out_stride = m.full.qdim();
+  a.window = s.attn_window, a.sinks = s.attn_sinks;
+  a.scale = g.scale;
+  a.error = s.d_error;
+  return a;
+}
+
+void launch_attn_decode_batched(const Model &m, Session &s, int layer, int n_rows, cudaStream_t st) {
+  QkvRowsParams p;
+  p.q.g = geom(m, s);
+  p.q.layer = layer;
+  p.q.pool = s.kv;
+  p.q.qkv = s.qkv;
+  p.q.qn = m.layers[layer].qn;
+  p.q.kn = m.layers[layer].kn;
+  p.q.cos_tab = m.rope_cos;
+  p.q.sin_tab = m.rope_sin;
+  p.q.q_out = s.pq;
+  p.page_table = s.d_page_table;
+  p.cur_pos = s.d_cur_pos;
+  p.active = s.d_active;
+  p.len = s.d_len;
+  if (m.d.head_dim == 128)
+    k_qkv_post_rows<128><<<n_rows, 256, 0, st>>>(p);
+  else
+    k_qkv_post_rows<64><<<n_rows, 256, 0, st>>>(p);
+  YAR_CUDA(cudaGetLastError());
+  KvAttnParams a = paged_params(m, s, p.q.g, layer);
+  a.table = s.d_page_table;
+  a.rows = n_rows;
+  a.lengths = s.d_len;
+  a.out = s.attn + m.tp.q_row0;
+  launch_kv_attn_decode(a, m.d.head_dim, st);
 }
 
 void launch_qkv_post_prefill(const Model &m, Session &s, int layer, int row, int start, int T,
@@ -629,6 +718,20 @@ void launch_attn_prefill(const Model &m, Session &s, int layer, int row, int sta
   p.out = s.pattn + m.tp.q_row0;
   p.out_stride = m.full.qdim();
   const int D = m.d.head_dim;
+  if (s.attn_window > 0 || s.prefill_attn_tc == 2) {  // the paged operator: any window, head_dim 64 and 128
+    KvPool pool;
+    pool.data = s.kv;
+    pool.layers = m.d.layers, pool.pages = s.num_pages, pool.kv_heads = m.d.kv_heads;
+    pool.page_tokens = s.page_tokens, pool.page_shift = p.g.page_shift, pool.head_dim = D;
+    KvAttnParams a = paged_params(m, s, p.g, layer);
+    a.table = p.ptab;
+    a.rows = 1;
+    a.length = start + T;
+    a.n_queries = T;
+    a.out = p.out;
+    launch_kv_attn_prefill(pool, layer, a, st);
+    return;
+  }
   if (D == 128 && s.prefill_attn_tc && launch_attn_prefill_tc(m, s, p.g, layer, row, start, T, st)) return;
   dim3 grid((T + 63) / 64, m.d.heads);
   if (D == 128)

@@ -162,18 +162,18 @@ struct UnitInfo {
   bool active;
 };
 template <int NB>
-__device__ __forceinline__ int step_units(const StepRows<NB> &r, int kvh_n, int max_splits) {
+__device__ __forceinline__ int step_units(const StepRows<NB> &r, const AttnGeom &g, int max_splits) {
   int U = 0;
-  for (int b = 0; b < NB; ++b) U += kvh_n * (r.active[b] ? split_plan(r.pos[b] + 1, max_splits).n_splits : 1);
+  for (int b = 0; b < NB; ++b) U += g.kv_heads * (r.active[b] ? split_plan(g, r.pos[b] + 1, max_splits).n_splits : 1);
   return U;
 }
 template <int NB>
-__device__ __forceinline__ UnitInfo step_unit(const StepRows<NB> &r, int kvh_n, int max_splits, int u) {
+__device__ __forceinline__ UnitInfo step_unit(const StepRows<NB> &r, const AttnGeom &g, int max_splits, int u) {
   UnitInfo ui{};
   for (int b = 0; b < NB; ++b) {
     const bool act = r.active[b] != 0;
-    const SplitPlan sp = act ? split_plan(r.pos[b] + 1, max_splits) : SplitPlan{0, 1, 1};
-    const int ub = kvh_n * sp.n_splits;
+    const SplitPlan sp = act ? split_plan(g, r.pos[b] + 1, max_splits) : SplitPlan{0, 1, 1};
+    const int ub = g.kv_heads * sp.n_splits;
     if (u < ub || b == NB - 1) {
       ui.row = b;
       ui.active = act;
@@ -328,15 +328,15 @@ struct Producer {
       rows.active[b] = a && q < __ldcg(capacity + b);
       rows.pos[b] = q;
     }
-    const int U = step_units(rows, g.kv_heads, max_splits);
+    const int U = step_units(rows, g, max_splits);
     for (int u = arank; u < U; u += gridDim.x) {
-      const UnitInfo ui = step_unit(rows, g.kv_heads, max_splits, u);
+      const UnitInfo ui = step_unit(rows, g, max_splits, u);
       for (int c = ui.c0; c < ui.c1; ++c) {
         if (nkv == kMaxCtaChunks) {
           atomicOr(error, 32);
           return false;
         }
-        const int base = c * kKvChunk;
+        const int base = attn_chunk_base(g, rows.pos[ui.row] + 1, c);
         kv[nkv++] = KvChunkRef{__ldcg(page_table + size_t(ui.row) * g.pages_per_row + (base >> g.page_shift)),
                                ui.kvh, base, min(kKvChunk, rows.pos[ui.row] - base)};
       }
@@ -693,12 +693,12 @@ __global__ void __launch_bounds__(kPersistThreads, 1) k_decode_persistent(const 
     srows.active[b] = rowst[b].active;
     srows.pos[b] = rowst[b].pos;
   }
-  const int U = step_units(srows, kvh_n, nsplit), arank = p.attn_rank[blockIdx.x];
+  const int U = step_units(srows, p.ap.g, nsplit), arank = p.attn_rank[blockIdx.x];
   // Merge jobs of this step: rows that are active and split their context.
   bool merge_row[NB];
   int merge_splits[NB], n_merges = 0;
   for (int b = 0; b < NB; ++b) {
-    merge_splits[b] = srows.active[b] ? split_plan(srows.pos[b] + 1, nsplit).n_splits : 1;
+    merge_splits[b] = srows.active[b] ? split_plan(p.ap.g, srows.pos[b] + 1, nsplit).n_splits : 1;
     merge_row[b] = srows.active[b] && merge_splits[b] > 1;
     if (merge_row[b]) n_merges += kvh_n;
   }
@@ -779,7 +779,7 @@ __global__ void __launch_bounds__(kPersistThreads, 1) k_decode_persistent(const 
           if (p.inject_op == c_op(l, 1)) ap.qkv_flag ^= 0x80000000u;
           long long itk = it;
           for (int ku = 0, u = arank; u < U; ++ku, u += gridDim.x) {
-            const UnitInfo ui = step_unit(srows, kvh_n, nsplit, u);
+            const UnitInfo ui = step_unit(srows, p.ap.g, nsplit, u);
             const int nch = ui.c1 - ui.c0;
             unsigned long long *st =
                 (trace && ku == 0) ? trace + (size_t(blockIdx.x) * (5 * nL + 1) + 5 * l + 1) * 8 : nullptr;
@@ -809,9 +809,10 @@ __global__ void __launch_bounds__(kPersistThreads, 1) k_decode_persistent(const 
               if (j == 0) attn_stamp(st, 1, ctid);  // the unit's first chunk has landed
               if (!wbad) {
                 const bf16 *ks = reinterpret_cast<const bf16 *>(ringb + size_t(sidx) * kSlot);
-                const int base = (ui.c0 + j) * kKvChunk, n_main = min(kKvChunk, rs.pos - base);
+                const int base = attn_chunk_base(ap.g, rs.pos + 1, ui.c0 + j), n_main = min(kKvChunk, rs.pos - base);
+                const HiddenRange hide = attn_hidden(ap.g, rs.pos + 1);
                 attn_chunk<128, 2>(team_sm->q_b, team_sm->knew, team_sm->vnew, ks, ks + kKvChunk * 128, n_main,
-                                   rs.pos - base < kKvChunk, ap.g.scale, wacc, ctid);
+                                   rs.pos - base < kKvChunk, hide.h0 - base, hide.h1 - base, ap.g.scale, wacc, ctid);
               }
               __syncwarp();
               if (lane == 0 && landed) mbar_arrive(&empty[sidx]);
@@ -1070,6 +1071,8 @@ void launch_decode_persistent(const Model &m, Session &s, int n_rows, int phase,
   while ((1 << a.g.page_shift) < s.page_tokens) ++a.g.page_shift;
   if ((1 << a.g.page_shift) != s.page_tokens || s.page_tokens < kKvChunk)
     throw Error("RuntimeError", "persistent decode needs power-of-two pages of at least 64 positions");
+  a.g.window = s.attn_window;
+  a.g.sinks = s.attn_sinks;
   a.g.pages_per_row = s.pages_per_row;
   a.g.num_pages = s.num_pages;
   a.g.page_elems = s.kv_page_elems;
