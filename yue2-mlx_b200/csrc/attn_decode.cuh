@@ -125,7 +125,10 @@ struct SplitPlan {
 struct HiddenRange {
   int h0, h1;
 };
+// WIN: the session has a window (a kernel instance of its own: the others keep their code).
+template <bool WIN>
 __host__ __device__ __forceinline__ HiddenRange attn_hidden(const AttnGeom &g, int L) {
+  if constexpr (!WIN) return {0, 0};
   const int lo = g.window > 0 && L > g.window ? L - g.window : 0;
   return {g.sinks < lo ? g.sinks : lo, lo};
 }
@@ -136,15 +139,21 @@ __host__ __device__ __forceinline__ int attn_skipped(const HiddenRange &h, int &
   return end > first ? end - first : 0;
 }
 // First position of the row's c-th counted chunk.
+template <bool WIN>
 __host__ __device__ __forceinline__ int attn_chunk_base(const AttnGeom &g, int L, int c) {
+  if constexpr (!WIN) return c * kKvChunk;
   int first;
-  const int skipped = attn_skipped(attn_hidden(g, L), first);
+  const int skipped = attn_skipped(attn_hidden<WIN>(g, L), first);
   return (c < first ? c : c + skipped) * kKvChunk;
 }
+template <bool WIN>
 __host__ __device__ __forceinline__ SplitPlan split_plan(const AttnGeom &g, int L, int max_splits) {
   SplitPlan r;
-  int first;
-  r.nchunks = (L + kKvChunk - 1) / kKvChunk - attn_skipped(attn_hidden(g, L), first);
+  r.nchunks = (L + kKvChunk - 1) / kKvChunk;
+  if constexpr (WIN) {
+    int first;
+    r.nchunks -= attn_skipped(attn_hidden<WIN>(g, L), first);
+  }
   r.cps = (r.nchunks + max_splits - 1) / max_splits;
   r.n_splits = (r.nchunks + r.cps - 1) / r.cps;
   return r;
@@ -406,7 +415,7 @@ __device__ __forceinline__ int attn_kchunk(int lane, int j) {
 // exp(m_old - m_new); only this warp's rows are read.
 // q comes from shared memory (q_b, after attn_qk) chunk by chunk in the same rotated order
 // as the K loads (conflict-free too), which keeps 32 registers free in the caller.
-template <int D, int G>
+template <int D, int G, bool WIN>
 __device__ __forceinline__ void attn_chunk(const bf16 (&q_b)[G][D], const bf16 *knew, const bf16 *vnew,
                                            const bf16 *Ks, const bf16 *Vs, int n_main, bool extra, int hide0,
                                            int hide1, float scale, AttnWarpAcc<D, G> &acc, int tid) {
@@ -414,7 +423,7 @@ __device__ __forceinline__ void attn_chunk(const bf16 (&q_b)[G][D], const bf16 *
   const int lane = tid & 31, warp = tid >> 5;
   const int n = n_main + (extra ? 1 : 0);
   const int i = warp * 8 + (lane >> 2);
-  const bool valid = i < n && !(i >= hide0 && i < hide1);
+  const bool valid = i < n && !(WIN && i >= hide0 && i < hide1);
   float sc[G];
   {
     float lo[G], hi[G];
@@ -470,8 +479,8 @@ __device__ __forceinline__ void attn_chunk(const bf16 (&q_b)[G][D], const bf16 *
     float w[G];
 #pragma unroll
     for (int h = 0; h < G; ++h) w[h] = __shfl_sync(0xFFFFFFFFu, pv[h], pp * 4);
-    const int r = warp * 8 + pp;
-    if (pp < nw && !(r >= hide0 && r < hide1)) {
+    if (pp < nw && !(WIN && warp * 8 + pp >= hide0 && warp * 8 + pp < hide1)) {
+      const int r = warp * 8 + pp;
       const bf16 *vr = (r < n_main ? Vs + size_t(r) * D : vnew) + lane * DL;
       float v[DL];
       if constexpr (DL == 4) {

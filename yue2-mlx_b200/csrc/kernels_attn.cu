@@ -44,7 +44,7 @@ static AttnGeom geom(const Model &m, const Session &s) {
 template <int D>
 __host__ __device__ constexpr size_t attn_decode_dyn_smem() { return size_t(2) * 2 * kKvChunk * D * sizeof(bf16); }
 
-template <int D, int G>
+template <int D, int G, bool WIN>
 __global__ void __launch_bounds__(kAttnThreads) k_attn_decode(DecodeAttnParams p) {
   __shared__ AttnTeamSmem<D, G> sm;
   __shared__ AttnRow<D> rs;
@@ -66,14 +66,14 @@ __global__ void __launch_bounds__(kAttnThreads) k_attn_decode(DecodeAttnParams p
   __syncthreads();
   if (!rs.active) return;
   const int pos = rs.pos;
-  const SplitPlan sp = split_plan(p.g, pos + 1, p.max_splits);
-  const HiddenRange hide = attn_hidden(p.g, pos + 1);
+  const SplitPlan sp = split_plan<WIN>(p.g, pos + 1, p.max_splits);
+  const HiddenRange hide = attn_hidden<WIN>(p.g, pos + 1);
   if (split >= sp.n_splits) return;  // beyond the context: no work, no arrival
   const int c0 = split * sp.cps, c1 = min((split + 1) * sp.cps, sp.nchunks);
   // Chunk c's cached K and V rows (positions < pos: the new one is appended by attn_qk and
   // read from shared memory) into buffer `slot`, as one cp.async group.
   auto issue = [&](int c, int slot) {
-    const int base = attn_chunk_base(p.g, pos + 1, c), n_main = min(kKvChunk, pos - base);
+    const int base = attn_chunk_base<WIN>(p.g, pos + 1, c), n_main = min(kKvChunk, pos - base);
     bf16 *kb = kvbuf + size_t(slot) * 2 * kKvChunk * D, *vb = kb + kKvChunk * D;
     if (bulk) {
       if (tid == 0) {
@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(kAttnThreads) k_attn_decode(DecodeAttnParams p
     }
     for (int idx = tid; idx < n_main * (D / 8); idx += kAttnThreads) {
       const int r = idx / (D / 8), cc = idx % (D / 8);
-      if (base + r >= hide.h0 && base + r < hide.h1) continue;  // (its page may be another row's by now)
+      if (WIN && base + r >= hide.h0 && base + r < hide.h1) continue;  // (its page may be another row's by now)
       const bf16 *ks = kv_row_ptr<D>(p, rs, row, p.layer, 0, kvh, base + r) + cc * 8;
       const bf16 *vs = kv_row_ptr<D>(p, rs, row, p.layer, 1, kvh, base + r) + cc * 8;
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(
@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(kAttnThreads) k_attn_decode(DecodeAttnParams p
   bool bad = false;
   int done = 0;  // chunks whose copies completed
   for (int c = c0; c < c1; ++c) {
-    const int slot = (c - c0) & 1, base = attn_chunk_base(p.g, pos + 1, c), n_main = min(kKvChunk, pos - base);
+    const int slot = (c - c0) & 1, base = attn_chunk_base<WIN>(p.g, pos + 1, c), n_main = min(kKvChunk, pos - base);
     // The other buffer was last read by chunk c - 1, which every warp had finished at the
     // barrier ending that iteration: it is free for chunk c + 1.
     if (c + 1 < c1 && !bad) {
@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(kAttnThreads) k_attn_decode(DecodeAttnParams p
     }
     team_sync(1);
     const bf16 *kb = kvbuf + size_t(slot) * 2 * kKvChunk * D;
-    attn_chunk<D, G>(sm.q_b, sm.knew, sm.vnew, kb, kb + kKvChunk * D, n_main, pos - base < kKvChunk, hide.h0 - base,
+    attn_chunk<D, G, WIN>(sm.q_b, sm.knew, sm.vnew, kb, kb + kKvChunk * D, n_main, pos - base < kKvChunk, hide.h0 - base,
                      hide.h1 - base, p.g.scale, wacc, tid);
     team_sync(1);
   }
@@ -181,14 +181,15 @@ void launch_attn_decode(const Model &m, Session &s, int layer, int n_rows, cudaS
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   const int G = m.d.heads / m.d.kv_heads;
+  const bool win = p.g.window > 0;
   if (m.d.head_dim == 128 && G == 2)
-    YAR_CUDA(cudaLaunchKernelEx(&cfg, k_attn_decode<128, 2>, p));
+    YAR_CUDA(cudaLaunchKernelEx(&cfg, win ? k_attn_decode<128, 2, true> : k_attn_decode<128, 2, false>, p));
   else if (m.d.head_dim == 128 && G == 1)
-    YAR_CUDA(cudaLaunchKernelEx(&cfg, k_attn_decode<128, 1>, p));
+    YAR_CUDA(cudaLaunchKernelEx(&cfg, win ? k_attn_decode<128, 1, true> : k_attn_decode<128, 1, false>, p));
   else if (m.d.head_dim == 64 && G == 2)
-    YAR_CUDA(cudaLaunchKernelEx(&cfg, k_attn_decode<64, 2>, p));
+    YAR_CUDA(cudaLaunchKernelEx(&cfg, win ? k_attn_decode<64, 2, true> : k_attn_decode<64, 2, false>, p));
   else if (m.d.head_dim == 64 && G == 1)
-    YAR_CUDA(cudaLaunchKernelEx(&cfg, k_attn_decode<64, 1>, p));
+    YAR_CUDA(cudaLaunchKernelEx(&cfg, win ? k_attn_decode<64, 1, true> : k_attn_decode<64, 1, false>, p));
   else
     throw Error("ValueError", "head_dim must be 64 or 128 and the GQA group 1 or 2");
 }
@@ -688,14 +689,12 @@ __global__ void __launch_bounds__(128) k_attn_prefill_mma(PrefillAttnParams p) {
 }
 
 void configure_attn_kernels() {
-  YAR_CUDA(cudaFuncSetAttribute(k_attn_decode<128, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                int(attn_decode_dyn_smem<128>())));
-  YAR_CUDA(cudaFuncSetAttribute(k_attn_decode<128, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                int(attn_decode_dyn_smem<128>())));
-  YAR_CUDA(cudaFuncSetAttribute(k_attn_decode<64, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                int(attn_decode_dyn_smem<64>())));
-  YAR_CUDA(cudaFuncSetAttribute(k_attn_decode<64, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                int(attn_decode_dyn_smem<64>())));
+  for (auto k : {k_attn_decode<128, 2, false>, k_attn_decode<128, 1, false>, k_attn_decode<128, 2, true>,
+                 k_attn_decode<128, 1, true>})
+    YAR_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(attn_decode_dyn_smem<128>())));
+  for (auto k : {k_attn_decode<64, 2, false>, k_attn_decode<64, 1, false>, k_attn_decode<64, 2, true>,
+                 k_attn_decode<64, 1, true>})
+    YAR_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(attn_decode_dyn_smem<64>())));
   YAR_CUDA(cudaFuncSetAttribute(k_attn_prefill_mma, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kPfSmem)));
   YAR_CUDA(cudaFuncSetAttribute(k_attn_prefill<64>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                 int(prefill_attn_smem(64))));

@@ -161,18 +161,18 @@ struct UnitInfo {
   int row, kvh, split, n_splits, c0, c1;
   bool active;
 };
-template <int NB>
+template <int NB, bool WIN>
 __device__ __forceinline__ int step_units(const StepRows<NB> &r, const AttnGeom &g, int max_splits) {
   int U = 0;
-  for (int b = 0; b < NB; ++b) U += g.kv_heads * (r.active[b] ? split_plan(g, r.pos[b] + 1, max_splits).n_splits : 1);
+  for (int b = 0; b < NB; ++b) U += g.kv_heads * (r.active[b] ? split_plan<WIN>(g, r.pos[b] + 1, max_splits).n_splits : 1);
   return U;
 }
-template <int NB>
+template <int NB, bool WIN>
 __device__ __forceinline__ UnitInfo step_unit(const StepRows<NB> &r, const AttnGeom &g, int max_splits, int u) {
   UnitInfo ui{};
   for (int b = 0; b < NB; ++b) {
     const bool act = r.active[b] != 0;
-    const SplitPlan sp = act ? split_plan(g, r.pos[b] + 1, max_splits) : SplitPlan{0, 1, 1};
+    const SplitPlan sp = act ? split_plan<WIN>(g, r.pos[b] + 1, max_splits) : SplitPlan{0, 1, 1};
     const int ub = g.kv_heads * sp.n_splits;
     if (u < ub || b == NB - 1) {
       ui.row = b;
@@ -295,7 +295,7 @@ struct ProdCursor {
 // stages into the ring, and `prefetch_stages` stages ahead of that to pull the same
 // bytes into L2 (cp.async.bulk.prefetch), so HBM keeps streaming while the consumers wait
 // at operation boundaries and the ring copies of those stages then hit L2.
-template <int NB, int QB>
+template <int NB, int QB, bool WIN>
 struct Producer {
   static constexpr bool kQ8 = QB != 0;  // quantized weights (8 or 4 bits)
   static constexpr int kQStage = kQ8 ? q_stage_bytes<(QB ? QB : 8)>() : 0;
@@ -328,15 +328,15 @@ struct Producer {
       rows.active[b] = a && q < __ldcg(capacity + b);
       rows.pos[b] = q;
     }
-    const int U = step_units(rows, g, max_splits);
+    const int U = step_units<NB, WIN>(rows, g, max_splits);
     for (int u = arank; u < U; u += gridDim.x) {
-      const UnitInfo ui = step_unit(rows, g, max_splits, u);
+      const UnitInfo ui = step_unit<NB, WIN>(rows, g, max_splits, u);
       for (int c = ui.c0; c < ui.c1; ++c) {
         if (nkv == kMaxCtaChunks) {
           atomicOr(error, 32);
           return false;
         }
-        const int base = attn_chunk_base(g, rows.pos[ui.row] + 1, c);
+        const int base = attn_chunk_base<WIN>(g, rows.pos[ui.row] + 1, c);
         kv[nkv++] = KvChunkRef{__ldcg(page_table + size_t(ui.row) * g.pages_per_row + (base >> g.page_shift)),
                                ui.kvh, base, min(kKvChunk, rows.pos[ui.row] - base)};
       }
@@ -447,7 +447,7 @@ struct Producer {
 
 // QB: the weights' precision — 0 (BF16, stage-map copies), 8 or 4 (affine 8- or 4-bit stage
 // images, ring_consume_q8); everything else is shared.
-template <int NB, int QB>
+template <int NB, int QB, bool WIN>
 __global__ void __launch_bounds__(kPersistThreads, 1) k_decode_persistent(const __grid_constant__ PersistParams p) {
   // 1024-byte alignment: the weight stages are 128-byte-swizzled tensor copies.
   extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -539,7 +539,7 @@ __global__ void __launch_bounds__(kPersistThreads, 1) k_decode_persistent(const 
       auto pstamp = [&](int o, int k) {
         if (trace) trace[(size_t(blockIdx.x) * (5 * nL + 1) + o) * 8 + k] = sm_clock();
       };
-      Producer<NB, QB> pr(p, epoch, kv_chunks);
+      Producer<NB, QB, WIN> pr(p, epoch, kv_chunks);
       ProdCursor ic, pc;
       pr.begin(ic);
       pc = ic;
@@ -693,12 +693,12 @@ __global__ void __launch_bounds__(kPersistThreads, 1) k_decode_persistent(const 
     srows.active[b] = rowst[b].active;
     srows.pos[b] = rowst[b].pos;
   }
-  const int U = step_units(srows, p.ap.g, nsplit), arank = p.attn_rank[blockIdx.x];
+  const int U = step_units<NB, WIN>(srows, p.ap.g, nsplit), arank = p.attn_rank[blockIdx.x];
   // Merge jobs of this step: rows that are active and split their context.
   bool merge_row[NB];
   int merge_splits[NB], n_merges = 0;
   for (int b = 0; b < NB; ++b) {
-    merge_splits[b] = srows.active[b] ? split_plan(p.ap.g, srows.pos[b] + 1, nsplit).n_splits : 1;
+    merge_splits[b] = srows.active[b] ? split_plan<WIN>(p.ap.g, srows.pos[b] + 1, nsplit).n_splits : 1;
     merge_row[b] = srows.active[b] && merge_splits[b] > 1;
     if (merge_row[b]) n_merges += kvh_n;
   }
@@ -779,7 +779,7 @@ __global__ void __launch_bounds__(kPersistThreads, 1) k_decode_persistent(const 
           if (p.inject_op == c_op(l, 1)) ap.qkv_flag ^= 0x80000000u;
           long long itk = it;
           for (int ku = 0, u = arank; u < U; ++ku, u += gridDim.x) {
-            const UnitInfo ui = step_unit(srows, p.ap.g, nsplit, u);
+            const UnitInfo ui = step_unit<NB, WIN>(srows, p.ap.g, nsplit, u);
             const int nch = ui.c1 - ui.c0;
             unsigned long long *st =
                 (trace && ku == 0) ? trace + (size_t(blockIdx.x) * (5 * nL + 1) + 5 * l + 1) * 8 : nullptr;
@@ -809,9 +809,9 @@ __global__ void __launch_bounds__(kPersistThreads, 1) k_decode_persistent(const 
               if (j == 0) attn_stamp(st, 1, ctid);  // the unit's first chunk has landed
               if (!wbad) {
                 const bf16 *ks = reinterpret_cast<const bf16 *>(ringb + size_t(sidx) * kSlot);
-                const int base = attn_chunk_base(ap.g, rs.pos + 1, ui.c0 + j), n_main = min(kKvChunk, rs.pos - base);
-                const HiddenRange hide = attn_hidden(ap.g, rs.pos + 1);
-                attn_chunk<128, 2>(team_sm->q_b, team_sm->knew, team_sm->vnew, ks, ks + kKvChunk * 128, n_main,
+                const int base = attn_chunk_base<WIN>(ap.g, rs.pos + 1, ui.c0 + j), n_main = min(kKvChunk, rs.pos - base);
+                const HiddenRange hide = attn_hidden<WIN>(ap.g, rs.pos + 1);
+                attn_chunk<128, 2, WIN>(team_sm->q_b, team_sm->knew, team_sm->vnew, ks, ks + kKvChunk * 128, n_main,
                                    rs.pos - base < kKvChunk, hide.h0 - base, hide.h1 - base, ap.g.scale, wacc, ctid);
               }
               __syncwarp();
@@ -957,18 +957,25 @@ size_t persistent_smem(int NB, int QB) {
   return ring + (act > teams ? act : teams) + size_t(ring_gred_floats(NB)) * 4;
 }
 
-// The kernel instance for a row count and precision.
-static const void *persistent_kernel(int n_rows, int bits) {
-  if (bits == 8) return n_rows == 1 ? (const void *)k_decode_persistent<1, 8> : (const void *)k_decode_persistent<2, 8>;
-  if (bits == 4) return n_rows == 1 ? (const void *)k_decode_persistent<1, 4> : (const void *)k_decode_persistent<2, 4>;
-  return n_rows == 1 ? (const void *)k_decode_persistent<1, 0> : (const void *)k_decode_persistent<2, 0>;
+// The kernel instance for a row count, a precision and with or without a sliding window.
+using PersistKernel = void (*)(PersistParams);
+template <int QB>
+static PersistKernel persistent_kernel(int n_rows, bool win) {
+  if (n_rows == 1) return win ? k_decode_persistent<1, QB, true> : k_decode_persistent<1, QB, false>;
+  return win ? k_decode_persistent<2, QB, true> : k_decode_persistent<2, QB, false>;
+}
+static PersistKernel persistent_kernel(int n_rows, int bits, bool win) {
+  return bits == 8   ? persistent_kernel<8>(n_rows, win)
+         : bits == 4 ? persistent_kernel<4>(n_rows, win)
+                     : persistent_kernel<0>(n_rows, win);
 }
 
 void configure_persistent_kernels() {
   for (int bits : {0, 8, 4})
     for (int rows = 1; rows <= 2; ++rows)
-      YAR_CUDA(cudaFuncSetAttribute(persistent_kernel(rows, bits), cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    int(persistent_smem(rows, bits))));
+      for (bool win : {false, true})
+        YAR_CUDA(cudaFuncSetAttribute((const void *)persistent_kernel(rows, bits, win),
+                                      cudaFuncAttributeMaxDynamicSharedMemorySize, int(persistent_smem(rows, bits))));
 }
 
 // True when the persistent kernel handles this model and row count.
@@ -1002,14 +1009,16 @@ bool persistent_supported(const Model &m, int n_rows) {
   // The register split (setmaxnreg) assumes the launch's per-thread registers.
   cudaFuncAttributes fa{};
   if (m.bits && (!m.d_qlayers || m.tp_world > 1)) return false;
-  if (cudaFuncGetAttributes(&fa, persistent_kernel(n_rows, m.bits)) != cudaSuccess ||
-      fa.numRegs != kPersistLaunchRegs)
-    return false;
   int per_sm = 0;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, persistent_kernel(n_rows, m.bits), kPersistThreads,
-                                                    persistent_smem(n_rows, m.bits)) != cudaSuccess)
-    return false;
-  return per_sm >= 1;
+  for (bool win : {false, true}) {
+    const void *k = (const void *)persistent_kernel(n_rows, m.bits, win);
+    if (cudaFuncGetAttributes(&fa, k) != cudaSuccess || fa.numRegs != kPersistLaunchRegs) return false;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k, kPersistThreads, persistent_smem(n_rows, m.bits)) !=
+            cudaSuccess ||
+        per_sm < 1)
+      return false;
+  }
+  return true;
 }
 
 void launch_decode_persistent(const Model &m, Session &s, int n_rows, int phase, cudaStream_t st) {
@@ -1123,15 +1132,7 @@ void launch_decode_persistent(const Model &m, Session &s, int n_rows, int phase,
   attr[0].val.cooperative = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (m.bits == 8)
-    YAR_CUDA(n_rows == 1 ? cudaLaunchKernelEx(&cfg, k_decode_persistent<1, 8>, p)
-                         : cudaLaunchKernelEx(&cfg, k_decode_persistent<2, 8>, p));
-  else if (m.bits == 4)
-    YAR_CUDA(n_rows == 1 ? cudaLaunchKernelEx(&cfg, k_decode_persistent<1, 4>, p)
-                         : cudaLaunchKernelEx(&cfg, k_decode_persistent<2, 4>, p));
-  else
-    YAR_CUDA(n_rows == 1 ? cudaLaunchKernelEx(&cfg, k_decode_persistent<1, 0>, p)
-                         : cudaLaunchKernelEx(&cfg, k_decode_persistent<2, 0>, p));
+  YAR_CUDA(cudaLaunchKernelEx(&cfg, persistent_kernel(n_rows, m.bits, s.attn_window > 0), p));
 }
 
 }  // namespace yar
