@@ -628,13 +628,13 @@ def kv_compact(pool, page_table, counts, out=None, error=None, stream=None):
     if out.shape != page_table.shape:
         raise ValueError("out must have page_table's shape")
     new = _kv_rows(out, counts)
-    remap = page_table.new_empty((c_pool.pages,))
-    used = page_table.new_empty((1,))
-    work = page_table.new_empty((1 + 2 * c_pool.pages,))
+    n = c_pool.pages
+    buf = page_table.new_empty((3 * n + 2,))  # remap [n], used [1], scratch [1 + 2 n]
+    at = buf.data_ptr()
     _check(lib.yar_kv_compact(c_pool, rows.page_table, rows.table_stride, rows.rows, rows.pages_per_row, rows.lengths,
-                              new.page_table, new.table_stride, remap.data_ptr(), used.data_ptr(), work.data_ptr(),
-                              _kv_error(error), _kv_stream(pool, stream)))
-    return out, remap, used
+                              new.page_table, new.table_stride, at, at + 4 * n, at + 4 * n + 4, _kv_error(error),
+                              _kv_stream(pool, stream)))
+    return out, buf[:n], buf[n:n + 1]
 
 
 def header_functions(header: str | None = None) -> list[str]:
