@@ -143,6 +143,19 @@ __device__ __forceinline__ void exp2_poly2(uint64_t t, float &e0, float &e1) {
   e0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(r0) << 23));
   e1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(r1) << 23));
 }
+// 16 columns of this warp's lanes (waited for).
+__device__ __forceinline__ void ld16(uint32_t addr, float *v) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+      "[%16];\n tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
 // Store 32 columns of this warp's lanes (not waited for).
 __device__ __forceinline__ void st32_async(uint32_t addr, const uint32_t *v) {
   asm volatile(
@@ -730,63 +743,49 @@ __global__ void __launch_bounds__(kPreThreads, 1)
           if (lv[c] != 0.f) L += lv[c] * (mv[c] == M ? 1.f : pre_ex2(mv[c] - M));
         w = row_l == 0.f ? 0.f : row_m == M ? 1.f : pre_ex2(row_m - M);
       }
+      // (Loops of 16 columns, not unrolled: a block runs this once, and fetching the code of an
+      // unrolled exchange took longer than the exchange.)
       const int cols = D / int(C), own = int(rank) * cols;
-      float mine_o[D / 2];  // this block's columns (C >= 2)
-      if (warp < 8) {
+#pragma unroll 1
+      for (int c16 = 0; c16 < D; c16 += 16) {
+        const int r = c16 / cols;
+        if (r == int(rank)) continue;
+        float v[16];
+        ld16(col_o + c16, v);
+        const int sender = int(rank) < r ? int(rank) : int(rank) - 1;
+        const uint32_t a = pre_mapa(
+            at_smem(ring + ((size_t(sender) * (cols / 4) + (c16 % cols) / 4) * 256 + wg * kPreM + t) * 16), r);
 #pragma unroll
-        for (int cb = 0; cb < D; cb += 32) {
-          float v[32];
-          at_ld32(col_o + cb, v);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = row_l == 0.f ? 0.f : v[i] * w;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {  // 16 columns: all of one block's (cols is 16, 32 or 64)
-            const int r = (cb + 16 * h) / cols, at = (cb + 16 * h) % cols;
-            if (r == int(rank)) {
-#pragma unroll
-              for (int q4 = 0; q4 < D / 32; ++q4)  // at = 16 q4 (static indexes only)
-                if (at == 16 * q4) {
-#pragma unroll
-                  for (int i = 0; i < 16; ++i) mine_o[16 * q4 + i] = v[16 * h + i];
-                }
-            } else {
-              const int sender = int(rank) < r ? int(rank) : int(rank) - 1;
-#pragma unroll
-              for (int c = 0; c < 4; ++c) {
-                const uint32_t a =
-                    pre_mapa(at_smem(ring + ((size_t(sender) * (cols / 4) + at / 4 + c) * 256 + wg * kPreM + t) * 16), r);
-                asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(a), "f"(v[16 * h + 4 * c]),
-                             "f"(v[16 * h + 4 * c + 1]), "f"(v[16 * h + 4 * c + 2]), "f"(v[16 * h + 4 * c + 3])
-                             : "memory");
-              }
-            }
-          }
-        }
+        for (int c = 0; c < 4; ++c)
+          asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(a + c * 4096),
+                       "f"(row_l == 0.f ? 0.f : v[4 * c] * w), "f"(row_l == 0.f ? 0.f : v[4 * c + 1] * w),
+                       "f"(row_l == 0.f ? 0.f : v[4 * c + 2] * w), "f"(row_l == 0.f ? 0.f : v[4 * c + 3] * w)
+                       : "memory");
       }
       pre_cluster_sync();
       if (!failed) {
         const float inv = L == 0.f ? 0.f : 1.0f / L;
+#pragma unroll 1
+        for (int c16 = 0; c16 < cols; c16 += 16) {
+          float v[16];
+          ld16(col_o + own + c16, v);
 #pragma unroll
-        for (int c8 = 0; c8 < D / 16; ++c8) {
-          if (c8 * 8 < cols) {
-            float v[8];
+          for (int e = 0; e < 16; ++e) v[e] = row_l == 0.f ? 0.f : v[e] * w;
+          for (int s = 0; s + 1 < int(C); ++s)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = mine_o[8 * c8 + i];
-            for (int s = 0; s + 1 < int(C); ++s)
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const float4 f = *reinterpret_cast<const float4 *>(
-                    ring + ((size_t(s) * (cols / 4) + 2 * c8 + h) * 256 + wg * kPreM + t) * 16);
-                v[4 * h] += f.x, v[4 * h + 1] += f.y, v[4 * h + 2] += f.z, v[4 * h + 3] += f.w;
-              }
-            uint32_t o[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const __nv_bfloat162 o2 = __floats2bfloat162_rn(v[2 * e] * inv, v[2 * e + 1] * inv);
-              o[e] = *reinterpret_cast<const uint32_t *>(&o2);
+            for (int c = 0; c < 4; ++c) {
+              const float4 f = *reinterpret_cast<const float4 *>(
+                  ring + ((size_t(s) * (cols / 4) + c16 / 4 + c) * 256 + wg * kPreM + t) * 16);
+              v[4 * c] += f.x, v[4 * c + 1] += f.y, v[4 * c + 2] += f.z, v[4 * c + 3] += f.w;
             }
-            *reinterpret_cast<uint4 *>(stash_at(lane, c8, cols / 8)) = make_uint4(o[0], o[1], o[2], o[3]);
+          uint32_t o[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const __nv_bfloat162 o2 = __floats2bfloat162_rn(v[2 * e] * inv, v[2 * e + 1] * inv);
+            o[e] = *reinterpret_cast<const uint32_t *>(&o2);
           }
+          *reinterpret_cast<uint4 *>(stash_at(lane, c16 / 8, cols / 8)) = make_uint4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<uint4 *>(stash_at(lane, c16 / 8 + 1, cols / 8)) = make_uint4(o[4], o[5], o[6], o[7]);
         }
         flush(cols, own);
       }
