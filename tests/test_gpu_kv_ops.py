@@ -214,32 +214,39 @@ def test_values_that_are_not_finite_reach_only_the_queries_that_see_them(yar, to
     q, _ = queries(torch, n, heads, dim, 8)
     offs = torch.tensor([0, n], dtype=torch.int32, device="cuda")
     clean = yar.kv_attn_prefill(c.pool, 1, c.table, c.lengths, offs, q, window=window, sinks=sinks)
-    at = 270
-    page, slot = int(c.table[0, at // 64]), at % 64
-    sees = torch.tensor([at in visible(n, i, window, sinks) for i in range(n)], device="cuda")
-    assert 0 < sees.sum() < n
-    for what, value in (("v", float("inf")), ("v", float("nan")), ("k", float("nan"))):
-        pool = c.pool.clone()
-        pool[1, page, 0 if what == "k" else 1, 0, slot, 7] = value  # KV head 0: heads 0 and 1
-        got = yar.kv_attn_prefill(pool, 1, c.table, c.lengths, offs, q, window=window, sinks=sinks)
-        err = (got.float() - clean.float()).abs()
-        assert torch.equal(got[:, 2:], clean[:, 2:])
-        hidden = err[~sees][:, :2]  # recomputed sums may round differently
-        assert torch.isfinite(hidden).all() and (hidden <= 2.0 ** -6 * (clean[~sees][:, :2].float().abs() + 1)).all()
-        seen = got[sees][:, :2].float()
-        if what == "k":
-            assert torch.isnan(seen).all()
-        else:
-            assert not torch.isfinite(seen[..., 7]).any()
-            rest = torch.ones(dim, dtype=torch.bool)
-            rest[7] = False
-            assert torch.isfinite(seen[..., rest]).all()
-        one = yar.kv_attn_decode(pool, 1, c.table, c.lengths, q[-1:], window=window, sinks=sinks)
-        before = yar.kv_attn_decode(c.pool, 1, c.table, c.lengths, q[-1:], window=window, sinks=sinks)
-        if not sees[-1]:
-            assert torch.equal(one, before)
-        else:
-            assert not torch.isfinite(one[0, :2].float()).all() and torch.equal(one[:, 2:], before[:, 2:])
+    last = yar.kv_attn_decode(c.pool, 1, c.table, c.lengths, q[-1:], window=window, sinks=sinks)
+    # Positions all over a key tile, in tiles that most queries see whole and in edge tiles.
+    for at in (270, 256, 257, 260, 261, 275, 2, 317, 399):
+        page, slot = int(c.table[0, at // 64]), at % 64
+        sees = torch.tensor([at in visible(n, i, window, sinks) for i in range(n)], device="cuda")
+        assert 0 < sees.sum() < n or at == 2
+        for what, value in (("v", float("inf")), ("v", float("nan")), ("k", float("nan")), ("k", float("inf"))):
+            pool = c.pool.clone()
+            pool[1, page, 0 if what == "k" else 1, 0, slot, 7] = value  # KV head 0: heads 0 and 1
+            got = yar.kv_attn_prefill(pool, 1, c.table, c.lengths, offs, q, window=window, sinks=sinks)
+            err = (got.float() - clean.float()).abs()
+            assert torch.equal(got[:, 2:], clean[:, 2:])
+            hidden = err[~sees][:, :2]  # recomputed sums may round differently
+            assert torch.isfinite(hidden).all()
+            assert (hidden <= 2.0 ** -6 * (clean[~sees][:, :2].float().abs() + 1)).all()
+            seen = got[sees][:, :2].float()
+            if what == "v":
+                assert not torch.isfinite(seen[..., 7]).any()
+                rest = torch.ones(dim, dtype=torch.bool)
+                rest[7] = False
+                assert torch.isfinite(seen[..., rest]).all()
+            else:  # NaN scores, or infinite ones: +inf makes its weight NaN, -inf makes it vanish
+                plus = torch.ones_like(seen[..., 0], dtype=torch.bool)
+                if value == float("inf"):
+                    plus = q[sees][:, :2, 7].float() >= 0
+                assert torch.isnan(seen[plus]).all()
+                assert torch.isfinite(seen[~plus]).all()
+            one = yar.kv_attn_decode(pool, 1, c.table, c.lengths, q[-1:], window=window, sinks=sinks)
+            assert torch.equal(one[:, 2:], last[:, 2:])
+            if not sees[-1]:
+                assert torch.equal(one, last)
+            elif what == "v" or value != float("inf"):
+                assert not torch.isfinite(one[0, :2].float()).all()
 
 
 def test_strided_tensors_and_rows_behind_the_last(yar, torch):
@@ -385,6 +392,60 @@ def test_calls_on_two_streams_at_once(yar, torch):
     torch.cuda.synchronize()
     for o in outs[0] + outs[1]:
         assert torch.equal(o, want)
+
+
+def test_offsets_beyond_32_bits(yar, torch):
+    """A pool of 2.7 billion values (5.4 GB), used at its end: attention, copies and compaction."""
+    kv, dim, page, pages = 8, 128, 64, 20600
+    pool = torch.empty((1, pages, 2, kv, page, dim), dtype=torch.bfloat16, device="cuda")
+    assert pool.numel() > 2 ** 31
+    c = Cache(torch, [200], kv, dim, page, seed=17)
+    small = c.table[0].long()
+    far = torch.tensor([pages - 1, pages - 7, pages - 3, pages - 2], device="cuda")
+    pool[0, far] = c.pool[1][small]
+    table = far.to(torch.int32)[None].contiguous()
+    q, _ = queries(torch, 1, 16, dim, 3)
+    q9, _ = queries(torch, 9, 16, dim, 4)
+    offs = torch.tensor([0, 9], dtype=torch.int32, device="cuda")
+    want = yar.kv_attn_decode(c.pool, 1, c.table, c.lengths, q), yar.kv_attn_prefill(c.pool, 1, c.table, c.lengths, offs, q9)
+    assert torch.equal(yar.kv_attn_decode(pool, 0, table, c.lengths, q), want[0])
+    assert torch.equal(yar.kv_attn_prefill(pool, 0, table, c.lengths, offs, q9), want[1])
+    new, remap, used = yar.kv_compact(pool, table, torch.tensor([4], dtype=torch.int32, device="cuda"))
+    assert used.item() == 4 and sorted(new[0].tolist()) == [0, 1, 2, 3]
+    assert torch.equal(yar.kv_attn_decode(pool, 0, new, c.lengths, q), want[0])
+    yar.kv_copy_pages(pool, new[0].tolist(), [pages - 20, pages - 21, pages - 22, pages - 23])
+    table = torch.tensor([[pages - 20, pages - 21, pages - 22, pages - 23]], dtype=torch.int32, device="cuda")
+    assert torch.equal(yar.kv_attn_prefill(pool, 0, table, c.lengths, offs, q9), want[1])
+
+
+def test_calls_from_two_threads(yar, torch):
+    import threading
+    c = Cache(torch, [500, 90], 2, 64, 16, seed=19)
+    q, _ = queries(torch, 2, 4, 64, 5)
+    offs = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+    want = yar.kv_attn_decode(c.pool, 1, c.table, c.lengths, q), yar.kv_attn_prefill(c.pool, 1, c.table, c.lengths, offs, q)
+    torch.cuda.synchronize()
+    bad = []
+
+    def work():
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            got = [(yar.kv_attn_decode(c.pool, 1, c.table, c.lengths, q),
+                    yar.kv_attn_prefill(c.pool, 1, c.table, c.lengths, offs, q)) for _ in range(50)]
+            try:
+                yar.kv_attn_decode(c.pool, 7, c.table, c.lengths, q)  # an error of this thread alone
+                bad.append("layer")
+            except yar.YarError as e:
+                bad.extend([] if "layer" in e.message else [e.message])
+        s.synchronize()
+        bad.extend(1 for a, b in got if not (torch.equal(a, want[0]) and torch.equal(b, want[1])))
+
+    threads = [threading.Thread(target=work) for _ in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
 
 
 def test_host_memory_is_refused(yar, torch):

@@ -118,12 +118,13 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+// The largest of three; NaN when one is.
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-// 2^t of two values t <= 100 on the FMA units (t below -125 gives 2^-125): t = n + f with f in
+// 2^t of two finite values t <= 100 on the FMA units (t below -125 gives 2^-125): t = n + f with f in
 // [-1/2, 1/2], 2^f by the degree-4 polynomial of least maximal relative error on that interval
 // (2.6e-6, Remez exchange), n added to its exponent.
 __device__ __forceinline__ void exp2_poly2(uint64_t t, float &e0, float &e1) {
@@ -588,9 +589,9 @@ __global__ void __launch_bounds__(kPreThreads, 1)
 #pragma unroll
         for (int c = 0; c < 4; ++c) mx4[c] = max3(mx4[c], s[k + c], s[k + 4 + c]);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) mx4[c] = fmaxf(mx4[c], s[kPreN - 4 + c]);
-      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sl2;
-      const bool raise = mx > row_m + kPreRescale;  // false while both are -inf
+      for (int c = 0; c < 4; ++c) mx4[c] = max3(mx4[c], mx4[c], s[kPreN - 4 + c]);
+      const float mx = max3(max3(mx4[0], mx4[1], mx4[2]), mx4[2], mx4[3]) * sl2;
+      const bool raise = mx > row_m + kPreRescale;  // false while both are -inf, and for NaN
       if (__any_sync(0xFFFFFFFFu, raise)) {
         const float c = raise ? pre_ex2(row_m - mx) : 1.f;  // 0 when m was -inf
         row_l *= c;
@@ -631,8 +632,9 @@ __global__ void __launch_bounds__(kPreThreads, 1)
           w[k] = *reinterpret_cast<const uint32_t *>(&h);
         }
       };
-      // Tiles with masked scores take the exponential unit only: 2^-inf has to be 0.
-      if (edge)
+      // Tiles with masked scores (2^-inf has to be 0), or with infinite ones or NaN (they have to
+      // stay NaN), take the exponential unit only.
+      if (edge || __any_sync(0xFFFFFFFFu, !(fabsf(mx) < INFINITY)))
         weights(std::false_type{});
       else
         weights(std::true_type{});
