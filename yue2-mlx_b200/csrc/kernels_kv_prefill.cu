@@ -180,8 +180,8 @@ __device__ __forceinline__ uint32_t pre_mapa(uint32_t a, uint32_t rank) {
 // Where a block's work lies.
 struct PreBlock {
   int row, first, n, len;  // the row, its first query, its queries, its cached positions
-  int pair;
-  int p0, p1;                // positions of its first and last query
+  int q0, r0, rows;  // its first M row is head r0 (of the group) of query q0; its M rows
+  int p0, p1;        // positions of its first and last query
   int kend, lo, sinks;       // keys seen by any query: [0, sinks) and [lo, kend)
   int sink_tiles, wfirst;    // key tile j: j < sink_tiles ? j : wfirst + j - sink_tiles
   int j0, j1;                // this block's share of the key tiles
@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
   // ---- which row and which 256 of its M rows: the last pairs (the longest) first -----------
   if (warp == 0) {
     const int slot = x.pairs - 1 - int(blockIdx.x / C);
-    int row = -1, first = 0, n = 0, pair = 0;
+    int row = -1, first = 0, n = 0, pair = 0, len = p.length;
     if (!p.offsets) {
       row = 0, n = p.n_queries, pair = slot;
       if ((long long)pair * 256 >= (long long)n * G) row = -1;
@@ -220,9 +220,10 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       int before = 0;
       for (int r0 = 0; r0 < p.rows && row < 0; r0 += 32) {
         const int r = r0 + lane;
-        int f = 0, k = 0;
+        int f = 0, k = 0, l = 0;
         if (r < p.rows) {
           f = p.offsets[r];
+          l = p.lengths[r];
           const int e = p.offsets[r + 1];
           if (f >= 0 && e >= f && e <= p.n_queries)
             k = e - f;
@@ -242,6 +243,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
           row = r0 + src;
           first = __shfl_sync(0xFFFFFFFFu, f, src);
           n = __shfl_sync(0xFFFFFFFFu, k, src);
+          len = __shfl_sync(0xFFFFFFFFu, l, src);
           pair = slot - before - __shfl_sync(0xFFFFFFFFu, incl - mine, src);
         }
         before += __shfl_sync(0xFFFFFFFFu, incl, 31);
@@ -249,18 +251,20 @@ __global__ void __launch_bounds__(kPreThreads, 1)
     }
     if (lane == 0) {
       PreBlock b;
-      b.row = row, b.first = first, b.n = n, b.pair = pair;
+      b.row = row, b.first = first, b.n = n;
       if (row >= 0) {
         const int cap = p.pages_per_row << p.page_shift;
-        int len = p.lengths ? p.lengths[row] : p.length;
         if (len > cap) {
           if (p.error) atomicOr(p.error, kKvBadLength);
           len = cap;
         }
         b.len = max(len, 0);
-        const long long m0 = (long long)pair * 256, m1 = min((long long)n * G, m0 + 256) - 1;
-        b.p0 = b.len - n + int(m0 / G);
-        b.p1 = b.len - n + int(m1 / G);
+        const long long m0 = (long long)pair * 256;
+        b.rows = int(min((long long)n * G - m0, 256ll));
+        b.q0 = int(m0 / G);
+        b.r0 = int(m0 % G);
+        b.p0 = b.len - n + b.q0;
+        b.p1 = b.len - n + b.q0 + (b.r0 + b.rows - 1) / G;
         b.kend = b.p1 + 1;
         b.lo = p.window ? max(0, b.p0 - p.window + 1) : 0;
         b.sinks = p.window ? min(p.sinks, b.lo) : 0;
@@ -298,24 +302,12 @@ __global__ void __launch_bounds__(kPreThreads, 1)
   auto key_tile = [&](int j) { return (j < b.sink_tiles ? j : b.wfirst + j - b.sink_tiles) * kPreN; };
   // Whether some query of the block sees a key in [k0, k1).
   auto needed = [&](int k0, int k1) { return k0 < b.kend && !(k0 >= b.sinks && k1 <= b.lo); };
-  // Bad pages among the keys to come (their pieces are then masked one by one).
-  for (int i = tid; i < (b.j1 - b.j0) * pieces; i += kPreThreads) {
-    const int k0 = key_tile(b.j0 + i / pieces) + (i % pieces) * x.box_rows;
-    if (needed(k0, k0 + x.box_rows)) {
-      const int page = tab[k0 >> p.page_shift];
-      if (page < 0 || page >= p.pages) {
-        s_bad = 1;
-        if (p.error) atomicOr(p.error, kKvBadPage);
-      }
-    }
-  }
-  const long long rows_m = (long long)b.n * G;
   const int nt = b.j1 - b.j0;
   auto tile_of = [&](int t) {
     PreTile r;
-    const long long m0 = (long long)b.pair * 256 + t * kPreM, m1 = min(rows_m, m0 + kPreM) - 1;
-    r.pmin = b.len - b.n + int(m0 / G);
-    r.pmax = m0 < rows_m ? b.len - b.n + int(m1 / G) : -1;
+    const int m0 = t * kPreM, m1 = min(b.rows, m0 + kPreM) - 1, base = b.len - b.n + b.q0;
+    r.pmin = base + (b.r0 + m0) / G;
+    r.pmax = m0 < b.rows ? base + (b.r0 + m1) / G : -1;
     // As key tiles of the row: the sinks' before `sunk`, the window's [first, last].
     const int last = r.pmax >> 6, first = p.window ? max(r.pmin - p.window + 1, 0) >> 6 : 0;
     const int sunk = p.window ? min((p.sinks + kPreN - 1) / kPreN, last + 1) : 0;
@@ -329,9 +321,8 @@ __global__ void __launch_bounds__(kPreThreads, 1)
 
   // ---- Q: M row t of tile A or B into its swizzled slices -----------------------------------
   const int wg = warp >> 2, t = tid & 127;
-  const long long m = (long long)b.pair * 256 + wg * kPreM + t;
-  const bool mine = warp < 8 && m < rows_m;
-  const int qi = mine ? int(m / G) : 0, head = kvh * G + (mine ? int(m % G) : 0);
+  const bool mine = warp < 8 && tid < b.rows;
+  const int qi = mine ? b.q0 + (b.r0 + tid) / G : 0, head = kvh * G + (mine ? (b.r0 + tid) % G : 0);
   const bf16 *q_row = p.q + size_t(b.first + qi) * p.q_stride + size_t(head) * D;
   // A warp moves its 32 rows row by row (D / 8 lanes each): whole lines of global memory.
   constexpr int CPR = D / 8;
@@ -343,16 +334,30 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       const bf16 *src = reinterpret_cast<const bf16 *>(__shfl_sync(0xFFFFFFFFu, (unsigned long long)q_row, r));
       v[i] = __shfl_sync(0xFFFFFFFFu, int(mine), r) ? *reinterpret_cast<const uint4 *>(src + c * 8) : make_uint4(0, 0, 0, 0);
     }
+    // Bad pages among the keys to come (their pieces are then masked one by one).
+    for (int i = tid; i < nt * pieces; i += 256) {
+      const int k0 = key_tile(b.j0 + i / pieces) + (i % pieces) * x.box_rows;
+      if (needed(k0, k0 + x.box_rows)) {
+        const int page = tab[k0 >> p.page_shift];
+        if (page < 0 || page >= p.pages) {
+          s_bad = 1;
+          if (p.error) atomicOr(p.error, kKvBadPage);
+        }
+      }
+    }
 #pragma unroll
     for (int i = 0; i < CPR; ++i) {
       const int r = (warp & 3) * 32 + (i * 32 + lane) / CPR, c = lane % CPR;
       *reinterpret_cast<uint4 *>(sm + wg * Cfg::kQ + (c >> 3) * Cfg::kQSlice + at_sw(r, c & 7)) = v[i];
     }
   }
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  __syncthreads();
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  // Q and the tensor memory are ready for warps 0..9; the copies do not wait for them.
+  if (warp < 10) {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    asm volatile("bar.sync 3, 320;" ::: "memory");
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  }
   const uint32_t tmem = tmem_slot;
   auto stage = [&](int it) { return ring + (it % NST) * 2 * Cfg::kTile; };  // (V of tile i: it = i + 1)
 
