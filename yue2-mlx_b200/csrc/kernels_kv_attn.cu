@@ -11,10 +11,11 @@ namespace yar {
 //
 // A query row of a KV head's group reads each cached K and V value once for the whole
 // group, so the kernel is bound by HBM: 2 x 2 x D bytes per position and KV head. The work
-// of one (row, kv head) is split over a thread-block cluster of C blocks (C a power of two
-// up to 16: one row of eight heads then still fills 128 SMs), the parts joined through
-// distributed shared memory: no partials in global memory, no counters, nothing to clear
-// between calls.
+// of one (row, kv head) is split over a thread-block cluster of C blocks (a power of two up
+// to 16), the parts joined through distributed shared memory: no partials in global memory,
+// no counters, nothing to clear between calls. Large clusters leave SMs unused (of 16 blocks
+// with an SM each, 7 run at once), so a few long rows are split into as many parts as there
+// are SMs instead, given a workspace, and joined by a second kernel.
 //
 // Each of a block's warps takes 16 positions at a time (a slice) through its own ring
 // of cp.async copies (16 bytes a lane, any page size; rows that are not visible or whose
@@ -25,8 +26,12 @@ namespace yar {
 //   m = max(m, S), P = 2^(S scale log2(e) - m), l += P in FP32;
 //   O^T [D x 8] += V^T P, with P as two BF16 parts (P keeps 16 bits, so the result's error
 //   is its own rounding): P's fragment is transposed in registers (movmatrix).
-// The tensor work per slice is 8 KB of shared memory read once: about a third of the time in
-// which HBM delivers the slice's 8 KB to an SM.
+// The tensor and issue work per slice is well below the time in which HBM delivers its 8 KB to
+// an SM (issue slots 40 % busy at 6.2 TB/s), which is why the plain mma.sync form suffices.
+// Measured: 64 rows with 2,052 visible positions 81 us (524 MB, the rate of a plain copy); one
+// row of 24,000 positions 23 us with a workspace, 28 without (98 MB, 15 us at that rate: the
+// start of the launch, the table's round trip and the join are the rest); one row of 513
+// positions 6 us, of 64 3.5 us; 33 rows of 14 heads of 64 on pages of 16, 9.7 us.
 namespace {
 constexpr int kDecSlice = 16, kDecMaxCluster = 16;
 

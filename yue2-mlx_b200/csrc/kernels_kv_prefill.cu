@@ -24,6 +24,17 @@
 //
 // Few blocks (a chunk of one prompt) are split along the keys over a cluster of 2 or 4, whose
 // states are joined through distributed shared memory, each block finishing D / C columns.
+//
+// What bounds it: per 64-key step of A and B (~1,770 cycles) the tensor pipe has ~1,150 cycles
+// of work (S at N = 64 reads Q again for every 64 keys: 53 cycles a product instead of 32), and
+// a softmax group ~1,250, most of them exponentials; the rest is the hand-over between them.
+// Measured (16 query / 8 KV heads of 128): 16,384 tokens with a window of 2,048: 302 us, 854
+// TFLOP/s; 1,024 queries over 8,192 positions: 78 us, 821 TFLOP/s (145 us without the split);
+// 24 ragged rows: 148 us; 77 queries of 4 heads of 64: 10 us. Tried and slower: 128-key tiles
+// with one S buffer each (1.9 times the time, issue-bound), S and P V issued by warps of
+// their own (84 us on the second case), A's and B's exponentials taking turns (151), the
+// exponentials of a tile run beside the next one's maximum (182: S would have to be three
+// tiles ahead), no maximum but for tiles that leave the range (146 against 139).
 #include <cuda.h>
 
 #include <algorithm>
@@ -61,7 +72,9 @@ struct PreCfg {
 // Tensor memory: two S (and P) buffers of A at columns 0 and 64, of B at 128 and 192, O at 256, 384.
 constexpr uint32_t kPreColO = 256, kPreCols = 512;
 constexpr float kPreRescale = 8.f;
-constexpr int kPrePoly = 3;  // of 8 pairs of exponentials, those on the FMA units
+// Of 8 pairs of exponentials, those on the FMA units (1,024 at 7,168 unsplit: 145 us with 0, 143
+// with 1, 139 with 2, 3 and 4).
+constexpr int kPrePoly = 3;
 
 struct PrefillExtra {
   int row0;        // the layer's first cached row in the pool seen as [rows][D]
