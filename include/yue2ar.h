@@ -332,33 +332,43 @@ typedef struct yar_kv_rows {
   int32_t rows, pages_per_row;
 } yar_kv_rows;
 
-/* Attention of one new token per row over its cached positions: for row r and each head,
- * out = softmax(scale * q . k_j) v_j over the visible j. The query is the row's last cached
- * position; j < lengths[r] is visible when window is 0, or j < sinks, or
- * j >= lengths[r] - window (the last `window` positions, itself included, and the first
- * `sinks`). A row that sees nothing gets zeros. q and out: BF16 [rows][heads][head_dim],
- * row strides in elements (multiples of 8), not overlapping; heads: a multiple of kv_heads,
- * at most 16 for each. FP32 scores, statistics and sums; one rounding of the result.
- * max_length (0: the table's end): a bound of the lengths; it only chooses into how many
- * parts a row's positions are split, longer rows stay right. workspace (device memory, any
- * contents; NULL and 0: none) lets a few long rows be split over the whole GPU; with fewer
- * bytes than yar_kv_attn_decode_workspace says it is not used. Calls that may overlap (other
- * streams, graphs replayed at the same time) need a workspace each. */
-int yar_kv_attn_decode(const yar_kv_pool *pool, int layer, const yar_kv_rows *rows, const void *q, int64_t q_stride,
-                       int heads, void *out, int64_t out_stride, int window, int sinks, double scale, int max_length,
-                       void *workspace, int64_t workspace_bytes, int32_t *error, void *stream);
+/* What both forms of attention take. q and out: BF16, one row [heads][head_dim] per query, row
+ * strides in elements (multiples of 8), 16-byte aligned, not overlapping; heads: a multiple
+ * of kv_heads, at most 16 for each (query head h reads KV head h / (heads / kv_heads)). The
+ * query at position p sees j <= p when window is 0, else j < sinks or j > p - window (the
+ * last `window` positions, its own included, and the first `sinks`). FP32 scores, statistics
+ * and sums; the result is rounded once; a query that sees nothing gets zeros. */
+typedef struct yar_kv_attn {
+  yar_kv_pool pool;
+  yar_kv_rows rows;
+  int32_t layer, heads;
+  const void *q;
+  int64_t q_stride;
+  void *out;
+  int64_t out_stride;
+  int32_t window, sinks;
+  double scale;
+  int32_t *error;
+} yar_kv_attn;
+
+/* Attention of one new token per row over its cached positions: q and out [rows], the query of
+ * row r at position lengths[r] - 1. max_length (0: the table's end): a bound of the lengths;
+ * it only chooses into how many parts a row's positions are split, longer rows stay right.
+ * workspace (device memory, any contents; NULL and 0: none) lets a few long rows be split
+ * over the whole GPU; with fewer bytes than yar_kv_attn_decode_workspace says it is not used.
+ * Calls that may overlap (other streams, graphs replayed at the same time) need a workspace
+ * each. */
+int yar_kv_attn_decode(const yar_kv_attn *call, int max_length, void *workspace, int64_t workspace_bytes,
+                       void *stream);
 /* The bytes of workspace that yar_kv_attn_decode can use for these heads. */
 int yar_kv_attn_decode_workspace(int heads, int kv_heads, int head_dim, int64_t *bytes);
 
 /* The same for prompts: row r's queries are q[offsets[r]] .. q[offsets[r + 1] - 1] (int32
  * [rows + 1], ascending, at most n_queries), the last n of its lengths[r] cached positions
- * (their keys and values are in the cache already); the query at position p sees j <= p when
- * window is 0, or j < sinks, or j > p - window. A query before position 0 (more queries than
- * lengths[r]) sees nothing and gets zeros. q and out: [n_queries][heads][head_dim]; out rows
- * in front of offsets[0] or behind offsets[rows] are left as they were. */
-int yar_kv_attn_prefill(const yar_kv_pool *pool, int layer, const yar_kv_rows *rows, const int32_t *offsets,
-                        int64_t n_queries, const void *q, int64_t q_stride, int heads, void *out, int64_t out_stride,
-                        int window, int sinks, double scale, int32_t *error, void *stream);
+ * (their keys and values are in the cache already). A query before position 0 (more queries
+ * than lengths[r]) sees nothing. q and out: [n_queries]; out rows in front of offsets[0] or
+ * behind offsets[rows] are left as they were. */
+int yar_kv_attn_prefill(const yar_kv_attn *call, const int32_t *offsets, int64_t n_queries, void *stream);
 
 /* Copy page src_pages[i] of `src` to page dst_pages[i] of `dst`, i < n, in every layer: the
  * first tokens[i] positions of K and V (tokens NULL: the whole page). The pools are one, or

@@ -451,11 +451,25 @@ def test_calls_from_two_threads(yar, torch):
 def test_host_memory_is_refused(yar, torch):
     c = Cache(torch, [20], 2, 64, 16, seed=1)
     q, _ = queries(torch, 1, 4, 64, 1)
+    ok = (c.pool, 1, c.table, c.lengths, q)
+    for i, bad in ((4, q.cpu()), (4, q.float()), (4, q[0]), (4, q[..., :32]), (4, q.transpose(1, 2)), (0, c.pool[0]),
+                   (0, c.pool.cpu()), (0, c.pool.transpose(0, 1)), (2, c.table.long()), (2, c.table[0]), (2, c.table.cpu()),
+                   (3, c.lengths[:0]), (3, c.lengths.long()), (3, c.lengths.cpu()), (4, torch.cat([q, q]))):
+        with pytest.raises(ValueError):
+            yar.kv_attn_decode(*ok[:i], bad, *ok[i + 1:])
+    for out in (q.float(), q.cpu(), torch.cat([q, q]), q.transpose(1, 2)):
+        with pytest.raises(ValueError):
+            yar.kv_attn_decode(*ok, out=out)
+        with pytest.raises(ValueError):
+            yar.kv_attn_prefill(*ok[:4], torch.tensor([0, 1], dtype=torch.int32).cuda(), q, out=out)
     with pytest.raises(ValueError):
-        yar.kv_attn_decode(c.pool, 1, c.table, c.lengths, q.cpu())
+        yar.kv_attn_prefill(*ok[:4], torch.tensor([0], dtype=torch.int32).cuda(), q)
+    with pytest.raises(ValueError):
+        yar.kv_attn_decode(*ok, error=torch.zeros(1, device="cuda"))
     host = torch.zeros(1, 4, 64, dtype=torch.bfloat16)
-    st = yar.lib.yar_kv_attn_decode(yar._kv_pool(c.pool), 1, yar._kv_rows(c.table, c.lengths), host.data_ptr(), 256, 4,
-                                    q.data_ptr(), 256, 0, 0, 0.125, 0, None, 0, None, None)
+    call = yar._KvAttn(yar._kv_pool(c.pool), yar._kv_rows(c.table, c.lengths), 0, 4, host.data_ptr(), 256, q.data_ptr(),
+                       256, 0, 0, 0.125, None)
+    st = yar.lib.yar_kv_attn_decode(bytes(call), 0, None, 0, None)
     assert st == yar.INVALID_INPUT and b"device memory" in yar.lib.yar_last_error()
 
 

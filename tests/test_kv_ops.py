@@ -54,16 +54,28 @@ ROWS = [
 ]
 
 
+def record(yar, p, r, layer, heads, q, q_stride, out, out_stride, window, sinks, scale, error):
+    return ctypes.byref(yar._KvAttn(p or pool(yar), r or rows(yar), layer, heads, q, q_stride, out, out_stride, window,
+                                    sinks, scale, error))
+
+
 def decode(yar, p=None, r=None, layer=0, q=PTR, q_stride=256, heads=4, out=PTR, out_stride=256, window=0, sinks=0,
            scale=0.125, max_length=0, workspace=None, workspace_bytes=0, error=None):
-    return yar.lib.yar_kv_attn_decode(p or pool(yar), layer, r or rows(yar), q, q_stride, heads, out, out_stride,
-                                      window, sinks, scale, max_length, workspace, workspace_bytes, error, None)
+    return yar.lib.yar_kv_attn_decode(record(yar, p, r, layer, heads, q, q_stride, out, out_stride, window, sinks,
+                                             scale, error), max_length, workspace, workspace_bytes, None)
 
 
 def prefill(yar, p=None, r=None, layer=0, offsets=PTR, n=5, q=PTR, q_stride=256, heads=4, out=PTR, out_stride=256,
             window=0, sinks=0, scale=0.125, error=None):
-    return yar.lib.yar_kv_attn_prefill(p or pool(yar), layer, r or rows(yar), offsets, n, q, q_stride, heads, out,
-                                       out_stride, window, sinks, scale, error, None)
+    return yar.lib.yar_kv_attn_prefill(record(yar, p, r, layer, heads, q, q_stride, out, out_stride, window, sinks,
+                                              scale, error), offsets, n, None)
+
+
+def test_the_packed_record_is_the_structure(yar):
+    v = list(range(1, 20))
+    s = yar._KvAttn(yar._KvPool(*v[:6]), yar._KvRows(*v[6:11]), *v[11:18], 0, 0.5, 77)
+    s.window, s.sinks = 18, 19
+    assert bytes(s) == yar._kv_attn_bytes(*v[:17], 18, 19, 0.5, 77)
 
 
 @pytest.mark.parametrize("call", [decode, prefill])
@@ -86,8 +98,8 @@ def test_decode_and_prefill_own_arguments(yar):
     refused(yar, prefill(yar, n=1 << 31), "n_queries")
     refused(yar, prefill(yar, offsets=None), "offsets")
     assert prefill(yar, n=0, q=None, out=None, offsets=None) == yar.OK
-    refused(yar, yar.lib.yar_kv_attn_decode(None, 0, rows(yar), PTR, 256, 4, PTR, 256, 0, 0, .1, 0, None, 0, None, None), "pool")
-    refused(yar, yar.lib.yar_kv_attn_decode(pool(yar), 0, None, PTR, 256, 4, PTR, 256, 0, 0, .1, 0, None, 0, None, None), "rows")
+    refused(yar, yar.lib.yar_kv_attn_decode(None, 0, None, 0, None), "record")
+    refused(yar, yar.lib.yar_kv_attn_prefill(None, PTR, 5, None), "record")
 
 
 def copy(yar, src, dst, tokens=None, a=None, b=None):

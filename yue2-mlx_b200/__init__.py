@@ -20,6 +20,7 @@ from __future__ import annotations
 import ctypes
 import json
 import os
+import struct
 import sys
 from dataclasses import dataclass
 
@@ -61,6 +62,17 @@ class _KvPool(ctypes.Structure):
 class _KvRows(ctypes.Structure):
     _fields_ = [("page_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("lengths", ctypes.c_void_p),
                 ("rows", ctypes.c_int32), ("pages_per_row", ctypes.c_int32)]
+
+
+class _KvAttn(ctypes.Structure):
+    _fields_ = [("pool", _KvPool), ("rows", _KvRows), ("layer", ctypes.c_int32), ("heads", ctypes.c_int32),
+                ("q", ctypes.c_void_p), ("q_stride", ctypes.c_int64), ("out", ctypes.c_void_p),
+                ("out_stride", ctypes.c_int64), ("window", ctypes.c_int32), ("sinks", ctypes.c_int32),
+                ("scale", ctypes.c_double), ("error", ctypes.c_void_p)]
+
+
+# _KvAttn's fields in order, as bytes: one step instead of nineteen assignments per call.
+_kv_attn_bytes = struct.Struct("P5iPqPiiiiPqPqiidP").pack
 
 
 CANCEL_FN = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p)
@@ -120,12 +132,10 @@ def _load_library(path: str = LIB_PATH) -> ctypes.CDLL:
                                 ctypes.POINTER(ctypes.c_float)]),
         "yar_sample_device_noalloc": (I, [P, P, ctypes.c_int64, I, I, D, ctypes.POINTER(_Sampling), i32p, I, I, I,
                                           U64, P, P, P]),
-        "yar_kv_attn_decode": (I, [ctypes.POINTER(_KvPool), I, ctypes.POINTER(_KvRows), P, ctypes.c_int64, I, P,
-                                   ctypes.c_int64, I, I, D, I, P, ctypes.c_int64, P, P]),
+        "yar_kv_attn_decode": (I, [P, I, P, ctypes.c_int64, P]),
         "yar_kv_attn_decode_workspace": (I, [I, I, I, ctypes.POINTER(ctypes.c_int64)]),
-        "yar_kv_attn_prefill": (I, [ctypes.POINTER(_KvPool), I, ctypes.POINTER(_KvRows), P, ctypes.c_int64, P,
-                                    ctypes.c_int64, I, P, ctypes.c_int64, I, I, D, P, P]),
-        "yar_kv_copy_pages": (I, [ctypes.POINTER(_KvPool), ctypes.POINTER(_KvPool), i32p, i32p, i32p, I, P]),
+        "yar_kv_attn_prefill": (I, [P, P, ctypes.c_int64, P]),
+        "yar_kv_copy_pages": (I, [ctypes.POINTER(_KvPool), ctypes.POINTER(_KvPool), P, P, P, I, P]),
         "yar_kv_compact": (I, [ctypes.POINTER(_KvPool), P, ctypes.c_int64, I, I, P, P, ctypes.c_int64, P, P, P, P, P]),
     }
     for name, (res, args) in sig.items():
@@ -549,6 +559,36 @@ def _kv_heads(t, name: str, dim: int) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1] * dim
 
 
+def _kv_attn(pool, layer, page_table, lengths, q, out, window, sinks, scale, error):
+    """(the yar_kv_attn record, out) of a call. The checks on contiguous tensors go first and in
+    one expression (a small call is as long as its host side); others are looked at one by one."""
+    torch = sys.modules["torch"]
+    ps, qs, ts = pool.shape, q.shape, page_table.shape
+    if out is None and pool.dtype is torch.bfloat16 is q.dtype and page_table.dtype is torch.int32 is lengths.dtype \
+            and len(ps) == 6 and ps[2] == 2 and len(qs) == 3 and qs[2] == ps[5] and len(ts) == 2 \
+            and lengths.dim() == 1 and lengths.shape[0] >= ts[0] \
+            and pool.is_contiguous() and q.is_contiguous() and page_table.is_contiguous() and lengths.is_contiguous() \
+            and pool.is_cuda and q.is_cuda and page_table.is_cuda and lengths.is_cuda:
+        out = torch.empty_like(q)
+        q_stride = out_stride = qs[1] * qs[2]
+        table_stride = ts[1]
+    else:
+        _kv_pool(pool)
+        table_stride = _kv_rows(page_table, lengths).table_stride
+        q_stride = _kv_heads(q, "q", ps[5])
+        out = q.new_empty(qs) if out is None else out
+        out_stride = _kv_heads(out, "out", ps[5])
+        if out.shape != qs:
+            raise ValueError("out must have q's shape")
+    try:
+        return _kv_attn_bytes(pool.data_ptr(), ps[0], ps[1], ps[3], ps[4], ps[5], page_table.data_ptr(), table_stride,
+                              lengths.data_ptr(), ts[0], ts[1], layer, qs[1], q.data_ptr(), q_stride, out.data_ptr(),
+                              out_stride, window, sinks, ps[5] ** -0.5 if scale is None else scale,
+                              0 if error is None else _kv_error(error)), out
+    except struct.error as e:
+        raise ValueError(f"layer, window, sinks or scale: {e}") from None
+
+
 def _kv_stream(t, stream):
     if stream is not None:
         return stream
@@ -573,20 +613,19 @@ def kv_attn_decode(pool, layer: int, page_table, lengths, q, out=None, window: i
     ``window``/``sinks``: only the last ``window`` positions and the first ``sinks`` are visible
     (0: all). ``scale`` defaults to dim ** -0.5, ``stream`` to torch's current one, ``workspace``
     (any tensor of ``kv_attn_decode_workspace`` bytes) to fresh memory where rows are long."""
-    c_pool, rows = _kv_pool(pool), _kv_rows(page_table, lengths)
-    out = q.new_empty(q.shape) if out is None else out
-    dim = c_pool.head_dim
-    if q.shape[0] != rows.rows or out.shape != q.shape:
+    call, out = _kv_attn(pool, layer, page_table, lengths, q, out, window, sinks, scale, error)
+    rows, per_row = page_table.shape
+    if q.shape[0] != rows:
         raise ValueError("q and out need one row for each row of page_table")
-    qs, os_ = _kv_heads(q, "q", dim), _kv_heads(out, "out", dim)
-    heads = q.shape[1]
-    if workspace is None and stream is None and (max_length or rows.pages_per_row * c_pool.page_tokens) > 4096 and \
-            not 0 < window < 4096 and rows.rows * c_pool.kv_heads <= 74:
-        workspace = q.new_empty((kv_attn_decode_workspace(heads, c_pool.kv_heads, dim) // 2,))
-    w, wb = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
-    _check(lib.yar_kv_attn_decode(c_pool, layer, rows, q.data_ptr(), qs, heads, out.data_ptr(), os_, window,
-                                  sinks, dim ** -0.5 if scale is None else scale, max_length, w, wb,
-                                  _kv_error(error), _kv_stream(q, stream)))
+    w, wb = None, 0
+    if workspace is not None:
+        w, wb = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    elif stream is None and rows * pool.shape[3] <= 74 and (max_length or per_row * pool.shape[4]) > 4096 and \
+            not 0 < window < 4096:
+        wb = kv_attn_decode_workspace(q.shape[1], pool.shape[3], q.shape[2])
+        workspace = q.new_empty((wb // 2,))
+        w = workspace.data_ptr()
+    _check(lib.yar_kv_attn_decode(call, max_length, w, wb, _kv_stream(q, stream)))
     return out
 
 
@@ -596,15 +635,9 @@ def kv_attn_prefill(pool, layer: int, page_table, lengths, offsets, q, out=None,
     lengths[r] cached positions) over its paged cache (yar_kv_attn_prefill); the other
     arguments as ``kv_attn_decode``'s. A result allocated here is undefined outside the rows'
     queries."""
-    c_pool, rows = _kv_pool(pool), _kv_rows(page_table, lengths)
-    out = q.new_empty(q.shape) if out is None else out
-    dim = c_pool.head_dim
-    if out.shape != q.shape:
-        raise ValueError("out must have q's shape")
-    qs, os_ = _kv_heads(q, "q", dim), _kv_heads(out, "out", dim)
-    _check(lib.yar_kv_attn_prefill(c_pool, layer, rows, _kv_int32(offsets, "offsets", rows.rows + 1), q.shape[0],
-                                   q.data_ptr(), qs, q.shape[1], out.data_ptr(), os_, window, sinks,
-                                   dim ** -0.5 if scale is None else scale, _kv_error(error), _kv_stream(q, stream)))
+    call, out = _kv_attn(pool, layer, page_table, lengths, q, out, window, sinks, scale, error)
+    _check(lib.yar_kv_attn_prefill(call, _kv_int32(offsets, "offsets", page_table.shape[0] + 1), q.shape[0],
+                                   _kv_stream(q, stream)))
     return out
 
 
@@ -615,24 +648,28 @@ def kv_copy_pages(pool, src, dst, tokens=None, dst_pool=None, stream=None):
     t = None if tokens is None else _i32(tokens)
     if a.ndim != 1 or a.shape != b.shape or (t is not None and t.shape != a.shape):
         raise ValueError("src, dst and tokens must be lists of one length")
-    _check(lib.yar_kv_copy_pages(_kv_pool(pool), _kv_pool(pool if dst_pool is None else dst_pool),
-                                 _ptr(a, ctypes.c_int32), _ptr(b, ctypes.c_int32),
-                                 None if t is None else _ptr(t, ctypes.c_int32), a.size, _kv_stream(pool, stream)))
+    c_pool = _kv_pool(pool)
+    _check(lib.yar_kv_copy_pages(c_pool, c_pool if dst_pool is None else _kv_pool(dst_pool), a.tobytes(), b.tobytes(),
+                                 None if t is None else t.tobytes(), a.size, _kv_stream(pool, stream)))
 
 
 def kv_compact(pool, page_table, counts, out=None, error=None, stream=None):
     """Move the used pages to the front of the pool (yar_kv_compact). Returns (the renamed
     table, remap [pages]: each page's new index or -1, used [1]); ``out`` may be ``page_table``."""
     c_pool, rows = _kv_pool(pool), _kv_rows(page_table, counts)
-    out = page_table.new_empty(page_table.shape) if out is None else out
-    if out.shape != page_table.shape:
-        raise ValueError("out must have page_table's shape")
-    new = _kv_rows(out, counts)
+    if out is None:
+        out = page_table.new_empty(page_table.shape)
+        new, new_stride = out.data_ptr(), rows.pages_per_row
+    else:
+        if out.shape != page_table.shape:
+            raise ValueError("out must have page_table's shape")
+        r = _kv_rows(out, counts)
+        new, new_stride = r.page_table, r.table_stride
     n = c_pool.pages
     buf = page_table.new_empty((3 * n + 2,))  # remap [n], used [1], scratch [1 + 2 n]
     at = buf.data_ptr()
     _check(lib.yar_kv_compact(c_pool, rows.page_table, rows.table_stride, rows.rows, rows.pages_per_row, rows.lengths,
-                              new.page_table, new.table_stride, at, at + 4 * n, at + 4 * n + 4, _kv_error(error),
+                              new, new_stride, at, at + 4 * n, at + 4 * n + 4, _kv_error(error),
                               _kv_stream(pool, stream)))
     return out, buf[:n], buf[n:n + 1]
 

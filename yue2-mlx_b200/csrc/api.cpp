@@ -35,13 +35,10 @@ void sample_device_noalloc(Model &m, const uint16_t *logits, long long row_strid
                            double cfg_scale, const ::yar_sampling &smp, const int32_t *history, int n_history,
                            int step, int phase, uint64_t seed, int32_t *token, float *scores,
                            cudaStream_t st);
-void kv_attn_decode(const ::yar_kv_pool *pool, int layer, const ::yar_kv_rows *rows, const void *q, int64_t q_stride,
-                    int heads, void *out, int64_t out_stride, int window, int sinks, double scale, int max_length,
-                    void *workspace, int64_t workspace_bytes, int32_t *error, cudaStream_t st);
+void kv_attn_decode(const ::yar_kv_attn *call, int max_length, void *workspace, int64_t workspace_bytes,
+                    cudaStream_t st);
 size_t kv_attn_decode_workspace(int heads, int kv_heads, int head_dim);
-void kv_attn_prefill(const ::yar_kv_pool *pool, int layer, const ::yar_kv_rows *rows, const int32_t *offsets,
-                     int64_t n_queries, const void *q, int64_t q_stride, int heads, void *out, int64_t out_stride,
-                     int window, int sinks, double scale, int32_t *error, cudaStream_t st);
+void kv_attn_prefill(const ::yar_kv_attn *call, const int32_t *offsets, int64_t n_queries, cudaStream_t st);
 void kv_copy_pages(const ::yar_kv_pool *from, const ::yar_kv_pool *to, const int32_t *src, const int32_t *dst,
                    const int32_t *tokens, int n, cudaStream_t st);
 void kv_compact(const ::yar_kv_pool *pool, const int32_t *table, int64_t table_stride, int rows, int pages_per_row,
@@ -516,12 +513,10 @@ int yar_sample_device_noalloc(yar_model *model, const uint16_t *logits, int64_t 
   });
 }
 
-int yar_kv_attn_decode(const yar_kv_pool *pool, int layer, const yar_kv_rows *rows, const void *q, int64_t q_stride,
-                       int heads, void *out, int64_t out_stride, int window, int sinks, double scale, int max_length,
-                       void *workspace, int64_t workspace_bytes, int32_t *error, void *stream) {
+int yar_kv_attn_decode(const yar_kv_attn *call, int max_length, void *workspace, int64_t workspace_bytes,
+                       void *stream) {
   return guarded([&] {
-    yar::kv_attn_decode(pool, layer, rows, q, q_stride, heads, out, out_stride, window, sinks, scale, max_length,
-                        workspace, workspace_bytes, error, static_cast<cudaStream_t>(stream));
+    yar::kv_attn_decode(call, max_length, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
   });
 }
 
@@ -534,13 +529,8 @@ int yar_kv_attn_decode_workspace(int heads, int kv_heads, int head_dim, int64_t 
   });
 }
 
-int yar_kv_attn_prefill(const yar_kv_pool *pool, int layer, const yar_kv_rows *rows, const int32_t *offsets,
-                        int64_t n_queries, const void *q, int64_t q_stride, int heads, void *out, int64_t out_stride,
-                        int window, int sinks, double scale, int32_t *error, void *stream) {
-  return guarded([&] {
-    yar::kv_attn_prefill(pool, layer, rows, offsets, n_queries, q, q_stride, heads, out, out_stride, window, sinks,
-                         scale, error, static_cast<cudaStream_t>(stream));
-  });
+int yar_kv_attn_prefill(const yar_kv_attn *call, const int32_t *offsets, int64_t n_queries, void *stream) {
+  return guarded([&] { yar::kv_attn_prefill(call, offsets, n_queries, static_cast<cudaStream_t>(stream)); });
 }
 
 int yar_kv_copy_pages(const yar_kv_pool *src, const yar_kv_pool *dst, const int32_t *src_pages,

@@ -91,10 +91,14 @@ void configure_device(int device) {
   done[size_t(device)] = 1;
 }
 
-KvAttnParams attn_params(const KvPool &pool, int layer, const ::yar_kv_rows *rows, const void *q, int64_t q_stride,
-                         int heads, void *out, int64_t out_stride, int window, int sinks, double scale,
-                         int32_t *error) {
-  need(rows, "rows is required");
+KvAttnParams attn_params(const KvPool &pool, const ::yar_kv_attn &c) {
+  const ::yar_kv_rows *rows = &c.rows;
+  const int layer = c.layer, heads = c.heads, window = c.window, sinks = c.sinks;
+  const int64_t q_stride = c.q_stride, out_stride = c.out_stride;
+  const void *q = c.q;
+  void *out = c.out;
+  const double scale = c.scale;
+  int32_t *error = c.error;
   need(layer >= 0 && layer < pool.layers, "layer outside the pool");
   check_table(pool, rows->page_table, rows->table_stride, rows->rows, rows->pages_per_row);
   need(rows->rows == 0 || (rows->lengths && aligned(rows->lengths, 4)), "lengths is required");
@@ -132,41 +136,40 @@ KvAttnParams attn_params(const KvPool &pool, int layer, const ::yar_kv_rows *row
 }
 }  // namespace
 
-void kv_attn_decode(const ::yar_kv_pool *c_pool, int layer, const ::yar_kv_rows *rows, const void *q, int64_t q_stride,
-                    int heads, void *out, int64_t out_stride, int window, int sinks, double scale, int max_length,
-                    void *workspace, int64_t workspace_bytes, int32_t *error, cudaStream_t st) {
-  const KvPool pool = checked_pool(c_pool);
-  KvAttnParams p = attn_params(pool, layer, rows, q, q_stride, heads, out, out_stride, window, sinks, scale, error);
+void kv_attn_decode(const ::yar_kv_attn *call, int max_length, void *workspace, int64_t workspace_bytes,
+                    cudaStream_t st) {
+  need(call, "the call's record is required");
+  const KvPool pool = checked_pool(&call->pool);
+  KvAttnParams p = attn_params(pool, *call);
   need(max_length >= 0, "max_length must not be negative");
   need(workspace_bytes >= 0 && (workspace || workspace_bytes == 0) && aligned(workspace, 4),
        "workspace must be a 4-byte aligned buffer of workspace_bytes (or NULL and 0)");
   p.max_length = max_length;
-  if (workspace && size_t(workspace_bytes) >= kv_attn_decode_workspace(heads, pool.kv_heads, pool.head_dim))
+  if (workspace && size_t(workspace_bytes) >= kv_attn_decode_workspace(p.heads, pool.kv_heads, pool.head_dim))
     p.partials = static_cast<float *>(workspace);
   if (p.rows == 0) return;
-  need(q && out, "q and out are required");
-  const int device = device_of({{"the pool", pool.data}, {"the page table", p.table}, {"lengths", p.lengths}, {"q", q},
-                                {"out", out}, {"workspace", workspace}, {"error", error}});
+  need(p.q && p.out, "q and out are required");
+  const int device = device_of({{"the pool", pool.data}, {"the page table", p.table}, {"lengths", p.lengths}, {"q", p.q},
+                                {"out", p.out}, {"workspace", workspace}, {"error", p.error}});
   DeviceGuard guard(device);
   configure_device(device);
   launch_kv_attn_decode(p, pool.head_dim, st);
 }
 
-void kv_attn_prefill(const ::yar_kv_pool *c_pool, int layer, const ::yar_kv_rows *rows, const int32_t *offsets,
-                     int64_t n_queries, const void *q, int64_t q_stride, int heads, void *out, int64_t out_stride,
-                     int window, int sinks, double scale, int32_t *error, cudaStream_t st) {
-  const KvPool pool = checked_pool(c_pool);
-  KvAttnParams p = attn_params(pool, layer, rows, q, q_stride, heads, out, out_stride, window, sinks, scale, error);
+void kv_attn_prefill(const ::yar_kv_attn *call, const int32_t *offsets, int64_t n_queries, cudaStream_t st) {
+  need(call, "the call's record is required");
+  const KvPool pool = checked_pool(&call->pool);
+  KvAttnParams p = attn_params(pool, *call);
   need(n_queries >= 0 && n_queries <= kKvMaxPositions, "n_queries must be in [0, 2**30]");
   if (p.rows == 0 || n_queries == 0) return;
-  need(q && out && offsets && aligned(offsets, 4), "q, out and offsets are required");
+  need(p.q && p.out && offsets && aligned(offsets, 4), "q, out and offsets are required");
   p.offsets = offsets;
   p.n_queries = int(n_queries);
   const int device = device_of({{"the pool", pool.data}, {"the page table", p.table}, {"lengths", p.lengths},
-                                {"offsets", offsets}, {"q", q}, {"out", out}, {"error", error}});
+                                {"offsets", offsets}, {"q", p.q}, {"out", p.out}, {"error", p.error}});
   DeviceGuard guard(device);
   configure_device(device);
-  launch_kv_attn_prefill(pool, layer, p, st);
+  launch_kv_attn_prefill(pool, call->layer, p, st);
 }
 
 void kv_copy_pages(const ::yar_kv_pool *c_from, const ::yar_kv_pool *c_to, const int32_t *src, const int32_t *dst,
