@@ -187,6 +187,80 @@ def test_prefill_matches_the_definition(yar, torch, ns, before, kv, group, dim, 
     assert err.item() == 0
 
 
+MANY = [
+    # more pieces of work than a GPU has SMs: blocks take several in turn
+    ([1 + 7 * i % 61 for i in range(45)], [13 * i % 300 for i in range(45)], 8, 2, 64, 16, 0, 0),
+    ([1 + 7 * i % 61 for i in range(45)], [13 * i % 300 for i in range(45)], 8, 3, 64, 32, 37, 3),
+    ([i * 5 % 4 for i in range(150)] + [700, 0, 3], [i * 11 % 90 for i in range(153)], 2, 4, 128, 32, 40, 5),
+    ([4000], [100], 8, 2, 64, 64, 200, 70), ([900, 60], [0, 500], 8, 7, 128, 256, 0, 0),
+    ([2 + 31 * i % 400 for i in range(20)], [0] * 20, 8, 16, 64, 16, 90, 20),
+]
+
+
+@pytest.mark.parametrize("ns,before,kv,group,dim,page,window,sinks", MANY)
+def test_many_rows_and_long_prompts(yar, torch, ns, before, kv, group, dim, page, window, sinks):
+    """First, middle and last query of every row against the definition; the same bits again; and a
+    bad page or a value that is not finite in one row leaves the other rows' bits alone."""
+    lens = [n + b for n, b in zip(ns, before)]
+    c = Cache(torch, lens, kv, dim, page, seed=len(lens), window=window, sinks=sinks, first_pos=before)
+    offs = np.concatenate([[0], np.cumsum(ns)])
+    q, q64 = queries(torch, int(offs[-1]), kv * group, dim, lens[0])
+    d_offs = torch.tensor(offs, dtype=torch.int32, device="cuda")
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+
+    def run(pool, table):
+        err.zero_()
+        return yar.kv_attn_prefill(pool, 1, table, c.lengths, d_offs, q, window=window, sinks=sinks, error=err)
+
+    got = run(c.pool, c.table)
+    assert err.item() == 0
+    for r, n in enumerate(ns):
+        for i in sorted({0, n // 2, n - 1} if n else ()):
+            t = offs[r] + i
+            want, tol = c.attend(q64[t], r, before[r] + i, dim ** -0.5, window, sinks, P_ROUND["prefill"])
+            check(torch, got[t], want, tol)
+    assert torch.equal(run(c.pool, c.table), got)
+    row = len(ns) // 2 if ns[len(ns) // 2] else int(np.argmax(ns))
+    mine = torch.zeros(int(offs[-1]), dtype=torch.bool, device="cuda")
+    mine[offs[row]:offs[row + 1]] = True
+    last = (lens[row] - 1) // page  # the page of the row's last position
+    table = c.table.clone()
+    table[row, last] = -1
+    bad = run(c.pool, table)
+    assert err.item() == 1 and torch.equal(bad[~mine], got[~mine]) and torch.isfinite(bad.float()).all()
+    assert not torch.equal(bad[mine], got[mine])
+    pool = c.pool.clone()
+    pool[1, int(c.table[row, last]), 1, 0, (lens[row] - 1) % page, 5] = float("inf")  # seen by its last query only
+    far = run(pool, c.table)
+    assert err.item() == 0 and torch.equal(far[~mine], got[~mine])
+    assert torch.isinf(far[offs[row + 1] - 1, :group, 5].float()).all()
+    mine[offs[row + 1] - 1] = False
+    assert torch.isfinite(far[mine].float()).all()
+
+
+def test_rows_aligned_to_16_bytes(yar, torch):
+    """q and out rows whose addresses are multiples of 16 bytes, not of 32."""
+    for dim, heads in ((64, 4), (128, 6)):
+        c = Cache(torch, [150, 30], 2, dim, 16, seed=12)
+        offs = torch.tensor([0, 100, 130], dtype=torch.int32, device="cuda")
+        q, _ = queries(torch, 130, heads, dim, 3)
+        want = yar.kv_attn_prefill(c.pool, 1, c.table, c.lengths, offs, q)
+        width = heads * dim
+        qs, os_ = (torch.full((131 * (width + 8),), 7.0, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+        q2, out = (x[8:].as_strided((130, heads, dim), (width + 8, dim, 1), 8) for x in (qs, os_))
+        q2.copy_(q)
+        assert out.data_ptr() % 32 == 16
+        yar.kv_attn_prefill(c.pool, 1, c.table, c.lengths, offs, q2, out=out)
+        assert torch.equal(out, want)
+        rest = torch.ones_like(os_, dtype=torch.bool)
+        rest.as_strided(out.shape, out.stride(), 8)[:] = False
+        assert (os_[rest] == 7).all()
+        one = yar.kv_attn_decode(c.pool, 1, c.table, c.lengths, q[:2])
+        os_.fill_(7.0)
+        yar.kv_attn_decode(c.pool, 1, c.table, c.lengths, q2[:2], out=out[:2])
+        assert torch.equal(out[:2], one) and (os_[rest] == 7).all()
+
+
 def test_large_scores_and_a_given_scale(yar, torch):
     """Scores far from zero (a running maximum that moves, weights that vanish)."""
     for dim, spread, scale in ((128, 6.0, None), (64, 3.0, 0.7)):

@@ -185,6 +185,8 @@ void configure_gemm_tc_kernels();
 // A 2-D TMA map of `rows` dense rows of `width` BF16 at `base`, {64, box_rows} boxes,
 // 128-byte swizzle; false when the driver's encoder is unavailable or refuses it.
 bool encode_rows_map(CUtensorMap *map, const bf16 *base, uint64_t rows, int width, int box_rows);
+bool encode_heads_map(CUtensorMap *map, const bf16 *base, uint64_t queries, int heads, int width, uint64_t stride,
+                      int box_heads, int box_queries);
 void launch_qkv_post_prefill(const Model &m, Session &s, int layer, int row, int start, int T,
                              cudaStream_t st);
 void launch_attn_prefill(const Model &m, Session &s, int layer, int row, int start, int T,

@@ -362,6 +362,22 @@ bool encode_rows_map(CUtensorMap *map, const bf16 *base, uint64_t rows, int widt
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// [queries][heads][width] BF16, `stride` elements between queries: boxes of box_heads x box_queries
+// rows of 64 values.
+bool encode_heads_map(CUtensorMap *map, const bf16 *base, uint64_t queries, int heads, int width, uint64_t stride,
+                      int box_heads, int box_queries) {
+  const EncodeTiled fn = encode_fn();
+  if (!fn || queries == 0 || (reinterpret_cast<uintptr_t>(base) & 15) != 0 || stride % 8 != 0 || stride >= 1ull << 38)
+    return false;
+  const cuuint64_t dims[3] = {cuuint64_t(width), cuuint64_t(heads), cuuint64_t(queries)};
+  const cuuint64_t strides[2] = {cuuint64_t(width) * 2, cuuint64_t(stride) * 2};
+  const cuuint32_t box[3] = {64, cuuint32_t(box_heads), cuuint32_t(box_queries)};
+  const cuuint32_t es[3] = {1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<bf16 *>(base), dims, strides, box, es,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 void configure_gemm_tc_kernels() {
   YAR_CUDA(cudaFuncSetAttribute(k_gemm_tc<kEpiStore>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTcSmem));
   YAR_CUDA(cudaFuncSetAttribute(k_gemm_tc<kEpiResidual>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTcSmem));
