@@ -452,6 +452,61 @@ def test_captured_calls_on_another_stream_replay(yar, torch):
         assert torch.equal(spare[:, n:n + 2].view(torch.int16), spare[:, src].view(torch.int16))
 
 
+def test_calls_in_a_row_see_each_others_results(yar, torch):
+    """Copies, both forms of attention and compaction on each other's results without a pause
+    (a call may get ready while the one before it runs): as with a synchronization after each.
+    The same captured, behind fills and copies and behind another stream's work."""
+    c = Cache(torch, [4 * 64, 4 * 64, 900], 8, 64, 64, seed=44)
+    q, _ = queries(torch, 3, 16, 64, 6)
+    offs = torch.arange(4, dtype=torch.int32, device="cuda")
+    counts = torch.tensor([4, 4, 15], dtype=torch.int32, device="cuda")
+    a, b = c.table[0, :4].tolist(), c.table[1, :4].tolist()
+    pool, dst = torch.empty_like(c.pool), torch.empty_like(c.table)
+
+    def chain(sync, side=None):
+        outs = []
+
+        def step(x=None):
+            if x is not None:
+                outs.append(x)
+            if sync:
+                torch.cuda.synchronize()
+
+        pool.copy_(c.pool)
+        for n in range(3):
+            if side is not None:  # the chain goes on behind another stream's work
+                side.wait_stream(torch.cuda.current_stream())
+                with torch.cuda.stream(side):
+                    dst.fill_(n)
+                torch.cuda.current_stream().wait_stream(side)
+            yar.kv_copy_pages(pool, a, b, tokens=[16 * (n + 1)] * 4), step()
+            step(yar.kv_attn_decode(pool, 1, c.table, c.lengths, q))
+            step(yar.kv_attn_prefill(pool, 1, c.table, c.lengths, offs, outs[-1]))
+            step(yar.kv_attn_decode(pool, 1, c.table, c.lengths, outs[-1], window=100, sinks=3))
+            table = yar.kv_compact(pool, c.table, counts, out=dst)[0]
+            step()
+            step(yar.kv_attn_prefill(pool, 1, table, c.lengths, offs, outs[-1]))
+            pool.copy_(c.pool)
+        return outs
+
+    want = chain(True)
+    for _ in range(5):
+        for got in zip(chain(False), want):
+            assert torch.equal(*got)
+    side = torch.cuda.Stream()
+    for other in (None, side):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs = chain(False, other)
+        for _ in range(3):
+            for o in outs:
+                o.zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            for got in zip(outs, want):
+                assert torch.equal(*got)
+
+
 def test_calls_on_two_streams_at_once(yar, torch):
     c = Cache(torch, [1500, 700, 900], 2, 128, 64, seed=13)
     q, _ = queries(torch, 3, 4, 128, 4)

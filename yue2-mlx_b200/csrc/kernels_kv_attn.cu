@@ -3,6 +3,7 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "kv_launch.cuh"
 #include "kv_ops.h"
 
 namespace yar {
@@ -107,7 +108,7 @@ __global__ void __launch_bounds__(32 * W, 8 / W) k_kv_attn_decode(const __grid_c
   __shared__ float part_o[Q * D];         // the block's output, scaled to its m
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int C = gridDim.x, rank = blockIdx.x, kvh = blockIdx.y, row = blockIdx.z, G = p.heads / p.kv_heads;
-  if (p.partials) pdl_launch_dependents();  // the join kernel may get ready; it waits for this grid's end
+  kv_overlap();
 
   const int P = 1 << p.page_shift, cap = p.pages_per_row << p.page_shift;
   int len = p.lengths[row];
@@ -341,7 +342,7 @@ __global__ void __launch_bounds__(32 * W, 8 / W) k_kv_attn_decode(const __grid_c
 template <int D>
 __global__ void __launch_bounds__(D) k_kv_attn_join(const __grid_constant__ KvAttnParams p, int parts) {
   const int h = blockIdx.x, row = blockIdx.y, d = threadIdx.x;
-  pdl_wait();
+  kv_overlap();
   const float *src = p.partials + (size_t(row) * p.heads + h) * parts * (D + 2);
   constexpr int B = 8;  // parts read in one round trip
   float M = -INFINITY, L = 0.f, O = 0.f;
@@ -372,29 +373,9 @@ __global__ void __launch_bounds__(D) k_kv_attn_join(const __grid_constant__ KvAt
 // `split` blocks per (row, kv head): a cluster, or (p.partials) parts for k_kv_attn_join.
 template <int D, int NT, int W>
 void decode_launch(const KvAttnParams &p, int split, cudaStream_t st) {
-  const int cluster = p.partials ? 1 : split;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(split, p.kv_heads, p.rows);
-  cfg.blockDim = dim3(32 * W);
-  cfg.dynamicSmemBytes = DecCfg<D, W>::kRing;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = cluster;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  YAR_CUDA(cudaLaunchKernelEx(&cfg, k_kv_attn_decode<D, NT, W>, p));
-  if (!p.partials) return;
-  cudaLaunchConfig_t join = {};
-  join.gridDim = dim3(p.heads, p.rows);
-  join.blockDim = dim3(D);
-  join.stream = st;
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  join.attrs = attr;
-  join.numAttrs = 1;
-  YAR_CUDA(cudaLaunchKernelEx(&join, k_kv_attn_join<D>, p, split));
+  kv_launch(k_kv_attn_decode<D, NT, W>, dim3(split, p.kv_heads, p.rows), 32 * W, DecCfg<D, W>::kRing,
+            p.partials ? 1 : split, st, p);
+  if (p.partials) kv_launch(k_kv_attn_join<D>, dim3(p.heads, p.rows), D, 0, 1, st, p, split);
 }
 
 template <int D, int NT, int W>

@@ -9,6 +9,7 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "kv_launch.cuh"
 #include "kv_ops.h"
 
 namespace yar {
@@ -40,6 +41,7 @@ __device__ __forceinline__ void copy_words(const uint4 *src, uint4 *dst, int n) 
 
 // Grid (run, layer, pair): a run is one head's K or V positions of a page, contiguous.
 __global__ void __launch_bounds__(kCopyThreads) k_kv_copy_pages(const __grid_constant__ CopyPagesParams p) {
+  kv_overlap();
   const int pair = blockIdx.z;
   const size_t run = size_t(p.page_tokens) * p.head_dim, page = run * p.runs;
   const bf16 *s = p.src + blockIdx.y * p.src_layer + p.from[pair] * page + blockIdx.x * run;
@@ -72,10 +74,10 @@ __device__ __forceinline__ bool listed_entry(const CompactParams &p, int row, in
 // no destination is a source and every move can run at once.
 __global__ void __launch_bounds__(kPlanThreads) k_kv_compact_plan(CompactParams p) {
   extern __shared__ unsigned bits[];
-  pdl_launch_dependents();
   __shared__ int warp_total[kPlanThreads / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, words = (p.pages + 31) / 32;
   for (int i = tid; i < words; i += kPlanThreads) bits[i] = 0;
+  kv_overlap();
   __syncthreads();
   // All entries of all rows in one pass (a row at a time would wait for each row's count).
   const long long entries = (long long)p.rows * p.pages_per_row;
@@ -150,7 +152,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_compact_plan(CompactParams 
 
 // The moves (a grid-stride loop over (move, layer)) and the rewritten tables.
 __global__ void __launch_bounds__(kCopyThreads) k_kv_compact_move(CompactParams p) {
-  pdl_wait();  // the plan is complete
+  kv_overlap();  // the plan is complete
   const long long entries = (long long)p.rows * p.pages_per_row;
   for (long long i = (long long)blockIdx.x * kCopyThreads + threadIdx.x; i < entries;
        i += (long long)gridDim.x * kCopyThreads) {
@@ -191,8 +193,7 @@ void launch_kv_copy_pages(const KvPool &from, const KvPool &to, const int32_t *s
       p.to[i] = dst[i0 + i];
       p.tokens[i] = tokens ? tokens[i0 + i] : from.page_tokens;
     }
-    k_kv_copy_pages<<<dim3(p.runs, from.layers, k), kCopyThreads, 0, st>>>(p);
-    YAR_CUDA(cudaGetLastError());
+    kv_launch(k_kv_copy_pages, dim3(p.runs, from.layers, k), kCopyThreads, 0, 1, st, p);
   }
 }
 
@@ -215,19 +216,8 @@ void launch_kv_compact(const KvPool &pool, const int *table, long long table_str
   p.used = used;
   p.work = work;
   p.error = error;
-  k_kv_compact_plan<<<1, kPlanThreads, size_t((pool.pages + 31) / 32) * 4, st>>>(p);
-  YAR_CUDA(cudaGetLastError());
-  // Eight blocks fill an SM's threads; the launch overlaps the plan.
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(148 * 8);
-  cfg.blockDim = dim3(kCopyThreads);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  YAR_CUDA(cudaLaunchKernelEx(&cfg, k_kv_compact_move, p));
+  kv_launch(k_kv_compact_plan, 1, kPlanThreads, size_t((pool.pages + 31) / 32) * 4, 1, st, p);
+  kv_launch(k_kv_compact_move, 148 * 8, kCopyThreads, 0, 1, st, p);  // eight blocks fill an SM's threads
 }
 
 void configure_kv_kernels() {

@@ -43,7 +43,8 @@
 // 128-key tiles with one S buffer each (1.9 times the time, issue-bound), S and P V issued by warps
 // of their own (84 us on the second case), A's and B's exponentials taking turns (151), the
 // exponentials of a tile run beside the next one's maximum (182: S would have to be three
-// tiles ahead), no maximum but for tiles that leave the range (146 against 139).
+// tiles ahead), no maximum but for tiles that leave the range (146 against 139); of the form with
+// items, two threads a row (294 against 270), P in columns of its own and S one tile ahead (283).
 #include <cuda.h>
 
 #include <algorithm>
@@ -51,6 +52,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "kv_launch.cuh"
 #include "kv_ops.h"
 #include "tcgen05.cuh"
 
@@ -316,6 +318,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  kv_overlap();  // (nothing so far touches what the kernel before this one writes)
   if (warp == 10) {
     __syncwarp();
     asm volatile("bar.arrive 3, %0;" ::"n"(kPreThreads) : "memory");
@@ -1031,18 +1034,8 @@ __global__ void __launch_bounds__(kPreThreads, 1)
 
 template <int D>
 void prefill_launch(const CUtensorMap &map, const CUtensorMap &q_map, const KvAttnParams &p, const PrefillExtra &x, int cluster, cudaStream_t st) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(x.pairs) * cluster, p.kv_heads);
-  cfg.blockDim = dim3(kPreThreads);
-  cfg.dynamicSmemBytes = PreCfg<D>::kSmem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = cluster;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  YAR_CUDA(cudaLaunchKernelEx(&cfg, k_kv_attn_prefill<D>, map, q_map, p, x));
+  kv_launch(k_kv_attn_prefill<D>, dim3(unsigned(x.pairs) * cluster, p.kv_heads), kPreThreads, PreCfg<D>::kSmem, cluster,
+            st, map, q_map, p, x);
 }
 }  // namespace
 
