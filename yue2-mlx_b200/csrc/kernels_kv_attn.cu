@@ -1,6 +1,7 @@
 // kernels_kv_attn.cu — attention of single tokens over a paged cache: softmax(scale q K^T) V of
 // the visible positions, zeros for a row that sees nothing.
 #include <algorithm>
+#include <cmath>
 
 #include "common.cuh"
 #include "kv_launch.cuh"
@@ -18,30 +19,33 @@ namespace yar {
 // with an SM each, 7 run at once), so a few long rows are split into as many parts as there
 // are SMs instead, given a workspace, and joined by a second kernel.
 //
-// Each of a block's warps takes 16 positions at a time (a slice) through its own ring
-// of cp.async copies (16 bytes a lane, any page size; rows that are not visible or whose
-// page is bad arrive as zeros), so no barrier separates the warps until their states are
-// joined. Per slice, on mma.m16n8k16 (BF16 in, FP32 out), with the group's queries as the
-// eight columns (two column tiles for groups of more than eight):
-//   S [16 keys x 8] = K q^T, D / 16 products;
+// Each of a block's warps takes 8 KB at a time (a slice: 16 positions of 128 dims, or 32 of 64, whose
+// two tiles of 16 take their steps side by side: 25 rows of up to 7,192 positions 77 -> 59 us, 33
+// of up to 1,505 12.0 -> 10.5) through its own ring of cp.async copies (16 bytes a lane, any page
+// size; rows that are not visible or whose page is bad arrive as zeros), so no barrier separates
+// the warps until their states are joined. Per slice, on mma.m16n8k16 (BF16 in, FP32 out), with
+// the group's queries as the eight columns (two column tiles for groups of more than eight):
+//   S [keys x 8] = K q^T, D / 16 products for each 16;
 //   m = max(m, S), P = 2^(S scale log2(e) - m), l += P in FP32;
 //   O^T [D x 8] += V^T P, with P as two BF16 parts (P keeps 16 bits, so the result's error
 //   is its own rounding): P's fragment is transposed in registers (movmatrix).
 // The tensor and issue work per slice is well below the time in which HBM delivers its 8 KB to
 // an SM (issue slots 40 % busy at 6.2 TB/s), which is why the plain mma.sync form suffices.
-// Measured: 64 rows with 2,052 visible positions 81 us (524 MB, the rate of a plain copy); one
-// row of 24,000 positions 23 us with a workspace, 28 without (98 MB, 15 us at that rate: the
-// start of the launch, the table's round trip and the join are the rest); one row of 513
-// positions 6 us, of 64 3.5 us; 33 rows of 14 heads of 64 on pages of 16, 9.7 us.
+// Measured (calls in a graph on inputs in turn): 64 rows with 2,052 visible positions 86 us (524
+// MB, 6.1 TB/s); one row of 24,000 positions 24 us with a workspace, 29 without (98 MB, 15 us at a
+// plain copy's rate: the start of the launch, the table's round trip and the join are the rest);
+// one row of 513 positions 6.8 us, of 16 4.4; 33 rows of 14 heads of 64 on pages of 16, 10.9 us.
 namespace {
-constexpr int kDecSlice = 16, kDecMaxCluster = 16;
+constexpr int kDecMaxCluster = 16;
+constexpr int dec_slice(int head_dim) { return 2048 / head_dim; }  // positions of a slice: its K and V are 8 KB
 
 // W warps of a block: 8, one block per SM (192 KB of rings), or 4, two blocks per SM.
 template <int D, int W>
 struct DecCfg {
   static constexpr int kThreads = 32 * W;
-  static constexpr int kStage = 2 * kDecSlice * D * 2;  // bytes of one slice: K, then V
-  static constexpr int kStages = D == 128 ? 3 : 6;      // ring depth of a warp
+  static constexpr int kSlice = dec_slice(D);
+  static constexpr int kStage = 2 * kSlice * D * 2;  // bytes of one slice: K, then V
+  static constexpr int kStages = 3;                  // ring depth of a warp
   static constexpr int kRing = W * kStages * kStage;
 };
 
@@ -99,7 +103,8 @@ __device__ __forceinline__ void cluster_sync() {
 template <int D, int NT, int W>
 __global__ void __launch_bounds__(32 * W, 8 / W) k_kv_attn_decode(const __grid_constant__ KvAttnParams p) {
   using Cfg = DecCfg<D, W>;
-  constexpr int KS = D / 16, CPR = D / 8, Q = 8 * NT;  // mma steps, 16-byte chunks of a row, columns
+  // mma steps, 16-byte chunks of a row, columns; positions of a slice, and mma tiles of them.
+  constexpr int KS = D / 16, CPR = D / 8, Q = 8 * NT, SL = Cfg::kSlice, KT = SL / 16;
   extern __shared__ __align__(128) unsigned char ring[];
   // After the loop the ring's space holds the warps' outputs, [warp][Q][D] FP32.
   static_assert(W * Q * D * 4 <= Cfg::kRing, "the warps' outputs fit the ring");
@@ -120,15 +125,15 @@ __global__ void __launch_bounds__(32 * W, 8 / W) k_kv_attn_decode(const __grid_c
   const int lo = p.window ? max(0, len - p.window) : 0, sinks = p.window ? min(p.sinks, lo) : 0;
   const int seen = len > 0 ? sinks + len - lo : 0;
   // Slices of this block: a contiguous share; warp w takes every W-th.
-  const int slices = (seen + kDecSlice - 1) / kDecSlice, per = (slices + C - 1) / C;
+  const int slices = (seen + SL - 1) / SL, per = (slices + C - 1) / C;
   const int s0 = min(slices, rank * per), s1 = min(slices, s0 + per);
   const int n = max(0, (s1 - s0 - warp + W - 1) / W);  // this warp's slices
 
   const int *tab = p.table + size_t(row) * p.table_stride;
-  // Lane l (and l + 16) looks after key l & 15 of a slice: its page-table entry (-1: no key),
+  // Lane l looks after key l % SL of a slice: its page-table entry (-1: no key),
   // loaded two slices before the copies that need it.
   auto entry_of = [&](int i) {
-    const int v = (s0 + warp + i * W) * kDecSlice + (lane & 15);
+    const int v = (s0 + warp + i * W) * SL + lane % SL;
     if (i >= n || v >= seen) return -1;
     const int e = tab[(v < sinks ? v : lo + v - sinks) >> p.page_shift];
     return e < 0 || e >= p.pages ? -2 : e;
@@ -145,20 +150,20 @@ __global__ void __launch_bounds__(32 * W, 8 / W) k_kv_attn_decode(const __grid_c
     bad |= page == -2;
     if (i < n) {
       const uint32_t st = my_ring + (i % Cfg::kStages) * Cfg::kStage;
-      const int v0 = (s0 + warp + i * W) * kDecSlice;
+      const int v0 = (s0 + warp + i * W) * SL;
 #pragma unroll
-      for (int r0 = 0; r0 < kDecSlice; r0 += RPI) {
+      for (int r0 = 0; r0 < SL; r0 += RPI) {
         const int r = r0 + cr, pg = __shfl_sync(0xFFFFFFFFu, page, r), v = v0 + r;
         const int j = v < sinks ? v : lo + v - sinks;
         const bool ok = pg >= 0;
         const char *src = head_base + (ok ? size_t(pg) * p.page_elems * 2 + size_t(j & (P - 1)) * (D * 2) : 0);
         const uint32_t dst = st + r * (D * 2) + ((cc ^ (r & 7)) << 4);
         cp16(dst, src, ok);
-        cp16(dst + kDecSlice * D * 2, src + v_off, ok);
+        cp16(dst + SL * D * 2, src + v_off, ok);
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
-    return __ballot_sync(0xFFFFFFFFu, page >= 0) & 0xFFFFu;
+    return __ballot_sync(0xFFFFFFFFu, page >= 0);
   };
   constexpr int S = Cfg::kStages;
   int pages[S + 1];
@@ -205,25 +210,38 @@ __global__ void __launch_bounds__(32 * W, 8 / W) k_kv_attn_decode(const __grid_c
     for (int k = 0; k + 2 < S; ++k) valid[k] = valid[k + 1];
     valid[S - 2] = ahead;
 
-    float s[NT][4];
+    float s[NT][KT][4];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      uint32_t a[4];
-      ldsm4(a, st + kr * (D * 2) + (((2 * k + kc) ^ (kr & 7)) << 4));
+      for (int x = 0; x < KT; ++x) s[t][x][0] = s[t][x][1] = s[t][x][2] = s[t][x][3] = 0.f;
 #pragma unroll
-      for (int t = 0; t < NT; ++t) mma16816(s[t], a, bq[t][k][0], bq[t][k][1]);
-    }
-    const bool in0 = (ok >> (lane >> 2)) & 1u, in1 = (ok >> ((lane >> 2) + 8)) & 1u;
-    uint32_t ph[NT][2], pl[NT][2];
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int x = 0; x < KT; ++x) {
+        uint32_t a[4];
+        ldsm4(a, st + (16 * x + kr) * (D * 2) + (((2 * k + kc) ^ (kr & 7)) << 4));
+#pragma unroll
+        for (int t = 0; t < NT; ++t) mma16816(s[t][x], a, bq[t][k][0], bq[t][k][1]);
+      }
+    uint32_t ph[NT][KT][2], pl[NT][KT][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      if (ok != 0xFFFFu) {
-        s[t][0] = in0 ? s[t][0] : -INFINITY, s[t][1] = in0 ? s[t][1] : -INFINITY;
-        s[t][2] = in1 ? s[t][2] : -INFINITY, s[t][3] = in1 ? s[t][3] : -INFINITY;
+      if (ok != 0xFFFFFFFFu) {
+#pragma unroll
+        for (int x = 0; x < KT; ++x) {
+          const bool in0 = (ok >> (16 * x + (lane >> 2))) & 1u, in1 = (ok >> (16 * x + (lane >> 2) + 8)) & 1u;
+          s[t][x][0] = in0 ? s[t][x][0] : -INFINITY, s[t][x][1] = in0 ? s[t][x][1] : -INFINITY;
+          s[t][x][2] = in1 ? s[t][x][2] : -INFINITY, s[t][x][3] = in1 ? s[t][x][3] : -INFINITY;
+        }
       }
-      float mn[2] = {fmaxf(s[t][0], s[t][2]) * sl2, fmaxf(s[t][1], s[t][3]) * sl2};
+      float mn[2] = {fmaxf(s[t][0][0], s[t][0][2]), fmaxf(s[t][0][1], s[t][0][3])};
+#pragma unroll
+      for (int x = 1; x < KT; ++x) {
+        mn[0] = fmaxf(mn[0], fmaxf(s[t][x][0], s[t][x][2]));
+        mn[1] = fmaxf(mn[1], fmaxf(s[t][x][1], s[t][x][3]));
+      }
+      mn[0] *= sl2, mn[1] *= sl2;
 #pragma unroll
       for (int x = 4; x < 32; x <<= 1) {
         mn[0] = fmaxf(mn[0], __shfl_xor_sync(0xFFFFFFFFu, mn[0], x));
@@ -240,24 +258,29 @@ __global__ void __launch_bounds__(32 * W, 8 / W) k_kv_attn_decode(const __grid_c
         m[t][0] = mn[0], m[t][1] = mn[1];
       }
       const float n0 = m[t][0] == -INFINITY ? 0.f : -m[t][0], n1 = m[t][1] == -INFINITY ? 0.f : -m[t][1];
-      const float e0 = kv_ex2(fmaf(s[t][0], sl2, n0)), e1 = kv_ex2(fmaf(s[t][1], sl2, n1));
-      const float e2 = kv_ex2(fmaf(s[t][2], sl2, n0)), e3 = kv_ex2(fmaf(s[t][3], sl2, n1));
-      l[t][0] += e0 + e2, l[t][1] += e1 + e3;
-      const uint32_t h0 = pack2(e0, e1), h1 = pack2(e2, e3);
-      ph[t][0] = transpose8(h0), ph[t][1] = transpose8(h1);
-      pl[t][0] = transpose8(pack2(e0 - bf_lo(h0), e1 - bf_hi(h0)));
-      pl[t][1] = transpose8(pack2(e2 - bf_lo(h1), e3 - bf_hi(h1)));
-    }
 #pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      uint32_t a[4];
-      ldsm4t(a, st + kDecSlice * D * 2 + vr * (D * 2) + (((2 * k + vc) ^ (vr & 7)) << 4));
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        mma16816(o[t][k], a, ph[t][0], ph[t][1]);
-        mma16816(o[t][k], a, pl[t][0], pl[t][1]);
+      for (int x = 0; x < KT; ++x) {
+        const float e0 = kv_ex2(fmaf(s[t][x][0], sl2, n0)), e1 = kv_ex2(fmaf(s[t][x][1], sl2, n1));
+        const float e2 = kv_ex2(fmaf(s[t][x][2], sl2, n0)), e3 = kv_ex2(fmaf(s[t][x][3], sl2, n1));
+        l[t][0] += e0 + e2, l[t][1] += e1 + e3;
+        const uint32_t h0 = pack2(e0, e1), h1 = pack2(e2, e3);
+        ph[t][x][0] = transpose8(h0), ph[t][x][1] = transpose8(h1);
+        pl[t][x][0] = transpose8(pack2(e0 - bf_lo(h0), e1 - bf_hi(h0)));
+        pl[t][x][1] = transpose8(pack2(e2 - bf_lo(h1), e3 - bf_hi(h1)));
       }
     }
+#pragma unroll
+    for (int x = 0; x < KT; ++x)
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        uint32_t a[4];
+        ldsm4t(a, st + SL * D * 2 + (16 * x + vr) * (D * 2) + (((2 * k + vc) ^ (vr & 7)) << 4));
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          mma16816(o[t][k], a, ph[t][x][0], ph[t][x][1]);
+          mma16816(o[t][k], a, pl[t][x][0], pl[t][x][1]);
+        }
+      }
     __syncwarp();
   }
 
@@ -403,29 +426,36 @@ void launch_kv_attn_decode(const KvAttnParams &p, int head_dim, cudaStream_t st)
   const long long cap = (long long)p.pages_per_row << p.page_shift;
   long long most = p.max_length > 0 ? std::min<long long>(p.max_length, cap) : cap;
   if (p.window) most = std::min<long long>(most, (long long)p.window + p.sinks);
-  const long long units = (long long)p.rows * p.kv_heads, slices = (most + kDecSlice - 1) / kDecSlice;
+  const long long units = (long long)p.rows * p.kv_heads, slices = (most + dec_slice(head_dim) - 1) / dec_slice(head_dim);
   // The form with the smallest estimated time in us: `split` blocks per unit, a block streaming
-  // at most at the rate that one was measured at alone (four warps 45 GB/s, eight 66), all of
-  // them at HBM's; ~3.5 us to start and end a launch, 1.3 more to join a cluster, 2 for the
-  // join kernel, 2.5 for each further wave of clusters (their blocks start together).
-  const double bytes = 2.0 * kDecSlice * head_dim * 2;
+  // at most at the rate that was measured (four warps 45 GB/s, 33 where two share an SM; eight 66),
+  // all of them at HBM's; ~3.5 us to start and end a launch (3.7 with eight warps), 1.3 more to
+  // join a cluster (1.8 of 16 blocks), 2 for the join kernel, 2.5 for each further wave of clusters
+  // (their blocks start together). The host does not know the lengths: the estimate is the mean of
+  // two, for rows of one length (a last wave that is not full counts half) and for ragged ones (0.55 of
+  // the longest at the mean: the longest unit's blocks, or all bytes). Measured, 128 dims, both
+  // kinds: 152 units of 4,000 positions 66 and 55 us with four warps, 80 and 42 with eight, 72 and
+  // 42 split in four; 400 units of 3,000: 115 and 74 with four warps, 100 and 68 with eight.
+  const double bytes = 2.0 * dec_slice(head_dim) * head_dim * 2;
   int split = 1, warps = 4;
   bool parts = false;
   double best = 1e30;
   auto consider = [&](int w, int c, int slots, double fixed) {
     const double blocks = double(units) * c, at_once = std::min(blocks, double(slots));
-    const double rate = std::min(w == 4 ? 45e3 : 66e3, 6500e3 / at_once);  // bytes per us
-    const double waves = std::max(1.0, blocks / slots);
-    const double t = fixed + waves * double((slices + c - 1) / c) * bytes / rate +
-                     (c > 1 && waves > 1 ? 2.5 * waves : 0.0);
+    const bool shared = w == 4 && blocks > kSlots8[0];
+    const double mine = double((slices + c - 1) / c) * bytes, more = blocks / slots;
+    const double waves = std::max(1.0, 0.5 * (more + std::ceil(more)));
+    const double even = waves * mine / std::min(w == 8 ? 66e3 : shared ? 33e3 : 45e3, 6500e3 / at_once);
+    const double ragged = std::max(mine / (w == 8 ? 66e3 : shared ? 39e3 : 45e3), 0.55 * units * slices * bytes / 6500e3);
+    const double t = fixed + 0.5 * (even + ragged) + (c > 1 && more > 1 ? 1.25 * (waves + more) : 0.0);
     if (t >= best) return false;
     best = t, split = c, warps = w;
     return true;
   };
   for (int i = 0; i < 5; ++i) {
-    const double fixed = i ? 4.8 : 3.5;
+    const double fixed = i == 0 ? 3.5 : i < 4 ? 4.8 : 5.3;
     consider(4, 1 << i, kSlots4[i], fixed);
-    if (i < 4) consider(8, 1 << i, kSlots8[i], fixed);  // (16 blocks of eight warps: half as many run)
+    if (i < 4) consider(8, 1 << i, kSlots8[i], fixed + 0.2);  // (16 blocks of eight warps: half as many run)
   }
   if (p.partials && 2 * units <= kSlots8[0])
     parts = consider(8, int(kSlots8[0] / units), kSlots8[0], 5.5);
