@@ -489,6 +489,27 @@ def test_calls_in_a_row_see_each_others_results(yar, torch):
             pool.copy_(c.pool)
         return outs
 
+    # Calls of more blocks than the GPU holds, each on the result of the one before.
+    long = Cache(torch, [3000], 8, 64, 64, seed=45)
+    q0, _ = queries(torch, 3000, 16, 64, 7)
+    ends = torch.tensor([0, 3000], dtype=torch.int32, device="cuda")
+
+    def rounds(sync):
+        x = q0
+        for n in range(4):
+            x = yar.kv_attn_prefill(long.pool, 1, long.table, long.lengths, ends, x, window=300 * n, sinks=2)
+            if sync:
+                torch.cuda.synchronize()
+            x = yar.kv_attn_decode(long.pool, 1, long.table.expand(3000, -1).contiguous(),
+                                   long.lengths.expand(3000).contiguous(), x, window=40) + x
+            if sync:
+                torch.cuda.synchronize()
+        return x
+
+    want = rounds(True)
+    for _ in range(3):
+        assert torch.equal(rounds(False), want)
+
     want = chain(True)
     for _ in range(5):
         for got in zip(chain(False), want):

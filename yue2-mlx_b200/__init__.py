@@ -658,7 +658,8 @@ def kv_compact(pool, page_table, counts, out=None, error=None, stream=None):
     table, remap [pages]: each page's new index or -1, used [1]); ``out`` may be ``page_table``."""
     c_pool, rows = _kv_pool(pool), _kv_rows(page_table, counts)
     if out is None:
-        out = page_table.new_empty(page_table.shape)
+        out = sys.modules["torch"].empty_like(page_table) if page_table.is_contiguous() else \
+            page_table.new_empty(page_table.shape)
         new, new_stride = out.data_ptr(), rows.pages_per_row
     else:
         if out.shape != page_table.shape:
