@@ -116,6 +116,11 @@ __global__ void __launch_bounds__(32 * W, 8 / W) k_kv_attn_decode(const __grid_c
   kv_overlap();
 
   const int P = 1 << p.page_shift, cap = p.pages_per_row << p.page_shift;
+  const int *tab = p.table + size_t(row) * p.table_stride;
+  // The table comes into the L2 while the length, which says where to look in it, is on its way (8.2
+  // -> 7.9 us for 18 rows that see 185 positions).
+  if (warp == 0)
+    for (int i = lane * 32; i < p.pages_per_row; i += 1024) asm volatile("prefetch.global.L2 [%0];" ::"l"(tab + i));
   int len = p.lengths[row];
   if (len > cap) {
     if (rank == 0 && kvh == 0 && tid == 0 && p.error) atomicOr(p.error, kKvBadLength);
@@ -129,7 +134,6 @@ __global__ void __launch_bounds__(32 * W, 8 / W) k_kv_attn_decode(const __grid_c
   const int s0 = min(slices, rank * per), s1 = min(slices, s0 + per);
   const int n = max(0, (s1 - s0 - warp + W - 1) / W);  // this warp's slices
 
-  const int *tab = p.table + size_t(row) * p.table_stride;
   // Lane l looks after key l % SL of a slice: its page-table entry (-1: no key),
   // loaded two slices before the copies that need it.
   auto entry_of = [&](int i) {
