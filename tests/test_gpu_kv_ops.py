@@ -616,6 +616,11 @@ def test_host_memory_is_refused(yar, torch):
         yar.kv_attn_prefill(*ok[:4], torch.tensor([0], dtype=torch.int32).cuda(), q)
     with pytest.raises(ValueError):
         yar.kv_attn_decode(*ok, error=torch.zeros(1, device="cuda"))
+    with pytest.raises(ValueError):  # (as many bytes as it says, but not in memory)
+        yar.kv_attn_decode(*ok, workspace=torch.zeros(1, device="cuda").expand(1 << 20))
+    for wrong in (dict(window=1 << 31), dict(window=2.5), dict(sinks=-1 << 40), dict(scale="x")):
+        with pytest.raises(ValueError):
+            yar.kv_attn_decode(*ok, **wrong)
     host = torch.zeros(1, 4, 64, dtype=torch.bfloat16)
     call = yar._KvAttn(yar._kv_pool(c.pool), yar._kv_rows(c.table, c.lengths), 0, 4, host.data_ptr(), 256, q.data_ptr(),
                        256, 0, 0, 0.125, None)

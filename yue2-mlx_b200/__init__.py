@@ -619,6 +619,8 @@ def kv_attn_decode(pool, layer: int, page_table, lengths, q, out=None, window: i
         raise ValueError("q and out need one row for each row of page_table")
     w, wb = None, 0
     if workspace is not None:
+        if not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous")
         w, wb = workspace.data_ptr(), workspace.numel() * workspace.element_size()
     elif stream is None and rows * pool.shape[3] <= 74 and (max_length or per_row * pool.shape[4]) > 4096 and \
             not 0 < window < 4096:

@@ -95,7 +95,9 @@ struct PrefillExtra {
   int q_boxes;     // Q comes by TMA (its M rows are boxes of whole queries: the group divides a tile)
 };
 
-// A bounded wait (2^16 polls of up to 20 us each) that also ends when another role gave up.
+// A bounded wait (2^16 polls of up to 20 us each, not counted while a tile's rows are recomputed
+// key by key) that also ends when another role gave up. state: [0] given up, [1], [2] tile A, B
+// recomputes.
 __device__ __forceinline__ bool pre_poll(uint64_t *bar, unsigned parity) {
   uint32_t done;
   asm volatile(
@@ -105,17 +107,17 @@ __device__ __forceinline__ bool pre_poll(uint64_t *bar, unsigned parity) {
       : "memory");
   return done != 0;
 }
-__device__ __forceinline__ bool pre_wait_slow(uint64_t *bar, unsigned parity, const volatile int *fail) {
-  for (int i = 0; i < 1 << 16; ++i) {
+__device__ __forceinline__ bool pre_wait_slow(uint64_t *bar, unsigned parity, const volatile int *state) {
+  for (int i = 0; i < 1 << 16; i += !(state[1] | state[2])) {
     if (pre_poll(bar, parity)) return true;
-    if (*fail) return false;
+    if (state[0]) return false;
   }
   return false;
 }
 // True on every lane of the (converged) warp when the phase is over.
-__device__ __forceinline__ bool pre_wait(uint64_t *bar, unsigned parity, const volatile int *fail) {
+__device__ __forceinline__ bool pre_wait(uint64_t *bar, unsigned parity, const volatile int *state) {
   if (__all_sync(0xFFFFFFFFu, pre_poll(bar, parity))) return true;
-  return __all_sync(0xFFFFFFFFu, pre_wait_slow(bar, parity, fail));
+  return __all_sync(0xFFFFFFFFu, pre_wait_slow(bar, parity, state));
 }
 // 2^x by the approximate base-2 exponential, results below 2^-126 as 0 (relative error below
 // 2^-22): without that flush each exponential costs three more instructions.
@@ -288,14 +290,14 @@ __global__ void __launch_bounds__(kPreThreads, 1)
   __shared__ PreTile tiles[2][2];
   __shared__ volatile int bad_keys[2];
   __shared__ uint32_t tmem_slot;
-  __shared__ volatile int s_fail;
+  __shared__ volatile int s_state[3];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = p.heads / p.kv_heads;
   uint32_t C, rank;
   asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(C));
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   // The copying warp sets the barriers up and goes on at once; the others also wait for the tensor memory.
   if (tid == 320) {
-    s_fail = 0;
+    for (int i = 0; i < 3; ++i) s_state[i] = 0;
     auto init = [](uint64_t *bar, int count) {
       asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(at_smem(bar)), "r"(count));
     };
@@ -361,7 +363,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
   auto live = [](const PreTile &t, int i) { return i < t.s1 || (i >= t.w0 && i < t.w1); };
   // The block's k-th item, once it is known (false: a wait ran out); `taken` gives its place back.
   // The place of item k is refilled for k + 2 when all eleven warps have taken k.
-  auto take = [&](int k) { return pre_wait(&item_full[k & 1], unsigned(k >> 1) & 1u, &s_fail); };
+  auto take = [&](int k) { return pre_wait(&item_full[k & 1], unsigned(k >> 1) & 1u, s_state); };
   auto taken = [&](int k) {
     __syncwarp();
     if (lane == 0) at_arrive(&item_empty[k & 1]);
@@ -476,12 +478,12 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         }
         if (lane == 0) pre_claim(claim, &claim_done);
         __syncwarp();
-        ok = pre_wait(&claim_done, unsigned(claims++) & 1u, &s_fail);
+        ok = pre_wait(&claim_done, unsigned(claims++) & 1u, s_state);
         more = ok && pre_claimed(claim, bx, by);
       }
       if (!more) b.row = -1;
       if (!ok) break;
-      if (k >= 2) ok = pre_wait(&item_empty[k & 1], unsigned((k >> 1) - 1) & 1u, &s_fail);
+      if (k >= 2) ok = pre_wait(&item_empty[k & 1], unsigned((k >> 1) - 1) & 1u, s_state);
       if (!ok) break;
       if (lane == 0) {
         items[k & 1] = b;
@@ -524,7 +526,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       };
       for (int j = 0; j <= nt && nt > 0; ++j) {
         const int it = base + j, s = it % NST, i = j + 1;  // the stage's K tile (j = 0: tiles 0 and 1)
-        if (it >= NST) ok = pre_wait(&kv_empty[s], unsigned(it / NST - 1) & 1u, &s_fail);
+        if (it >= NST) ok = pre_wait(&kv_empty[s], unsigned(it / NST - 1) & 1u, s_state);
         if (!ok) break;
         const int tiles = j == 0 ? min(nt, 2) : 1 + (i < nt);
         if (lane == 0)
@@ -548,12 +550,12 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       if (more) {
         if (lane == 0) pre_claim(claim, &claim_done);
         __syncwarp();
-        ok = pre_wait(&claim_done, unsigned(claims++) & 1u, &s_fail);
+        ok = pre_wait(&claim_done, unsigned(claims++) & 1u, s_state);
         more = ok && pre_claimed(claim, bx, by);
       }
     }
     if (!ok) {  // leave no copy in flight
-      s_fail = 1;
+      s_state[0] = 1;
       for (int i = issued > NST ? issued - NST : 0; i < issued; ++i)
         at_wait(&kv_full[i % NST], unsigned(i / NST) & 1u);
       if (claims > 0) at_wait(&claim_done, unsigned(claims - 1) & 1u);
@@ -572,7 +574,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
     int n_s = 0, n_p = 0;    // the tile's key tiles whose S, whose P V was issued (of all items)
     int slot = 0, ph = 0;    // the place in the ring and the parity of its use
     auto wait = [&](uint64_t *bar, int parity) {
-      ok = pre_wait(bar, unsigned(parity), &s_fail);
+      ok = pre_wait(bar, unsigned(parity), s_state);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     };
     auto next = [&] {
@@ -673,7 +675,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
     if (at_elect()) at_commit(&drain[X]);
     __syncwarp();
     if (!at_wait(&drain[X], 0u) || !ok) {
-      s_fail = 1;
+      s_state[0] = 1;
       if (lane == 0 && p.error) atomicOr(p.error, kKvExpired);
     }
   }
@@ -685,7 +687,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
 #pragma unroll
       for (int X = 0; X < 2; ++X) {
         if (!ok || !x.q_boxes) break;
-        if (k > 0) ok = pre_wait(&q_free[X], unsigned(k - 1) & 1u, &s_fail);
+        if (k > 0) ok = pre_wait(&q_free[X], unsigned(k - 1) & 1u, s_state);
         if (ok && lane == 0) {
           asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(at_smem(&q_ready[X])), "r"(Cfg::kQ)
                        : "memory");
@@ -722,7 +724,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
     for (int X = 0; X < 2; ++X)  // (leave no load in flight)
       if (boxes[X]) at_wait(&q_ready[X], unsigned(boxes[X] - 1) & 1u);
     if (!ok) {
-      s_fail = 1;
+      s_state[0] = 1;
       if (lane == 0 && p.error) atomicOr(p.error, kKvExpired);
     }
   }
@@ -773,7 +775,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         if (lane == 0) at_arrive(&q_ready[wg]);
       }
       bool poison = false;
-      ok = pre_wait(&scanned[item & 1], unsigned(item >> 1) & 1u, &s_fail);
+      ok = pre_wait(&scanned[item & 1], unsigned(item >> 1) & 1u, s_state);
       if (item > 0) bad = bad_keys[item & 1] != 0;
       const PreTile tl = tiles[item & 1][wg];
       const int sunk = bad ? 0 : tl.sunk, whole0 = tl.whole0, whole1 = bad ? 0 : tl.whole1;  // (a bad page: looked at piece by piece)
@@ -783,7 +785,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         const int j = b.j0 + i;
         if (!live(tl, i)) continue;
         const int buf = n_s & 1;
-        ok = pre_wait(&s_full[wg][buf], unsigned(n_s >> 1) & 1u, &s_fail);
+        ok = pre_wait(&s_full[wg][buf], unsigned(n_s >> 1) & 1u, s_state);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         float s[kPreN];
@@ -807,7 +809,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
           // A V value that is not finite in a row that only some of the queries see: the product
           // with P = 0 would carry it into the others (a thread looks at half a V row).
           const int it = base + i + 1, r = t & (kPreN - 1);
-          ok = pre_wait(&kv_full[it % NST], unsigned(it / NST) & 1u, &s_fail);
+          ok = pre_wait(&kv_full[it % NST], unsigned(it / NST) & 1u, s_state);
           if (!ok) break;
           if (k0 + r < b.kend && !(k0 + r >= b.sinks && k0 + r < b.lo)) {
             __nv_bfloat162 acc = __floats2bfloat162_rn(0.f, 0.f);
@@ -839,7 +841,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
           row_l *= c;
           row_m = raise ? mx : row_m;
           if (n_s > n_s0) {  // O, once the last P V has landed (the next one waits for this tile's P)
-            ok = pre_wait(&o_done[wg][buf ^ 1], unsigned((n_s - 1) >> 1) & 1u, &s_fail);
+            ok = pre_wait(&o_done[wg][buf ^ 1], unsigned((n_s - 1) >> 1) & 1u, s_state);
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
@@ -893,11 +895,11 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       if (ok) ok = take(item + 1);
       more = ok && items[(item + 1) & 1].row >= 0;
       if (more && !x.q_boxes) {  // (once the item's S products are complete, which are so when it had any)
-        ok = pre_wait(&q_free[wg], unsigned(item) & 1u, &s_fail);
+        ok = pre_wait(&q_free[wg], unsigned(item) & 1u, s_state);
         if (ok) load_q(items[(item + 1) & 1]);
       }
-      if (ok && n_s > n_s0) ok = pre_wait(&o_done[wg][(n_s - 1) & 1], unsigned((n_s - 1) >> 1) & 1u, &s_fail);
-      if (!ok) s_fail = 1;
+      if (ok && n_s > n_s0) ok = pre_wait(&o_done[wg][(n_s - 1) & 1], unsigned((n_s - 1) >> 1) & 1u, s_state);
+      if (!ok) s_state[0] = 1;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       // ---- the result ---------------------------------------------------------------------------
       bool failed = false;
@@ -908,6 +910,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       if (poison && !failed) {
         const bf16 *my_q = p.q + row_at(b, my_row ? tid : 0, p.q_stride);
         // Key by key with the statistics from above (V does not enter them), 32 columns at a time.
+        if (t == 0) s_state[1 + wg] = 1;
         const float nm = row_m == -INFINITY ? 0.f : -row_m;
         for (int cb = 0; cb < D; cb += 32) {
           float o[32];
@@ -930,6 +933,8 @@ __global__ void __launch_bounds__(kPreThreads, 1)
           __syncwarp();
           at_st32(col_o + cb, o);
         }
+        pre_any(1 + wg, false);
+        if (t == 0) s_state[1 + wg] = 0;
       }
       if (C == 1) {
         if (!failed) {
@@ -1019,7 +1024,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       more = more && ok;
     }
     if (!ok) {
-      s_fail = 1;
+      s_state[0] = 1;
       if (lane == 0 && p.error) atomicOr(p.error, kKvExpired);
     }
     if (C > 1 && !syncs) {  // every thread of a cluster takes its two exchanges
