@@ -25,8 +25,8 @@
 // P in BF16 costs 2^-9 of each weight at random, below the rounding of the BF16 result; two
 // BF16 parts would cost half as much tensor work again. Scores, m, l and O are FP32.
 // Masked positions cannot leak: hidden keys' scores are replaced, V rows that nothing in the
-// block sees are zeroed in shared memory, and when a tile that only some queries see holds
-// a V value that is not finite (0 x inf), the block recomputes its sums key by key.
+// item sees are zeroed in shared memory, and when a tile that only some queries see holds
+// a V value that is not finite (0 x inf), the tile's sums are recomputed key by key.
 //
 // Few blocks (a chunk of one prompt) are split along the keys over a cluster of 2 or 4, whose
 // states are joined through distributed shared memory, each block finishing D / C columns.
@@ -778,7 +778,8 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       ok = pre_wait(&scanned[item & 1], unsigned(item >> 1) & 1u, s_state);
       if (item > 0) bad = bad_keys[item & 1] != 0;
       const PreTile tl = tiles[item & 1][wg];
-      const int sunk = bad ? 0 : tl.sunk, whole0 = tl.whole0, whole1 = bad ? 0 : tl.whole1;  // (a bad page: looked at piece by piece)
+      // (With a bad page every tile is looked at piece by piece.)
+      const int sunk = bad ? 0 : tl.sunk, whole0 = tl.whole0, whole1 = bad ? 0 : tl.whole1;
       const int pos = tid < b.rows ? max(b.len - b.n + b.q0 + (((b.r0 + tid) * inv_g) >> 16), -1) : -1;
       float row_m = -INFINITY, row_l = 0.f;  // running maximum and sum
       for (int i = 0; i < nt && ok; ++i) {
@@ -1063,12 +1064,17 @@ void launch_kv_attn_prefill(const KvPool &pool, int layer, const KvAttnParams &p
   x.q_boxes = kPreM % G == 0 && encode_heads_map(&q_map, p.q, uint64_t(p.n_queries), p.heads, pool.head_dim,
                                                  uint64_t(p.q_stride), int(G), int(kPreM / G));
   // Blocks of one prompt's chunk that leave SMs idle are split along the keys (over 2, then 4
-  // blocks), as long as each keeps four key tiles.
+  // blocks), as long as each keeps five key tiles (24 blocks of
+  // at most 512 positions: 13.6 us whole, 15.0 halved; 40 of 768: 19.8, 18.4).
   const long long blocks = pairs * p.kv_heads;
   const long long positions = p.offsets ? (long long)p.pages_per_row << p.page_shift : p.length;
   const long long keys = p.window ? std::min<long long>(positions, (long long)p.window + p.sinks) : positions;
   int cluster = 1;
-  while (cluster < 4 && blocks * cluster * 2 <= 148 && keys >= cluster * 2 * 4 * kPreN) cluster *= 2;
+  while (cluster < 4 && blocks * cluster * 2 <= 148 && keys >= cluster * 2 * 5 * kPreN) cluster *= 2;
+  // One row with up to half a wave more blocks than SMs: halves end after 1.5 waves instead of 2, each
+  // wave of them ~10 us more (2,560 queries over 10,560 positions 272 -> 227 us, over 4,560 103 ->
+  // 102, over 2,560 50 -> 61). Ragged rows fill the gaps by themselves.
+  if (cluster == 1 && p.rows == 1 && blocks > 148 && blocks <= 222 && keys - p.n_queries / 2 >= 4096) cluster = 2;
   if (pool.head_dim == 128)
     prefill_launch<128>(map, q_map, p, x, cluster, st);
   else
