@@ -194,7 +194,7 @@ MANY = [
     ([i * 5 % 4 for i in range(150)] + [700, 0, 3], [i * 11 % 90 for i in range(153)], 2, 4, 128, 32, 40, 5),
     ([4000], [100], 8, 2, 64, 64, 200, 70), ([900, 60], [0, 500], 8, 7, 128, 256, 0, 0),
     ([2 + 31 * i % 400 for i in range(20)], [0] * 20, 8, 16, 64, 16, 90, 20),
-    ([2560], [4000], 8, 2, 64, 64, 0, 0),  # (halves of the keys, in more than one wave)
+    ([2560], [6000], 8, 2, 64, 64, 0, 0),  # (halves of the keys, in more than one wave)
 ]
 
 

@@ -36,10 +36,11 @@
 // a softmax group ~1,250, most of them exponentials; the rest is the hand-over between them. From
 // one item's last P to the next one's first S ~4,500 cycles (O's division and stores 2,700).
 // Measured (16 query / 8 KV heads of 128): 16,384 tokens with a window of 2,048: 270 us, 955
-// TFLOP/s; 1,024 queries over 8,192 positions: 75 us, 858 TFLOP/s (145 us without the split);
-// 24 ragged rows: 121 us; 77 queries of 4 heads of 64: 10 us. With one item a block 302, 77, 147
-// and 10 us; items in turn with Q through registers 313 and 151 (the loads' latency stood between
-// two items: ~10,000 cycles), by cp.async of the softmax warps 280 and 127. Tried and slower:
+// TFLOP/s; 8,000 tokens without one: 234 us, 1,120; 1,024 queries over 8,192 positions: 76 us, 850
+// (140 us without the split); 24 ragged rows: 122 us; 77 queries of 4 heads of 64: 10 us. With one
+// item a block 302, -, 77, 147 and 10 us; items in turn with Q through registers 313 and 151 for
+// the first and the ragged rows (the loads' latency stood between two items: ~10,000 cycles), by
+// cp.async of the softmax warps 280 and 127. Tried and slower:
 // 128-key tiles with one S buffer each (1.9 times the time, issue-bound), S and P V issued by warps
 // of their own (84 us on the second case), A's and B's exponentials taking turns (151), the
 // exponentials of a tile run beside the next one's maximum (182: S would have to be three
@@ -242,18 +243,16 @@ __device__ __forceinline__ void pre_claim(void *to, uint64_t *bar) {
       : "memory");
 }
 // The claimed block's index; false when none was left.
-__device__ __forceinline__ bool pre_claimed(const void *from, int &bx, int &by) {
-  uint32_t got, cx = 0, cy = 0;
+__device__ __forceinline__ bool pre_claimed(const void *from, int &bx) {
+  uint32_t got, cx;
   asm volatile(
-      "{\n .reg .b128 r;\n .reg .pred p;\n ld.shared.b128 r, [%3];\n"
-      " clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n selp.u32 %0, 1, 0, p;\n"
-      " mov.u32 %1, 0;\n mov.u32 %2, 0;\n"
-      " @p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n"
-      " @p clusterlaunchcontrol.query_cancel.get_first_ctaid::y.b32.b128 %2, r;\n}"
-      : "=r"(got), "=r"(cx), "=r"(cy)
+      "{\n .reg .b128 r;\n .reg .pred p;\n ld.shared.b128 r, [%2];\n"
+      " clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n selp.u32 %0, 1, 0, p;\n mov.u32 %1, 0;\n"
+      " @p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n}"
+      : "=r"(got), "=r"(cx)
       : "r"(at_smem(from))
       : "memory");
-  bx = int(cx), by = int(cy);
+  bx = int(cx);
   return got != 0;
 }
 
@@ -390,9 +389,12 @@ __global__ void __launch_bounds__(kPreThreads, 1)
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPreRegsIssue));
   if (warp == 10) {
     // ---- items and copies -----------------------------------------------------------------
-    // The row and the 256 M rows of block bx: the last pairs (the longest) first. False: none.
+    // The KV head, row and 256 M rows of block bx: the last pairs (the longest) of every head first, so
+    // that the last blocks to start are short (4,096 tokens from nothing: 106 us head after head, 76
+    // so). False: none.
     auto find = [&](int bx, PreBlock &b) {
-      const int slot = x.pairs - 1 - bx / int(C);
+      const int unit = bx / int(C), slot = x.pairs - 1 - unit / p.kv_heads;
+      b.kvh = unit % p.kv_heads;
       int row = -1, first = 0, n = 0, pair = 0, len = p.length;
       if (!p.offsets) {
         row = 0, n = p.n_queries, pair = slot;
@@ -464,14 +466,12 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       b.j0 = min(total, int(rank) * per), b.j1 = min(total, b.j0 + per);
       return true;
     };
-    int bx = int(blockIdx.x), by = int(blockIdx.y), claims = 0, base = 0, issued = 0;
+    int bx = int(blockIdx.x), claims = 0, base = 0, issued = 0;
     bool ok = true, more = true;
     for (int k = 0; ok; ++k) {
       PreBlock b;
       while (more) {
-        const bool found = find(bx, b);
-        b.kvh = by;
-        if (found) break;
+        if (find(bx, b)) break;
         if (C > 1) {  // (a cluster's blocks share their pair)
           more = false;
           break;
@@ -479,7 +479,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         if (lane == 0) pre_claim(claim, &claim_done);
         __syncwarp();
         ok = pre_wait(&claim_done, unsigned(claims++) & 1u, s_state);
-        more = ok && pre_claimed(claim, bx, by);
+        more = ok && pre_claimed(claim, bx);
       }
       if (!more) b.row = -1;
       if (!ok) break;
@@ -551,7 +551,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         if (lane == 0) pre_claim(claim, &claim_done);
         __syncwarp();
         ok = pre_wait(&claim_done, unsigned(claims++) & 1u, s_state);
-        more = ok && pre_claimed(claim, bx, by);
+        more = ok && pre_claimed(claim, bx);
       }
     }
     if (!ok) {  // leave no copy in flight
@@ -1040,7 +1040,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
 
 template <int D>
 void prefill_launch(const CUtensorMap &map, const CUtensorMap &q_map, const KvAttnParams &p, const PrefillExtra &x, int cluster, cudaStream_t st) {
-  kv_launch(k_kv_attn_prefill<D>, dim3(unsigned(x.pairs) * cluster, p.kv_heads), kPreThreads, PreCfg<D>::kSmem, cluster,
+  kv_launch(k_kv_attn_prefill<D>, unsigned(x.pairs) * p.kv_heads * cluster, kPreThreads, PreCfg<D>::kSmem, cluster,
             st, map, q_map, p, x);
 }
 }  // namespace
@@ -1055,7 +1055,7 @@ void launch_kv_attn_prefill(const KvPool &pool, int layer, const KvAttnParams &p
   const long long G = p.heads / p.kv_heads;
   // Pairs of 256 M rows: exactly, or rounded up for each row of queries.
   const long long pairs = (p.n_queries * G + 255) / 256 + (p.offsets ? p.rows - 1 : 0);
-  if (pairs > (1 << 28)) throw Error("ValueError", "too many queries for one call");
+  if (pairs * p.kv_heads > (1 << 28)) throw Error("ValueError", "too many queries for one call");
   x.pairs = int(pairs);
   CUtensorMap map;
   if (!encode_rows_map(&map, pool.data, uint64_t(x.total_rows), pool.head_dim, x.box_rows))
@@ -1072,9 +1072,9 @@ void launch_kv_attn_prefill(const KvPool &pool, int layer, const KvAttnParams &p
   int cluster = 1;
   while (cluster < 4 && blocks * cluster * 2 <= 148 && keys >= cluster * 2 * 5 * kPreN) cluster *= 2;
   // One row with up to half a wave more blocks than SMs: halves end after 1.5 waves instead of 2, each
-  // wave of them ~10 us more (2,560 queries over 10,560 positions 272 -> 227 us, over 4,560 103 ->
-  // 102, over 2,560 50 -> 61). Ragged rows fill the gaps by themselves.
-  if (cluster == 1 && p.rows == 1 && blocks > 148 && blocks <= 222 && keys - p.n_queries / 2 >= 4096) cluster = 2;
+  // wave of them ~10 us more (2,560 queries over 10,560 positions 255 -> 230 us, over 6,560 of 64
+  // dims 134 -> 136, over 4,560 87 -> 108). Ragged rows fill the gaps by themselves.
+  if (cluster == 1 && p.rows == 1 && blocks > 148 && blocks <= 222 && keys - p.n_queries / 2 >= 6144) cluster = 2;
   if (pool.head_dim == 128)
     prefill_launch<128>(map, q_map, p, x, cluster, st);
   else
