@@ -112,12 +112,12 @@ def test_windowed_persistent_decode_equals_the_per_operation_path(wide, rows, wi
     model, _, _ = wide
     out = []
     for persistent in (True, False):
-        s = model.session(max_rows=2, max_ctx=3072)
+        s = model.session(max_rows=2, max_ctx=2976)
         s.set_persistent(persistent)
         s.set_trace(persistent)
         s.set_window(window, sinks)
         for r in range(rows):
-            s.reset(r, 3072)
+            s.reset(r, 2976)
             s.prefill(r, ids(7 + r, n - 900 * r), phase=None)
         out.append(steps(s, list(range(rows)), ids(9, 70)))  # the window's start crosses chunk borders
         if persistent:
