@@ -545,6 +545,27 @@ def test_calls_on_two_streams_at_once(yar, torch):
         assert torch.equal(o, want)
 
 
+def test_prompts_on_two_streams_at_once(yar, torch):
+    """More pieces of work than SMs on either stream, and decode calls between them."""
+    ns, before = [1 + 9 * i % 130 for i in range(40)], [17 * i % 400 for i in range(40)]
+    c = Cache(torch, [n + b for n, b in zip(ns, before)], 8, 64, 16, seed=14)
+    offs = torch.tensor(np.concatenate([[0], np.cumsum(ns)]), dtype=torch.int32, device="cuda")
+    q, _ = queries(torch, int(offs[-1]), 16, 64, 4)
+    one = q[:40].contiguous()
+    want = yar.kv_attn_prefill(c.pool, 1, c.table, c.lengths, offs, q), yar.kv_attn_decode(c.pool, 1, c.table, c.lengths, one)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    for _ in range(10):
+        for s in streams:
+            with torch.cuda.stream(s):
+                outs.append((yar.kv_attn_prefill(c.pool, 1, c.table, c.lengths, offs, q),
+                             yar.kv_attn_decode(c.pool, 1, c.table, c.lengths, one)))
+    torch.cuda.synchronize()
+    for got in outs:
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def test_offsets_beyond_32_bits(yar, torch):
     """A pool of 2.7 billion values (5.4 GB), used at its end: attention, copies and compaction."""
     kv, dim, page, pages = 8, 128, 64, 20600
