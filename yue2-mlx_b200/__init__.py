@@ -560,7 +560,7 @@ def _kv_heads(t, name: str, dim: int) -> int:
 
 
 def _kv_attn(pool, layer, page_table, lengths, q, out, window, sinks, scale, error):
-    """(the yar_kv_attn record, out) of a call. The checks on contiguous tensors go first and in
+    """(the yar_kv_attn record, out, the shapes of pool, q and page_table) of a call. The checks on contiguous tensors go first and in
     one expression (a small call is as long as its host side); others are looked at one by one."""
     torch = sys.modules["torch"]
     ps, qs, ts = pool.shape, q.shape, page_table.shape
@@ -584,7 +584,7 @@ def _kv_attn(pool, layer, page_table, lengths, q, out, window, sinks, scale, err
         return _kv_attn_bytes(pool.data_ptr(), ps[0], ps[1], ps[3], ps[4], ps[5], page_table.data_ptr(), table_stride,
                               lengths.data_ptr(), ts[0], ts[1], layer, qs[1], q.data_ptr(), q_stride, out.data_ptr(),
                               out_stride, window, sinks, ps[5] ** -0.5 if scale is None else scale,
-                              0 if error is None else _kv_error(error)), out
+                              0 if error is None else _kv_error(error)), out, ps, qs, ts
     except struct.error as e:
         raise ValueError(f"layer, window, sinks or scale: {e}") from None
 
@@ -613,18 +613,16 @@ def kv_attn_decode(pool, layer: int, page_table, lengths, q, out=None, window: i
     ``window``/``sinks``: only the last ``window`` positions and the first ``sinks`` are visible
     (0: all). ``scale`` defaults to dim ** -0.5, ``stream`` to torch's current one, ``workspace``
     (any tensor of ``kv_attn_decode_workspace`` bytes) to fresh memory where rows are long."""
-    call, out = _kv_attn(pool, layer, page_table, lengths, q, out, window, sinks, scale, error)
-    rows, per_row = page_table.shape
-    if q.shape[0] != rows:
+    call, out, ps, qs, ts = _kv_attn(pool, layer, page_table, lengths, q, out, window, sinks, scale, error)
+    if qs[0] != ts[0]:
         raise ValueError("q and out need one row for each row of page_table")
     w, wb = None, 0
     if workspace is not None:
         if not workspace.is_contiguous():
             raise ValueError("workspace must be contiguous")
         w, wb = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    elif stream is None and rows * pool.shape[3] <= 74 and (max_length or per_row * pool.shape[4]) > 4096 and \
-            not 0 < window < 4096:
-        wb = kv_attn_decode_workspace(q.shape[1], pool.shape[3], q.shape[2])
+    elif stream is None and (max_length or ts[1] * ps[4]) > 4096 and ts[0] * ps[3] <= 74 and not 0 < window < 4096:
+        wb = kv_attn_decode_workspace(qs[1], ps[3], qs[2])
         workspace = q.new_empty((wb // 2,))
         w = workspace.data_ptr()
     _check(lib.yar_kv_attn_decode(call, max_length, w, wb, _kv_stream(q, stream)))
@@ -637,9 +635,8 @@ def kv_attn_prefill(pool, layer: int, page_table, lengths, offsets, q, out=None,
     lengths[r] cached positions) over its paged cache (yar_kv_attn_prefill); the other
     arguments as ``kv_attn_decode``'s. A result allocated here is undefined outside the rows'
     queries."""
-    call, out = _kv_attn(pool, layer, page_table, lengths, q, out, window, sinks, scale, error)
-    _check(lib.yar_kv_attn_prefill(call, _kv_int32(offsets, "offsets", page_table.shape[0] + 1), q.shape[0],
-                                   _kv_stream(q, stream)))
+    call, out, _, qs, ts = _kv_attn(pool, layer, page_table, lengths, q, out, window, sinks, scale, error)
+    _check(lib.yar_kv_attn_prefill(call, _kv_int32(offsets, "offsets", ts[0] + 1), qs[0], _kv_stream(q, stream)))
     return out
 
 
