@@ -1,0 +1,118 @@
+"""The paged-cache operators where calls are not alike: page tables wider than their rows, streams
+other than the tensors' own, offsets that are wrong, weights that one key dominates, captured calls
+on two streams. Against the definition in 64 bits, with the tolerance derived in
+test_gpu_kv_ops.py."""
+import numpy as np
+import pytest
+
+from tests.conftest import load_package
+from tests.test_gpu_kv_ops import P_ROUND, Cache, queries
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def yar():
+    return load_package()
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch
+    return torch
+
+
+def definition(torch, c, q64, row, first, scale, window, sinks, round_p):
+    """(result, tolerance) [n][heads][dim] of a row's queries at positions first, first + 1, ..: what
+    Cache.attend gives for one query, for all of them at once."""
+    n, heads, dim = q64.shape
+    dev = lambda x: torch.from_numpy(np.ascontiguousarray(x)).cuda()  # noqa: E731
+    group = heads // c.kv
+    q, k, v = dev(q64), dev(c.k[row]), dev(c.v[row])
+    k, v = (x.repeat_interleave(group, 0) for x in (k, v))  # [heads][positions][dim]
+    pos = first + torch.arange(n, device="cuda")[:, None]
+    j = torch.arange(c.lens[row], device="cuda")[None]
+    seen = j <= pos
+    if window:
+        seen &= (j < sinks) | (j > pos - window)
+    seen = seen[:, None]
+    none = ~seen.any(-1, keepdim=True)
+    s = torch.einsum("nhd,hjd->nhj", q, k) * scale
+    s = torch.where(seen, s, -torch.inf)
+    big = torch.where(seen, torch.einsum("nhd,hjd->nhj", q.abs(), k.abs()) * scale, 0.0).amax(-1, keepdim=True)
+    p = torch.where(none, 0.0, torch.exp(s - torch.where(none, 0.0, s.amax(-1, keepdim=True))))
+    p = p / torch.where(none, 1.0, p.sum(-1, keepdim=True))
+    out, a = torch.einsum("nhj,hjd->nhd", p, v), torch.einsum("nhj,hjd->nhd", p, v.abs())
+    off = torch.expm1(4 * (dim + 6) * 2.0 ** -24 * big) + 2.0 ** -18 + round_p
+    return out, torch.where(none, 0.0, off * a * (1 + 2.0 ** -8) + 2.0 ** -8 * out.abs() + 1e-30)
+
+
+def check(torch, got, want, tol):
+    assert torch.isfinite(got).all()
+    bad = (got.double() - want).abs() > tol
+    assert not bad.any(), (int(bad.sum()), bad.nonzero()[:3].tolist())
+
+
+def widened(torch, c, positions):
+    """The cache's page table with room for `positions` positions a row: entries that no call may
+    read point outside of the pool."""
+    rows, per = c.table.shape
+    table = torch.full((rows, max(per, positions // c.page)), 1 << 30, dtype=torch.int32, device="cuda")
+    table[:, :per] = c.table
+    return table
+
+
+def prompts(yar, torch, ns, before, kv, group, dim, page, positions, window=0, sinks=0, repeats=4):
+    """A batch of prompts in a table of `positions` positions a row: every query against the
+    definition, and the same bits from a cold L2, from other memory and again."""
+    c = Cache(torch, [n + b for n, b in zip(ns, before)], kv, dim, page, seed=ns[0] + dim, window=window, sinks=sinks,
+              first_pos=before)
+    table = widened(torch, c, positions)
+    offs = np.concatenate([[0], np.cumsum(ns)])
+    q, q64 = queries(torch, int(offs[-1]), kv * group, dim, ns[0])
+    d_offs = torch.tensor(offs, dtype=torch.int32, device="cuda")
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    cold = torch.empty(192 << 20, dtype=torch.uint8, device="cuda")  # larger than the L2
+    first = None
+    for i in range(repeats):
+        mine = q.clone()
+        cold.fill_(i)
+        got = yar.kv_attn_prefill(c.pool, 1, table, c.lengths, d_offs, mine, window=window, sinks=sinks, error=err)
+        if first is None:
+            first = got
+            for r, (n, b) in enumerate(zip(ns, before)):
+                if n:
+                    want, tol = definition(torch, c, q64[offs[r]:offs[r + 1]], r, b, dim ** -0.5, window, sinks,
+                                           P_ROUND["prefill"])
+                    check(torch, got[offs[r]:offs[r + 1]], want, tol)
+        assert torch.equal(got, first)
+    assert err.item() == 0
+
+
+HEADS = [(2, 1, 64), (2, 2, 64), (2, 4, 64), (2, 8, 64), (2, 16, 64), (2, 3, 64), (2, 1, 128), (2, 2, 128), (2, 4, 128),
+         (2, 8, 128), (2, 16, 128), (2, 3, 128), (8, 2, 128)]
+
+
+@pytest.mark.parametrize("kv,group,dim", HEADS)
+@pytest.mark.parametrize("positions", [1024, 4096])
+def test_short_prompts_in_wide_tables(yar, torch, kv, group, dim, positions):
+    """The split along the keys follows the table's width: most blocks of a cluster have no key
+    of such a prompt, or keys that one half of the block's queries does not see."""
+    for n in (1, 40, 64, 100, 200, 512):
+        prompts(yar, torch, [n], [0], kv, group, dim, 64, positions)
+
+
+@pytest.mark.parametrize("n,window,sinks", [(640, 0, 0), (1000, 0, 0), (1184, 0, 0), (700, 1000, 4), (1024, 1000, 4),
+                                            (1024, 640, 70)])
+@pytest.mark.parametrize("page,positions", [(64, 0), (256, 4096)])
+def test_first_chunks_of_a_prompt(yar, torch, n, window, sinks, page, positions):
+    prompts(yar, torch, [n], [0], 8, 2, 128, page, positions, window, sinks)
+
+
+@pytest.mark.parametrize("ns,before", [([1, 1300], [0, 0]), ([64, 1], [0, 1400]), ([3, 5, 40], [0, 2000, 0]),
+                                       ([0, 1, 130], [0, 0, 1500]), ([127, 128, 129], [1, 0, 1500])])
+@pytest.mark.parametrize("kv,group,dim", [(2, 1, 64), (2, 2, 128), (1, 16, 128), (2, 3, 128)])
+def test_short_rows_beside_long_ones(yar, torch, ns, before, kv, group, dim):
+    for positions in (0, 4096):
+        prompts(yar, torch, ns, before, kv, group, dim, 32, positions)
+    prompts(yar, torch, ns, before, kv, group, dim, 32, 4096, window=1300, sinks=5)

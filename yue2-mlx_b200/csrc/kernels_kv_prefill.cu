@@ -957,7 +957,10 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         // The cluster's states of a row weighted by 2^(m - M); block r finishes columns
         // [r D / C, (r + 1) D / C): the others send it theirs ([sender][4 columns][M row], 16 bytes
         // each) into its ring, which no copy or product uses any more.
-        // (m and l go where the tile's Q was: its products are complete, and there is no next item.)
+        // m and l go where the tile's Q was: there is no next item, and its products are complete. A
+        // tile that no key of this block's share concerns had none: its Q, which a copy brings whatever
+        // the share holds, has to be there before it is written over.
+        if (x.q_boxes && n_s == n_s0 && !pre_wait(&q_ready[wg], unsigned(item) & 1u, s_state)) failed = true;
         float2 *ml = reinterpret_cast<float2 *>(sm + wg * Cfg::kQ) + t;
         *ml = make_float2(row_m, row_l);
         pre_cluster_sync();
