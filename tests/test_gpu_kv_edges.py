@@ -116,3 +116,45 @@ def test_short_rows_beside_long_ones(yar, torch, ns, before, kv, group, dim):
     for positions in (0, 4096):
         prompts(yar, torch, ns, before, kv, group, dim, 32, positions)
     prompts(yar, torch, ns, before, kv, group, dim, 32, 4096, window=1300, sinks=5)
+
+
+def memory_of(torch, t):
+    """The stream whose memory the allocator made the tensor's storage."""
+    at = t.data_ptr()
+    for s in torch.cuda.memory_snapshot():
+        if s["address"] <= at < s["address"] + s["total_size"]:
+            return s["stream"]
+    raise AssertionError("not the allocator's memory")
+
+
+def test_results_on_a_given_stream_are_its_memory(yar, torch):
+    """What a call allocates belongs to the stream that writes it; ones that the caller brings are
+    used as they are, and without a stream the current one's memory is taken."""
+    c = Cache(torch, [700, 90], 2, 64, 16, seed=23)
+    q, _ = queries(torch, 2, 4, 64, 6)
+    wide = torch.cat([q, q], dim=1)[:, :4]  # (rows that are not contiguous to each other)
+    offs = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+    counts = torch.tensor([44, 6], dtype=torch.int32, device="cuda")
+    side = torch.cuda.Stream()
+    want = yar.kv_attn_decode(c.pool, 1, c.table, c.lengths, q), yar.kv_attn_prefill(c.pool, 1, c.table, c.lengths, offs, q)
+    torch.cuda.synchronize()
+    here = memory_of(torch, q)
+    for stream, home in ((side.cuda_stream, side.cuda_stream), (None, here), (0, 0),
+                         (torch.cuda.current_stream().cuda_stream, here)):
+        for x in (q, wide):
+            a = yar.kv_attn_decode(c.pool, 1, c.table, c.lengths, x, stream=stream)
+            b = yar.kv_attn_prefill(c.pool, 1, c.table, c.lengths, offs, x, stream=stream)
+            torch.cuda.synchronize()
+            assert torch.equal(a, want[0]) and torch.equal(b, want[1])
+            assert memory_of(torch, a) == memory_of(torch, b) == home
+        pool = c.pool.clone()
+        torch.cuda.synchronize()
+        table, remap, used = yar.kv_compact(pool, c.table, counts, stream=stream)
+        torch.cuda.synchronize()
+        assert used.item() == 50 and {memory_of(torch, t) for t in (table, remap, used)} == {home}
+        assert torch.equal(yar.kv_attn_decode(pool, 1, table, c.lengths, q), want[0])
+    mine = torch.empty_like(q)
+    torch.cuda.synchronize()
+    assert yar.kv_attn_decode(c.pool, 1, c.table, c.lengths, q, out=mine, stream=side.cuda_stream) is mine
+    side.synchronize()
+    assert torch.equal(mine, want[0])

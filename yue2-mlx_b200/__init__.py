@@ -559,7 +559,21 @@ def _kv_heads(t, name: str, dim: int) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1] * dim
 
 
-def _kv_attn(pool, layer, page_table, lengths, q, out, window, sinks, scale, error):
+def _kv_new(t, stream, make):
+    """make(), whose memory is the allocator's for the stream that the call runs on: memory of another
+    stream could still be in use there, and be handed out again there before this call is over."""
+    if stream is None:
+        return make()
+    torch = sys.modules["torch"]
+    raw = getattr(stream, "value", stream) or 0  # (a c_void_p, or a number)
+    if raw == torch._C._cuda_getCurrentRawStream(t.get_device()):
+        return make()
+    with torch.cuda.stream(torch.cuda.default_stream(t.device) if raw in (0, 1) else
+                           torch.cuda.ExternalStream(raw, device=t.device)):
+        return make()
+
+
+def _kv_attn(pool, layer, page_table, lengths, q, out, window, sinks, scale, error, stream):
     """(the yar_kv_attn record, out, the shapes of pool, q and page_table) of a call. The checks on contiguous tensors go first and in
     one expression (a small call is as long as its host side); others are looked at one by one."""
     torch = sys.modules["torch"]
@@ -569,14 +583,14 @@ def _kv_attn(pool, layer, page_table, lengths, q, out, window, sinks, scale, err
             and lengths.dim() == 1 and lengths.shape[0] >= ts[0] \
             and pool.is_contiguous() and q.is_contiguous() and page_table.is_contiguous() and lengths.is_contiguous() \
             and pool.is_cuda and q.is_cuda and page_table.is_cuda and lengths.is_cuda:
-        out = torch.empty_like(q)
+        out = torch.empty_like(q) if stream is None else _kv_new(q, stream, lambda: torch.empty_like(q))
         q_stride = out_stride = qs[1] * qs[2]
         table_stride = ts[1]
     else:
         _kv_pool(pool)
         table_stride = _kv_rows(page_table, lengths).table_stride
         q_stride = _kv_heads(q, "q", ps[5])
-        out = q.new_empty(qs) if out is None else out
+        out = _kv_new(q, stream, lambda: q.new_empty(qs)) if out is None else out
         out_stride = _kv_heads(out, "out", ps[5])
         if out.shape != qs:
             raise ValueError("out must have q's shape")
@@ -611,9 +625,12 @@ def kv_attn_decode(pool, layer: int, page_table, lengths, q, out=None, window: i
     """Attention of one token per row over its paged cache (yar_kv_attn_decode): q and the
     result [rows][heads][dim] BF16, page_table [rows][pages_per_row] and lengths [rows] int32.
     ``window``/``sinks``: only the last ``window`` positions and the first ``sinks`` are visible
-    (0: all). ``scale`` defaults to dim ** -0.5, ``stream`` to torch's current one, ``workspace``
-    (any tensor of ``kv_attn_decode_workspace`` bytes) to fresh memory where rows are long."""
-    call, out, ps, qs, ts = _kv_attn(pool, layer, page_table, lengths, q, out, window, sinks, scale, error)
+    (0: all). ``scale`` defaults to dim ** -0.5, ``workspace`` (any tensor of
+    ``kv_attn_decode_workspace`` bytes) to fresh memory where rows are long and no ``stream`` is
+    given. ``stream`` (a cudaStream_t's number) defaults to torch's current one; on another one
+    the caller orders the call against the streams that its tensors are made, read and freed on,
+    as for any work there. A result allocated here is that stream's memory."""
+    call, out, ps, qs, ts = _kv_attn(pool, layer, page_table, lengths, q, out, window, sinks, scale, error, stream)
     if qs[0] != ts[0]:
         raise ValueError("q and out need one row for each row of page_table")
     w, wb = None, 0
@@ -635,7 +652,7 @@ def kv_attn_prefill(pool, layer: int, page_table, lengths, offsets, q, out=None,
     lengths[r] cached positions) over its paged cache (yar_kv_attn_prefill); the other
     arguments as ``kv_attn_decode``'s. A result allocated here is undefined outside the rows'
     queries."""
-    call, out, _, qs, ts = _kv_attn(pool, layer, page_table, lengths, q, out, window, sinks, scale, error)
+    call, out, _, qs, ts = _kv_attn(pool, layer, page_table, lengths, q, out, window, sinks, scale, error, stream)
     _check(lib.yar_kv_attn_prefill(call, _kv_int32(offsets, "offsets", ts[0] + 1), qs[0], _kv_stream(q, stream)))
     return out
 
@@ -654,11 +671,12 @@ def kv_copy_pages(pool, src, dst, tokens=None, dst_pool=None, stream=None):
 
 def kv_compact(pool, page_table, counts, out=None, error=None, stream=None):
     """Move the used pages to the front of the pool (yar_kv_compact). Returns (the renamed
-    table, remap [pages]: each page's new index or -1, used [1]); ``out`` may be ``page_table``."""
+    table, remap [pages]: each page's new index or -1, used [1]); ``out`` may be ``page_table``.
+    ``stream`` as for ``kv_attn_decode``: the results and the scratch behind them are its memory."""
     c_pool, rows = _kv_pool(pool), _kv_rows(page_table, counts)
     if out is None:
-        out = sys.modules["torch"].empty_like(page_table) if page_table.is_contiguous() else \
-            page_table.new_empty(page_table.shape)
+        out = _kv_new(page_table, stream, lambda: sys.modules["torch"].empty_like(page_table)
+                      if page_table.is_contiguous() else page_table.new_empty(page_table.shape))
         new, new_stride = out.data_ptr(), rows.pages_per_row
     else:
         if out.shape != page_table.shape:
@@ -666,7 +684,7 @@ def kv_compact(pool, page_table, counts, out=None, error=None, stream=None):
         r = _kv_rows(out, counts)
         new, new_stride = r.page_table, r.table_stride
     n = c_pool.pages
-    buf = page_table.new_empty((3 * n + 2,))  # remap [n], used [1], scratch [1 + 2 n]
+    buf = _kv_new(page_table, stream, lambda: page_table.new_empty((3 * n + 2,)))  # remap [n], used [1], scratch [1 + 2 n]
     at = buf.data_ptr()
     _check(lib.yar_kv_compact(c_pool, rows.page_table, rows.table_stride, rows.rows, rows.pages_per_row, rows.lengths,
                               new, new_stride, at, at + 4 * n, at + 4 * n + 4, _kv_error(error),
