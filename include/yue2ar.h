@@ -248,7 +248,8 @@ int yar_session_set_window(yar_session *session, int window, int sinks);
  * copy of `src` at its present position (cache and last logits) with room for `capacity`
  * positions; full pages are shared, the one that is part full is copied, and what dst held
  * is dropped. yar_row_truncate cuts a row back to its first n positions (its logits stay
- * those of the last forward). yar_row_free gives a row's pages back; it needs yar_row_reset
+ * those of the last forward); refused where released pages would be seen again or n lies
+ * inside one. yar_row_free gives a row's pages back; it needs yar_row_reset
  * or a fork before it is used again. yar_row_release gives back the pages that no later
  * query of the row can see through the session's window (`released`: how many; may be
  * NULL). A call that would need more pages than the pool has left changes nothing

@@ -42,3 +42,30 @@ def test_a_windowed_first_chunk_caches_what_an_unwindowed_one_does(model, n, win
     for a, b in zip(got[1][:2], got[0][:2]):  # [kv_heads][positions][dim]
         assert max(rel_l2(a[:, i], b[:, i]) for i in range(n)) <= REL
     assert rel_l2(got[1][2], got[0][2]) <= REL
+
+
+def test_no_way_back_into_a_released_page(yar, model):
+    """Under a window of one position a row may go back to the start of a released page, not into
+    one: its lost positions would be there again for a wider window."""
+    s = model.session(max_rows=1, max_ctx=128, page_tokens=16)
+    s.set_window(1)
+    s.reset(0, 64)
+    s.prefill(0, ids(1, 40), phase=None)
+    assert s.release(0) == 2  # positions 0..31
+    for n in (5, 17, 31):
+        with pytest.raises(yar.YarError) as e:
+            s.truncate(0, n)
+        assert "released" in e.value.message
+    assert s.position(0) == 40
+    s.truncate(0, 35)
+    for w in (0, 2):
+        with pytest.raises(yar.YarError):
+            s.set_window(w)  # pages are missing still
+    s.truncate(0, 0)  # nothing is left to be seen: every page is the row's own again
+    s.set_window(0)
+    s.prefill(0, ids(2, 40), phase=None)
+    again = s.logits(0, None)
+    s.reset(0, 64)
+    s.prefill(0, ids(2, 40), phase=None)
+    np.testing.assert_array_equal(again, s.logits(0, None))
+    s.close()

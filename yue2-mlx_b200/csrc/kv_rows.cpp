@@ -108,6 +108,9 @@ void row_truncate(Session &s, int row, int n) {
     if (pages[i] < 0 && (s.attn_window == 0 || a < s.attn_sinks || b - 1 > n - s.attn_window))
       throw Error("ValueError", "positions that the row would see again have been released");
   }
+  // (A window of one position sees none of them; the page would count as whole from then on.)
+  if (n % P && pages[size_t(n / P)] < 0)
+    throw Error("ValueError", "the page that the row would go on in has been released");
   // Pages to be written from now on must be the row's own: shared ones are replaced (the one
   // that n falls into keeps its first n % P positions).
   int fresh = 0;
