@@ -241,8 +241,8 @@ int yar_row_hidden(yar_session *session, int row, int slot, uint16_t *out, int n
 /* Sliding-window attention for every row of the session (no counterpart in the reference):
  * from now on the query at position p sees the last `window` positions, its own included,
  * and the row's first `sinks` (window 0: everything, the default). It holds for prefill and
- * every decode path. One GPU only. Refused while a row has released pages that the new
- * window would need. */
+ * every decode path. Both are at most the session's max_ctx. One GPU only. While a row holds
+ * a gap of released pages only a window and sinks that are no larger are taken. */
 int yar_session_set_window(yar_session *session, int window, int sinks);
 /* Rows as lists of cache pages (no counterpart in the reference). yar_row_fork makes `dst` a
  * copy of `src` at its present position (cache and last logits) with room for `capacity`

@@ -205,7 +205,8 @@ void session_set_window(Session &s, int window, int sinks) {
     throw Error("ValueError", "window and sinks must be in [0, " + std::to_string(s.max_ctx) + "]");
   if (s.m->tp_world > 1) throw Error("ValueError", "a sliding window needs a model on one GPU");
   if (window == 0) sinks = 0;
-  // Rows whose pages were released behind the window cannot see more than they did.
+  // Rows whose pages were released behind the window cannot see more than they did. (Whether this row at
+  // this position would is not asked: the answer would change from step to step.)
   const bool wider = window == 0 || window > s.attn_window || sinks > s.attn_sinks;
   if (s.attn_window > 0 && wider)
     for (const auto &pages : s.row_pages)
