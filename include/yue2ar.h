@@ -310,7 +310,8 @@ int yar_sample_device_noalloc(yar_model *model, const uint16_t *logits, int64_t 
 enum {
   YAR_KV_BAD_PAGE = 1,    /* a page index outside the pool among the positions a query sees */
   YAR_KV_BAD_LENGTH = 2,  /* a length (count) beyond pages_per_row pages: cut to that */
-  YAR_KV_BAD_OFFSETS = 4, /* query offsets that decrease or pass n_queries: that row is skipped */
+  YAR_KV_BAD_OFFSETS = 4, /* query offsets that decrease or pass n_queries: that row is skipped, and so are
+                           * the rows behind it that start before an earlier offset */
   YAR_KV_EXPIRED = 64     /* a wait inside a kernel ran out: the outputs are not valid */
 };
 

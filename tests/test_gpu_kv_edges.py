@@ -158,3 +158,36 @@ def test_results_on_a_given_stream_are_its_memory(yar, torch):
     assert yar.kv_attn_decode(c.pool, 1, c.table, c.lengths, q, out=mine, stream=side.cuda_stream) is mine
     side.synchronize()
     assert torch.equal(mine, want[0])
+
+
+def offsets_case(rows, wrong):
+    offs = [3 * i for i in range(rows + 1)]
+    for at, value in wrong.items():
+        offs[at] = value
+    return offs
+
+
+@pytest.mark.parametrize("offs", [[0, 60, 0, 60], [0, 5, 3, 8, 8, 12], [9, 70, 70, 2, 20, 60], [-4, 10, 12], [0, 99, 5, 20],
+                                  offsets_case(150, {3: 200, 4: 3}), offsets_case(300, {140: 1, 141: 2}),
+                                  offsets_case(300, {127: -1, 200: 901}), offsets_case(400, {131: 1200, 390: 100})])
+@pytest.mark.parametrize("group", [2, 3])
+def test_rows_behind_wrong_offsets(yar, torch, offs, group):
+    """A row is skipped when its offsets are wrong or it starts before an earlier offset; every other
+    row has its result, and no query that belongs to none is written."""
+    rows, n = len(offs) - 1, 75 if len(offs) < 10 else 3 * (len(offs) - 1)
+    c = Cache(torch, [100] * rows, 2, 64, 32, seed=rows)
+    q, q64 = queries(torch, n, 2 * group, 64, rows)
+    out = torch.full_like(q, 7.0)
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    yar.kv_attn_prefill(c.pool, 1, c.table, c.lengths, torch.tensor(offs, dtype=torch.int32, device="cuda"), q, out=out,
+                        error=err)
+    assert err.item() == 4
+    written = torch.zeros(n, dtype=torch.bool, device="cuda")
+    for r, (a, b) in enumerate(zip(offs, offs[1:])):
+        if not 0 <= a <= b <= n or a < max(offs[:r + 1]):
+            continue
+        assert not written[a:b].any()
+        written[a:b] = True
+        want, tol = definition(torch, c, q64[a:b], r, 100 - (b - a), 64 ** -0.5, 0, 0, P_ROUND["prefill"])
+        check(torch, out[a:b], want, tol)
+    assert (out[~written] == 7).all()

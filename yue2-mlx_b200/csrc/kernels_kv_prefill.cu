@@ -400,7 +400,8 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         row = 0, n = p.n_queries, pair = slot;
         if ((long long)pair * 256 >= (long long)n * G) row = -1;
       } else {
-        int before = 0;
+        int before = 0, most = 0;
+        bool wrong = false;
         for (int r0 = 0; r0 < p.rows && row < 0; r0 += 128) {  // four rows a lane: one latency for 128
           int f[5], k[4], l[4], mine = 0;
 #pragma unroll
@@ -413,11 +414,34 @@ __global__ void __launch_bounds__(kPreThreads, 1)
             if (r0 + lane * 4 + i < p.rows) {
               if (f[i] >= 0 && f[i + 1] >= f[i] && f[i + 1] <= p.n_queries)
                 k[i] = f[i + 1] - f[i];
-              else if (p.error)
-                atomicOr(p.error, kKvBadOffsets);
+              else
+                k[i] = -1;
             }
-            mine += int(((long long)k[i] * G + 255) / 256);
           }
+          const bool bad = (k[0] | k[1] | k[2] | k[3]) < 0;
+          if (bad && p.error) atomicOr(p.error, kKvBadOffsets);
+          // Behind a wrong offset rows could overlap (two blocks would write the same queries, and
+          // the bound on the blocks not hold): those that start before an earlier offset are skipped.
+          if (wrong || __any_sync(0xFFFFFFFFu, bad)) {
+            if (!wrong) most = __shfl_sync(0xFFFFFFFFu, f[0], 0);  // (up to here they ascended)
+            wrong = true;
+            int top = max(max(f[0], f[1]), max(f[2], f[3]));
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+              const int v = __shfl_up_sync(0xFFFFFFFFu, top, o);
+              if (lane >= o) top = max(top, v);
+            }
+            int over = __shfl_up_sync(0xFFFFFFFFu, top, 1);
+            over = lane == 0 ? most : max(over, most);
+            most = max(most, __shfl_sync(0xFFFFFFFFu, top, 31));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              k[i] = f[i] < over ? 0 : max(k[i], 0);
+              over = max(over, f[i]);
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mine += int(((long long)k[i] * G + 255) / 256);
           int incl = mine;
 #pragma unroll
           for (int o = 1; o < 32; o <<= 1) {
