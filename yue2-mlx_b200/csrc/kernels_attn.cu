@@ -291,6 +291,7 @@ static KvAttnParams paged_params(const Model &m, const Session &s, const AttnGeo
   a.window = s.attn_window, a.sinks = s.attn_sinks;
   a.scale = g.scale;
   a.error = s.d_error;
+  a.error_shift = kKvSessionShift;
   return a;
 }
 

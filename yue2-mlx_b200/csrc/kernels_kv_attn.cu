@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(32 * W, 8 / W) k_kv_attn_decode(const __grid_c
     for (int i = lane * 32; i < p.pages_per_row; i += 1024) asm volatile("prefetch.global.L2 [%0];" ::"l"(tab + i));
   int len = p.lengths[row];
   if (len > cap) {
-    if (rank == 0 && kvh == 0 && tid == 0 && p.error) atomicOr(p.error, kKvBadLength);
+    if (rank == 0 && kvh == 0 && tid == 0 && p.error) atomicOr(p.error, kKvBadLength << p.error_shift);
     len = cap;
   }
   // The visible positions in order: [0, sinks), then [lo, len).
@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(32 * W, 8 / W) k_kv_attn_decode(const __grid_c
     __syncwarp();
   }
 
-  if (bad && p.error) atomicOr(p.error, kKvBadPage);
+  if (bad && p.error) atomicOr(p.error, kKvBadPage << p.error_shift);
   // Join the warps, then the cluster's blocks: each state weighted by 2^(m - M).
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();  // every warp is done with its ring

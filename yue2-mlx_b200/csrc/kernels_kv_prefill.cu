@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         bad = bad || page < 0 || page >= p.pages;
       }
     }
-    if (bad && p.error) atomicOr(p.error, kKvBadPage);
+    if (bad && p.error) atomicOr(p.error, kKvBadPage << p.error_shift);
     return bad;
   };
 
@@ -419,7 +419,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
             }
           }
           const bool bad = (k[0] | k[1] | k[2] | k[3]) < 0;
-          if (bad && p.error) atomicOr(p.error, kKvBadOffsets);
+          if (bad && p.error) atomicOr(p.error, kKvBadOffsets << p.error_shift);
           // Behind a wrong offset rows could overlap (two blocks would write the same queries, and
           // the bound on the blocks not hold): those that start before an earlier offset are skipped.
           if (wrong || __any_sync(0xFFFFFFFFu, bad)) {
@@ -470,7 +470,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       b.row = row, b.first = first, b.n = n;
       const int cap = p.pages_per_row << p.page_shift;
       if (len > cap) {
-        if (p.error && lane == 0) atomicOr(p.error, kKvBadLength);
+        if (p.error && lane == 0) atomicOr(p.error, kKvBadLength << p.error_shift);
         len = cap;
       }
       b.len = max(len, 0);
@@ -583,7 +583,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       for (int i = issued > NST ? issued - NST : 0; i < issued; ++i)
         at_wait(&kv_full[i % NST], unsigned(i / NST) & 1u);
       if (claims > 0) at_wait(&claim_done, unsigned(claims - 1) & 1u);
-      if (lane == 0 && p.error) atomicOr(p.error, kKvExpired);
+      if (lane == 0 && p.error) atomicOr(p.error, kKvExpired << p.error_shift);
     }
   } else if (warp < 10) {
     // ---- products of tile X = A (warp 8) or B (warp 9) ---------------------------------------
@@ -700,7 +700,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
     __syncwarp();
     if (!at_wait(&drain[X], 0u) || !ok) {
       s_state[0] = 1;
-      if (lane == 0 && p.error) atomicOr(p.error, kKvExpired);
+      if (lane == 0 && p.error) atomicOr(p.error, kKvExpired << p.error_shift);
     }
   }
   if (warp == 11) {
@@ -749,7 +749,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       if (boxes[X]) at_wait(&q_ready[X], unsigned(boxes[X] - 1) & 1u);
     if (!ok) {
       s_state[0] = 1;
-      if (lane == 0 && p.error) atomicOr(p.error, kKvExpired);
+      if (lane == 0 && p.error) atomicOr(p.error, kKvExpired << p.error_shift);
     }
   }
   if (C > 1) {  // (the softmax warps' two exchanges)
@@ -1053,7 +1053,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
     }
     if (!ok) {
       s_state[0] = 1;
-      if (lane == 0 && p.error) atomicOr(p.error, kKvExpired);
+      if (lane == 0 && p.error) atomicOr(p.error, kKvExpired << p.error_shift);
     }
     if (C > 1 && !syncs) {  // every thread of a cluster takes its two exchanges
       pre_cluster_sync();

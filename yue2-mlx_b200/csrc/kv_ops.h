@@ -7,6 +7,9 @@ namespace yar {
 
 // Bits of the device error word that these operators set (include/yue2ar.h).
 constexpr int kKvBadPage = 1, kKvBadLength = 2, kKvBadOffsets = 4, kKvExpired = 64;
+// A session's word has bits of its own (1 to 64): there these stand this many places higher, so
+// that "device error flags 256" is a bad page, 512 a bad length and 16384 a wait that ran out.
+constexpr int kKvSessionShift = 8;
 constexpr int kKvMaxGroup = 16;          // query heads of one KV head
 constexpr int kKvMaxPages = 1 << 20;     // pages of a pool that can be compacted
 constexpr int kKvMaxPositions = 1 << 30;  // positions of one page table
@@ -40,6 +43,7 @@ struct KvAttnParams {
   int max_length = 0;  // decode: a bound of the lengths, for the choice of splits only (0: the table's)
   float *partials = nullptr;  // decode: workspace of kv_attn_decode_workspace bytes (may be null)
   int *error = nullptr;
+  int error_shift = 0;  // places by which the bits stand higher there
 };
 
 size_t kv_attn_decode_workspace(int heads, int kv_heads, int head_dim);
