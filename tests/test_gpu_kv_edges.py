@@ -191,3 +191,32 @@ def test_rows_behind_wrong_offsets(yar, torch, offs, group):
         want, tol = definition(torch, c, q64[a:b], r, 100 - (b - a), 64 ** -0.5, 0, 0, P_ROUND["prefill"])
         check(torch, out[a:b], want, tol)
     assert (out[~written] == 7).all()
+
+
+def test_a_short_row_in_a_very_wide_table(yar, torch):
+    """A table of 2^24 pages a row, of which the first 7 are meant, in a tensor that ends with the
+    row: the result of a narrow table, in about its time (the table is not walked)."""
+    c = Cache(torch, [100], 2, 128, 16, seed=24)
+    q, _ = queries(torch, 1, 4, 128, 7)
+    table = torch.full((1, 1 << 24), 1 << 30, dtype=torch.int32, device="cuda")
+    table[:, :c.table.shape[1]] = c.table
+
+    def call(t):
+        return yar.kv_attn_decode(c.pool, 1, t, c.lengths, q, max_length=100)
+
+    def us(t, n=50):
+        times = []
+        for _ in range(5):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            for _ in range(n):
+                call(t)
+            b.record()
+            b.synchronize()
+            times.append(a.elapsed_time(b) * 1e3 / n)
+        return min(times)
+
+    assert torch.equal(call(table), call(c.table))
+    narrow, wide = us(c.table), us(table)
+    print(f"narrow {narrow:.1f} us, wide {wide:.1f} us")
+    assert wide <= 3 * narrow + 10
