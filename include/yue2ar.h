@@ -122,8 +122,10 @@ int yar_model_dims(const yar_model *model, int64_t *dims10);
  * activations, logits, sampler state and the captured decode-step graph. */
 int yar_session_create(yar_model *model, int max_rows, int max_ctx, int page_tokens,
                        yar_session **out);
-/* The same with a pool of `pool_pages` pages (0: enough for every row's max_ctx): rows then
- * compete for them, and yar_row_reset (so yar_generate too) is refused when they run out.
+/* The same with a pool of `pool_pages` pages (0: enough for every row's max_ctx). Rows then
+ * compete for them: yar_row_reset and yar_generate are refused when they run out and change
+ * nothing then, the requests of yar_generate_batch and yar_generate_requests wait for pages
+ * that others give back, and are refused when one alone asks for more than their rows can get.
  * Rows that share pages (yar_row_fork) or give back what their window hides
  * (yar_row_release) let fewer pages serve more rows. */
 int yar_session_create_pool(yar_model *model, int max_rows, int max_ctx, int page_tokens, int pool_pages,

@@ -176,8 +176,8 @@ void row_reset(Session &s, int row, int capacity) {
   if (capacity < 1 || capacity > s.max_ctx)
     throw Error("ValueError", "KV cache capacity must be in [1, " + std::to_string(s.max_ctx) + "]");
   YAR_CUDA(cudaStreamSynchronize(s.stream));
-  const int need = (capacity + s.page_tokens - 1) / s.page_tokens;
-  if (pages_after_drop(s, row) < need) throw Error("ValueError", "KV page pool exhausted; generation was not shortened");
+  const int need = pages_for(s, capacity);
+  if (pages_after_drop(s, row) < need) throw Error("ValueError", kPagesExhausted);
   drop_pages(s, row);
   for (int i = 0; i < need; ++i) s.row_pages[row].push_back(take_page(s));
   s.capacity[row] = capacity;
@@ -590,6 +590,14 @@ std::string generate(Session &s, const int32_t *prefix, int n_prefix, const ::ya
 
   YAR_CUDA(cudaSetDevice(m.device));
   YAR_CUDA(cudaStreamSynchronize(s.stream));
+  // (Both rows' pages at once: a refusal leaves the rows as they were.)
+  if (pages_after_drop(s, 0, rows) <
+      pages_for(s, n_prefix + smp.max_tokens) + (cfg ? pages_for(s, n_negative + smp.max_tokens) : 0))
+    throw Error("ValueError", kPagesExhausted);
+  for (int r = 0; r < rows; ++r) {
+    drop_pages(s, r);
+    s.capacity[r] = s.pos[r] = 0;
+  }
   const double t0 = now_s();
   row_reset(s, 0, n_prefix + smp.max_tokens);
   row_prefill(s, 0, prefix, n_prefix, phase, 0, cancel, cancel_ctx);
@@ -793,10 +801,19 @@ std::string generate_requests(Session &s, int n_req, int slots, const int32_t *p
   YAR_CUDA(cudaSetDevice(m.device));
   cudaStream_t st = s.stream;
   YAR_CUDA(cudaStreamSynchronize(st));
+  // A request for which the pool has no pages now waits for others to end; one that the slots' rows
+  // could not hold alone is refused before anything runs.
+  const int pool = pages_after_drop(s, 0, slots);
+  for (int r = 0; r < n_req; ++r)
+    if (pages_for(s, prefix_lens[r] + smps[r].max_tokens) > pool) throw Error("ValueError", kPagesExhausted);
+  for (int row = 0; row < slots; ++row) {
+    drop_pages(s, row);
+    s.capacity[row] = s.pos[row] = 0;
+  }
   const double t0 = now_s();
   double prefill_seconds = 0;
   std::vector<int> slot_req(slots, -1);  // request on each row (-1: none)
-  int next = 0, admitted_late = 0;
+  int next = 0;
   // Prefill request r on `row` and arm its sampler record.
   auto admit = [&](int row, int r) {
     const double p0 = now_s();
@@ -810,7 +827,19 @@ std::string generate_requests(Session &s, int n_req, int slots, const int32_t *p
     YAR_CUDA(cudaStreamSynchronize(st));  // the host values above are on the stack
     slot_req[row] = r;
   };
-  for (int row = 0; row < slots; ++row) admit(row, next++);
+  // Free rows take the next requests in order, as far as there are pages.
+  auto refill = [&] {
+    for (int row = 0; row < slots && next < n_req; ++row) {
+      if (slot_req[row] >= 0) continue;
+      if (int(s.free_pages.size()) < pages_for(s, prefix_lens[next] + smps[next].max_tokens)) return;
+      admit(row, next++);
+    }
+  };
+  // Rows without a request: idle, their record one with nothing left to sample.
+  YAR_CUDA(cudaMemsetAsync(s.d_active, 0, slots * sizeof(int), st));
+  YAR_CUDA(cudaMemsetAsync(s.d_req, 0, slots * sizeof(RequestState), st));
+  refill();
+  const int first = next;
   YAR_CUDA(cudaMemsetAsync(s.d_error, 0, sizeof(int), st));
   reset_step_sync(s);
   YAR_CUDA(cudaStreamSynchronize(st));
@@ -858,11 +887,8 @@ std::string generate_requests(Session &s, int n_req, int slots, const int32_t *p
         drop_pages(s, row);
         s.capacity[row] = 0;
         slot_req[row] = -1;
-        if (next < n_req) {
-          admit(row, next++);
-          ++admitted_late;
-        }
       }
+      refill();
     }
   } catch (...) {
     cudaEventDestroy(ev0);
@@ -876,7 +902,7 @@ std::string generate_requests(Session &s, int n_req, int slots, const int32_t *p
                            {"prefill_seconds", prefill_seconds},
                            {"requests", n_req},
                            {"slots", slots},
-                           {"refills", admitted_late},
+                           {"refills", n_req - first},
                            {"content_tokens", total},
                            {"decode_steps", steps},
                            {"decode_device_ms", decode_ms},

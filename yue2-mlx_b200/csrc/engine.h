@@ -315,7 +315,9 @@ struct Session {
 void check_row(const Session &s, int row);
 int take_page(Session &s);                             // an unused page (the caller has checked that there is one)
 void drop_pages(Session &s, int row);                  // the row holds no page any more
-int pages_after_drop(const Session &s, int row);       // unused pages, the row's own included
+int pages_for(const Session &s, int capacity);         // pages that hold so many positions
+int pages_after_drop(const Session &s, int row, int rows = 1);  // unused pages, those of rows [row, row + rows) included
+extern const char *const kPagesExhausted;              // the refusal when there are too few
 void upload_row(Session &s, int row);                  // the row's table, position and capacity to the device; inactive
 void row_fork(Session &s, int src, int dst, int capacity);
 void row_truncate(Session &s, int row, int n);

@@ -10,9 +10,9 @@
 
 namespace yar {
 
-namespace {
-const char *kExhausted = "KV page pool exhausted; generation was not shortened";
+const char *const kPagesExhausted = "KV page pool exhausted; generation was not shortened";
 
+namespace {
 void drop_page(Session &s, int page) {
   if (page >= 0 && --s.page_refs[page] == 0) s.free_pages.push_back(page);
 }
@@ -47,9 +47,13 @@ void drop_pages(Session &s, int row) {
   s.row_pages[row].clear();
 }
 
-int pages_after_drop(const Session &s, int row) {
+int pages_for(const Session &s, int capacity) { return (capacity + s.page_tokens - 1) / s.page_tokens; }
+
+int pages_after_drop(const Session &s, int row, int rows) {
+  std::vector<int> theirs(s.num_pages, 0);  // of a page's references
   int n = int(s.free_pages.size());
-  for (int p : s.row_pages[row]) n += p >= 0 && s.page_refs[p] == 1;
+  for (int r = row; r < row + rows; ++r)
+    for (int p : s.row_pages[r]) n += p >= 0 && ++theirs[p] == s.page_refs[p];
   return n;
 }
 
@@ -76,8 +80,8 @@ void row_fork(Session &s, int src, int dst, int capacity) {
     throw Error("ValueError", "KV cache capacity must be in [" + std::to_string(std::max(1, n)) + ", " +
                                   std::to_string(s.max_ctx) + "]");
   begin(s);
-  const int full = n / P, need = (capacity + P - 1) / P;
-  if (pages_after_drop(s, dst) < need - full) throw Error("ValueError", kExhausted);
+  const int full = n / P, need = pages_for(s, capacity);
+  if (pages_after_drop(s, dst) < need - full) throw Error("ValueError", kPagesExhausted);
   drop_pages(s, dst);
   std::vector<int> pages(s.row_pages[src].begin(), s.row_pages[src].begin() + full);
   for (int p : pages)
@@ -115,7 +119,7 @@ void row_truncate(Session &s, int row, int n) {
   // that n falls into keeps its first n % P positions).
   int fresh = 0;
   for (size_t i = size_t(n / P); i < pages.size(); ++i) fresh += pages[i] < 0 || s.page_refs[pages[i]] > 1;
-  if (int(s.free_pages.size()) < fresh) throw Error("ValueError", kExhausted);
+  if (int(s.free_pages.size()) < fresh) throw Error("ValueError", kPagesExhausted);
   for (size_t i = size_t(n / P); i < pages.size(); ++i) {
     const int old = pages[i];
     if (old >= 0 && s.page_refs[old] == 1) continue;
