@@ -220,3 +220,19 @@ def test_a_short_row_in_a_very_wide_table(yar, torch):
     narrow, wide = us(c.table), us(table)
     print(f"narrow {narrow:.1f} us, wide {wide:.1f} us")
     assert wide <= 3 * narrow + 10
+
+
+def test_compaction_into_a_table_beside_the_old_one(yar, torch):
+    """Both tables as columns of one tensor, either side first."""
+    pool = torch.arange(8, device="cuda").view(1, 8, 1, 1, 1, 1).expand(1, 8, 2, 1, 16, 64).bfloat16().contiguous()
+    counts = torch.tensor([3, 2], dtype=torch.int32, device="cuda")
+    for old, new in ((slice(0, 3), slice(3, 6)), (slice(3, 6), slice(0, 3)), (slice(0, 3), slice(4, 7))):
+        both = torch.full((2, 7), -9, dtype=torch.int32, device="cuda")
+        both[:, old] = torch.tensor([[7, 0, 5], [3, 7, 6]], dtype=torch.int32)
+        mine = pool.clone()
+        out, remap, used = yar.kv_compact(mine, both[:, old], counts, out=both[:, new])
+        assert used.item() == 4 and both[:, new].tolist() == [[2, 0, 1], [3, 2, 6]]
+        assert both[:, old].tolist() == [[7, 0, 5], [3, 7, 6]]
+        assert mine[0, :4, 0, 0, 0, 0].tolist() == [0, 5, 7, 3]
+    with pytest.raises(yar.YarError):
+        yar.kv_compact(pool, both[:, 0:3], counts, out=both[:, 1:4])

@@ -35,3 +35,26 @@ def test_a_session_tells_the_operators_error_bits_from_its_own():
         text = open(os.path.join(CSRC, f"kernels_kv_{name}.cu")).read()
         assert re.findall(r"atomicOr\(p\.error, kKv\w+(.*?)\);", text) and not re.search(r"atomicOr\(p\.error, kKv\w+\);", text)
     assert "a.error_shift = kKvSessionShift" in open(os.path.join(CSRC, "kernels_attn.cu")).read()
+
+
+PTR = 1 << 20  # 16-byte aligned, never followed
+
+
+def test_compact_takes_tables_that_do_not_overlap(yar):
+    """Tables of 3 rows of 4 entries: refused where an entry of one is an entry of the other, and not
+    where rows only lie between each other's (the made-up pointers are refused later then)."""
+    pool = yar._KvPool(PTR, 2, 8, 2, 16, 64)
+    for stride, new_stride, first in [(8, 8, d) for d in range(-28, 29)] + [(4, 4, d) for d in range(-13, 14)] + \
+            [(9, 9, d) for d in (3, 4, 5, 6, 22, 23, -4, -5, -6)] + [(8, 5, d) for d in (19, 20, 21, -13, -14, 30)]:
+        old = {r * stride + i for r in range(3) for i in range(4)}
+        new = {first + r * new_stride + i for r in range(3) for i in range(4)}
+        at = PTR + (1 << 12)
+        status = yar.lib.yar_kv_compact(pool, at, stride, 3, 4, PTR, at + 4 * first, new_stride, PTR, PTR, PTR, None, None)
+        assert status != yar.OK
+        said = "overlaps" in yar.lib.yar_last_error().decode()
+        if first == 0 and stride == new_stride:
+            assert not said  # the same table
+        elif stride == new_stride or min(max(old), max(new)) < max(min(old), min(new)):
+            assert said == bool(old & new), (stride, first)
+        else:
+            assert said  # (strides that differ and cross)

@@ -65,6 +65,17 @@ void check_table(const KvPool &p, const int32_t *table, int64_t stride, int rows
   need(rows == 0 || (table && aligned(table, 4)), "the page table is required");
 }
 
+// Whether the entries of two tables of one shape share memory (rows of one stride may lie in each
+// other's gaps; of two strides that cross, true).
+bool tables_overlap(const int32_t *a, int64_t a_stride, const int32_t *b, int64_t b_stride, int rows, int per) {
+  if (rows == 0) return false;
+  const int64_t d = (reinterpret_cast<intptr_t>(b) - reinterpret_cast<intptr_t>(a)) / int64_t(sizeof(int32_t));
+  if (d >= (rows - 1) * a_stride + per || -d >= (rows - 1) * b_stride + per) return false;
+  if (a_stride != b_stride) return true;
+  const int64_t off = (d % a_stride + a_stride) % a_stride;  // of b's rows in a's
+  return off < per || off > a_stride - per;
+}
+
 // The one device that holds every listed pointer (null ones are skipped).
 int device_of(std::initializer_list<std::pair<const char *, const void *>> ptrs) {
   int device = -1;
@@ -215,10 +226,9 @@ void kv_compact(const ::yar_kv_pool *c_pool, const int32_t *table, int64_t table
   need(rows == 0 || (counts && aligned(counts, 4)), "counts is required");
   need(remap && used && work && aligned(remap, 4) && aligned(used, 4) && aligned(work, 4) && aligned(error, 4),
        "remap, used and work are required, 4-byte aligned");
-  if (table != new_table || table_stride != new_stride) {
-    const int32_t *ae = table + int64_t(rows) * table_stride, *be = new_table + int64_t(rows) * new_stride;
-    need(rows == 0 || ae <= new_table || be <= table, "the new table overlaps the old one: pass the same one, or another");
-  }
+  if (table != new_table || table_stride != new_stride)
+    need(!tables_overlap(table, table_stride, new_table, new_stride, rows, pages_per_row),
+         "the new table overlaps the old one: pass the same one, or another");
   const int device = device_of({{"the pool", pool.data}, {"the page table", table}, {"counts", counts},
                                 {"the new table", new_table}, {"remap", remap}, {"used", used}, {"work", work},
                                 {"error", error}});
