@@ -341,7 +341,12 @@ typedef struct yar_kv_rows {
  * of kv_heads, at most 16 for each (query head h reads KV head h / (heads / kv_heads)). The
  * query at position p sees j <= p when window is 0, else j < sinks or j > p - window (the
  * last `window` positions, its own included, and the first `sinks`). FP32 scores, statistics
- * and sums; the result is rounded once; a query that sees nothing gets zeros. */
+ * and sums. The weights meet V as two BF16 parts (2^-16) in yar_kv_attn_decode, as BF16 in
+ * yar_kv_attn_prefill: off by up to 2^-8 each, so its result by up to 2^-8 of the weighted |V|
+ * (all of it only where few keys carry the weight) on top of the rounding to BF16, which is the
+ * last step of both. A query that sees nothing, or scores of -infinity only, gets zeros.
+ * Infinities and NaN in positions that a query does not see do not reach it; a V value of that
+ * kind that it sees makes its column of the result infinite or NaN. */
 typedef struct yar_kv_attn {
   yar_kv_pool pool;
   yar_kv_rows rows;

@@ -236,3 +236,31 @@ def test_compaction_into_a_table_beside_the_old_one(yar, torch):
         assert mine[0, :4, 0, 0, 0, 0].tolist() == [0, 5, 7, 3]
     with pytest.raises(yar.YarError):
         yar.kv_compact(pool, both[:, 0:3], counts, out=both[:, 1:4])
+
+
+@pytest.mark.parametrize("dim,kv,group,n", [(128, 2, 2, 300), (64, 1, 3, 200), (128, 8, 2, 1500)])
+def test_keys_that_carry_the_weight(yar, torch, dim, kv, group, n):
+    """Every 50th key is 3 to 7 (in units of log2) above the ones before it, less than makes the
+    running maximum follow, so that the dominating weight is not a power of two: the weights' rounding
+    does not average out, and the result stays within its tolerance (one rounding of the weights, one
+    of the result)."""
+    c = Cache(torch, [n], kv, dim, 64, seed=25, spread=0.05)
+    rng = np.random.default_rng(26)
+    unit = np.sign(rng.standard_normal((kv, dim)))
+    level = 0.0
+    for j in range(0, n, 50):
+        level += 3 + 4 * rng.random()
+        # q = unit (plus noise) below, so that this key scores level x ln 2
+        k = torch.from_numpy(unit * level * np.log(2) / dim ** 0.5).bfloat16()
+        c.k[0][:, j] = k.double().numpy()
+        c.pool[1, int(c.table[0, j // 64]), 0, :, j % 64] = k.cuda()
+    noise = rng.standard_normal((n, kv * group, dim)) * 0.02
+    q = torch.from_numpy(unit.repeat(group, 0)[None] + noise).bfloat16()
+    offs = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    for window, sinks in ((0, 0), (90, 3)):
+        got = yar.kv_attn_prefill(c.pool, 1, c.table, c.lengths, offs, q.cuda(), window=window, sinks=sinks)
+        want, tol = definition(torch, c, q.double().numpy(), 0, 0, dim ** -0.5, window, sinks, P_ROUND["prefill"])
+        check(torch, got, want, tol)
+        one = yar.kv_attn_decode(c.pool, 1, c.table, c.lengths, q[-1:].cuda(), window=window, sinks=sinks)
+        want, tol = definition(torch, c, q[-1:].double().numpy(), 0, n - 1, dim ** -0.5, window, sinks, P_ROUND["decode"])
+        check(torch, one, want, tol)
