@@ -264,3 +264,80 @@ def test_keys_that_carry_the_weight(yar, torch, dim, kv, group, n):
         one = yar.kv_attn_decode(c.pool, 1, c.table, c.lengths, q[-1:].cuda(), window=window, sinks=sinks)
         want, tol = definition(torch, c, q[-1:].double().numpy(), 0, n - 1, dim ** -0.5, window, sinks, P_ROUND["decode"])
         check(torch, one, want, tol)
+
+
+@pytest.mark.parametrize("dim,window,sinks,positions", [(128, 0, 0, 0), (64, 90, 3, 0), (128, 300, 0, 0), (128, 0, 0, 4096),
+                                                        (64, 700, 5, 1024)])
+def test_queries_that_do_not_see_a_value_keep_their_results(yar, torch, dim, window, sinks, positions):
+    """Values that are not finite: in K, what does not see them keeps every bit; in V, what does not see
+    them stays within the tolerance of the definition without them (the sums are formed again, key by
+    key, beside one), in the heads that share the value's KV head too."""
+    n, heads = 400, 4
+    c = Cache(torch, [n], 2, dim, 64, seed=31)
+    table = widened(torch, c, positions)
+    q, q64 = queries(torch, n, heads, dim, 8)
+    offs = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    want, tol = definition(torch, c, q64, 0, 0, dim ** -0.5, window, sinks, P_ROUND["prefill"])
+    clean = yar.kv_attn_prefill(c.pool, 1, table, c.lengths, offs, q, window=window, sinks=sinks)
+    check(torch, clean, want, tol)
+    for at in (0, 63, 64, 130, 257, 317, 399):
+        pos = torch.arange(n, device="cuda")
+        sees = (pos >= at) & ((pos - window < at) | (at < sinks) if window else True)
+        for what, value in ((0, float("nan")), (0, float("inf")), (1, float("nan")), (1, float("-inf"))):
+            pool = c.pool.clone()
+            pool[1, int(c.table[0, at // 64]), what, 0, at % 64, 7] = value
+            got = yar.kv_attn_prefill(pool, 1, table, c.lengths, offs, q, window=window, sinks=sinks)
+            assert torch.equal(got[:, 2:], clean[:, 2:])
+            if what == 0:
+                assert torch.equal(got[~sees], clean[~sees])
+            else:
+                check(torch, got[~sees], want[~sees], tol[~sees])
+                assert not torch.isfinite(got[sees][:, :2, 7].float()).any()
+                rest = torch.arange(dim, device="cuda") != 7
+                check(torch, got[..., rest], want[..., rest], tol[..., rest])
+
+
+def test_graphs_of_all_calls_on_two_streams(yar, torch):
+    """Two graphs, each of copies, both forms of attention and compaction on a pool and buffers of its
+    own, replayed at the same time on two streams, on new queries each time; a workspace each."""
+    def make(seed, window):
+        c = Cache(torch, [6000, 150, 60], 2, 128, 64, seed=seed)
+        counts = torch.tensor([94, 3, 1], dtype=torch.int32, device="cuda")
+        return dict(c=c, counts=counts, pool=c.pool.clone(), table=torch.empty_like(c.table), window=window,
+                    q=queries(torch, 3, 4, 128, seed)[0], offs=torch.tensor([0, 1, 2, 3], dtype=torch.int32, device="cuda"),
+                    ws=torch.empty(yar.kv_attn_decode_workspace(4, 2, 128), dtype=torch.uint8, device="cuda"),
+                    pages=[int(p) for p in c.table[0, :3]],
+                    spare=sorted(set(range(c.pool.shape[1])) - set(c.table.flatten().tolist()))[:3])
+
+    def run(s):
+        c, kw = s["c"], dict(window=s["window"], sinks=2)
+        s["pool"].copy_(c.pool)
+        yar.kv_copy_pages(s["pool"], s["pages"], s["spare"], tokens=[1, 20, 64])
+        a = yar.kv_attn_decode(s["pool"], 1, c.table, c.lengths, s["q"], workspace=s["ws"], **kw)
+        b = yar.kv_attn_prefill(s["pool"], 1, c.table, c.lengths, s["offs"], a, **kw)
+        new, remap, used = yar.kv_compact(s["pool"], c.table, s["counts"], out=s["table"])
+        return a, b, yar.kv_attn_decode(s["pool"], 1, new, c.lengths, b, workspace=s["ws"], **kw), remap, used
+
+    sets = [make(41, 0), make(42, 500)]
+    for s in sets:
+        run(s)  # (first calls outside of the capture)
+    torch.cuda.synchronize()
+    graphs, outs, streams = [], [], [torch.cuda.Stream() for _ in sets]
+    for s, stream in zip(sets, streams):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            outs.append(run(s))
+        graphs.append(g)
+    for seed in range(6):
+        for s in sets:
+            s["q"].copy_(queries(torch, 3, 4, 128, 60 + seed)[0])
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for g, stream in zip(graphs, streams):
+                with torch.cuda.stream(stream):
+                    g.replay()
+        torch.cuda.synchronize()
+        for s, out in zip(sets, outs):
+            keep = [x.clone() for x in out]
+            for x, want in zip(keep, run(s)):
+                assert torch.equal(x, want)
