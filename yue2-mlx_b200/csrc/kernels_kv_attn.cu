@@ -31,10 +31,12 @@ namespace yar {
 //   is its own rounding): P's fragment is transposed in registers (movmatrix).
 // The tensor and issue work per slice is well below the time in which HBM delivers its 8 KB to
 // an SM (issue slots 40 % busy at 6.2 TB/s), which is why the plain mma.sync form suffices.
-// Measured (calls in a graph on inputs in turn): 64 rows with 2,052 visible positions 86 us (524
-// MB, 6.1 TB/s); one row of 24,000 positions 24 us with a workspace, 29 without (98 MB, 15 us at a
-// plain copy's rate: the start of the launch, the table's round trip and the join are the rest);
-// one row of 513 positions 6.8 us, of 16 4.4; 33 rows of 14 heads of 64 on pages of 16, 10.9 us.
+// Measured (calls in a graph on inputs in turn, which overlap as far as their launches let them): 64
+// rows with 2,052 visible positions 81 us (524 MB, 6.5 TB/s); one row of 24,000 positions 23 us with
+// a workspace, 29 without (98 MB, 15 us at a plain copy's rate: the start of the launch, the table's
+// round trip and the join are the rest; a launch of its own for the join, 2 us, because a last part
+// that joins would need a counter that is zero before a call, and a workspace may hold anything); one
+// row of 513 positions 5.9 us, of 16 4.4; 33 rows of 14 heads of 64 on pages of 16, 9.3 us.
 namespace {
 constexpr int kDecMaxCluster = 16;
 constexpr int dec_slice(int head_dim) { return 2048 / head_dim; }  // positions of a slice: its K and V are 8 KB

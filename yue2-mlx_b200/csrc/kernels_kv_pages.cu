@@ -3,9 +3,9 @@
 //
 // Both move bytes and nothing else, so both are bound by HBM (each byte read once and
 // written once): a block moves a contiguous run with eight 16-byte loads a thread in flight.
-// Measured: 63 pages of 28 layers (1.85 GB) 581 us = 6.37 TB/s, 97% of the measured copy
-// rate; a compaction that moves 1.15 GB 372 us = 94% (one more launch, for the plan); one
-// part of a page (15 MB) 7.7 us, two of them the launch.
+// Measured: 63 pages of 28 layers (1.85 GB) 579 us = 6.39 TB/s, 98% of the measured copy
+// rate; a compaction that moves 1.15 GB 371 us = 94% captured, 370 to 400 called (one more launch,
+// for the plan, and the host's four tensors); one part of a page (15 MB) 7.2 us, two of them the launch.
 #include <algorithm>
 
 #include "common.cuh"

@@ -40,12 +40,14 @@
 // a softmax group ~1,250, most of them exponentials; the rest is the hand-over between them. From
 // one item's last P to the next one's first S ~4,500 cycles (O's division and stores 2,700).
 // Measured (16 query / 8 KV heads of 128): 16,384 tokens with a window of 2,048: 270 us, 955
-// TFLOP/s; 8,000 tokens without one: 234 us, 1,120; 1,024 queries over 8,192 positions: 76 us, 850
-// (140 us without the split); 24 ragged rows: 122 us; 77 queries of 4 heads of 64: 10 us. With one
+// TFLOP/s; 8,000 tokens without one: 234 us, 1,120; 1,024 queries over 8,192 positions: 73 us, 880
+// (140 us without the split); 24 ragged rows: 121 us; 77 queries of 4 heads of 64: 8 us. With one
 // item a block 302, -, 77, 147 and 10 us; items in turn with Q through registers 313 and 151 for
 // the first and the ragged rows (the loads' latency stood between two items: ~10,000 cycles), by
 // cp.async of the softmax warps 280 and 127. Tried and slower:
-// 128-key tiles with one S buffer each (1.9 times the time, issue-bound), S and P V issued by warps
+// 128-key tiles with one S buffer each (1.9 times the time, but of an early form whose products took
+// their operands from a thread's registers, which alone cost more than the products; with uniform
+// operands only 64 keys were measured), S and P V issued by warps
 // of their own (84 us on the second case), A's and B's exponentials taking turns (151), the
 // exponentials of a tile run beside the next one's maximum (182: S would have to be three
 // tiles ahead), no maximum but for tiles that leave the range (146 against 139); of the form with
@@ -395,7 +397,10 @@ __global__ void __launch_bounds__(kPreThreads, 1)
     // ---- items and copies -----------------------------------------------------------------
     // The KV head, row and 256 M rows of block bx: the last pairs (the longest) of every head first, so
     // that the last blocks to start are short (4,096 tokens from nothing: 106 us head after head, 76
-    // so). False: none.
+    // so; 8,000 282 and 234). That is longest first for one row; over a long cache, where all pairs
+    // are about as long, it costs a little (5,000 queries over 8,000 cached 427 us head after head,
+    // 449 so, 2,560 229 and 234), and so it does for batches of one pair a row (20 of 100 to 128
+    // tokens 19.1, 19.8). False: none.
     auto find = [&](int bx, PreBlock &b) {
       const int unit = bx / int(C), slot = x.pairs - 1 - unit / p.kv_heads;
       b.kvh = unit % p.kv_heads;
