@@ -144,3 +144,26 @@ def test_a_request_that_the_pool_can_never_hold_is_refused_first(yar, model):
     tokens = s.generate_batch([ids(3, 30), ids(4, 200)], smp, [1, 2], phase=None)[0]
     assert [len(t) for t in tokens] == [8, 8] and s.position(2) == 100
     s.close()
+
+
+def test_shared_pages_count_once_and_come_back(yar, model):
+    """Two rows that share pages, replaced by a request of both rows that needs the whole pool; one
+    that a third row shares stays that row's."""
+    smp, negative = sampling(yar, 8), ids(4, 150)
+    s = model.session(max_rows=3, max_ctx=512, page_tokens=64, pool_pages=6)
+    s.reset(0, 256), s.prefill(0, ids(1, 200), phase=None)
+    s.fork(0, 1, 256)  # 3 shared pages, 2 more: 1 is left
+    assert s.pages()[:2] == (6, 1)
+    got = s.generate(ids(3, 170), smp, 1, phase=None, negative=negative, cfg_scale=1.5)[0]  # 3 + 3 pages
+    assert len(got) == 8 and s.pages()[1] == 6
+    s.reset(0, 256), s.prefill(0, ids(1, 200), phase=None)
+    s.fork(0, 2, 200)
+    keep = s.kv(2, 1, 0, 200)
+    for call in (lambda: s.generate(ids(3, 170), smp, 1, phase=None),  # 3 pages, 2 can be had
+                 lambda: s.generate_batch([ids(3, 170)], smp, [1], phase=None)):
+        with pytest.raises(yar.YarError) as e:
+            call()
+        assert "exhausted" in e.value.message and s.position(0) == 200
+    assert len(s.generate(ids(3, 100), smp, 1, phase=None)[0]) == 8
+    np.testing.assert_array_equal(np.array(keep), np.array(s.kv(2, 1, 0, 200)))
+    s.close()
